@@ -172,8 +172,6 @@ int amdgo_asmlab_gemm_bf16(int v, const void* A, const void* Bt, void* C, int M,
     W4AP_CASE(131, 1, true)
     W4AP_CASE(132, 2, true)
     W4AP_CASE(133, 0, false)
-    W4AP_CASE(134, 3, true)
-    W4AP_CASE(135, 4, true)
     W4AP_CASE(136, 5, true)
     W4AP_CASE(137, 6, true)
     W4AP_CASE(138, 7, true)

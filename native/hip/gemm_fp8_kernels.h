@@ -266,8 +266,7 @@ gemm_fp8_256x256_w4s(const uint8_t* __restrict__ A, const uint8_t* __restrict__ 
 
 // q16: fp8 on the UNSCALED double-rate `v_mfma_f32_16x16x128_f8f6f4` (gfx950's f8f6f4 family runs
 // fp8 at twice the bf16 rate with or without the block scales; the older `*_fp8_fp8` forms are
-// the bf16-rate ones). hipBLASLt's gfx950 fp8 kernel (MT256x256x128, MI 16x16x128) is built on
-// it. The 16x16 output shape is also the one that holds clocks better under the power limit
+// the bf16-rate ones). The 16x16 output shape is also the one that holds clocks better under the power limit
 // (MI355X_MICROARCH.md, DVFS give-back item 7).
 // A wave's 128x128 sub-tile is 8x8 MFMAs of 16x16 (the bf16 w4s accumulator layout, so the bf16
 // epilogue applies as is). A fragment is 16 rows x 128 k = 32 B per lane (8 VGPRs, two

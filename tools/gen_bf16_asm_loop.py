@@ -64,12 +64,11 @@ def read_order(j: int):
     return False, j - 8
 
 
-def mfma(i: int, bout: bool = False, zero_c: bool = False) -> str:
-    """MFMA slot i: k-half i >> 6; A-outer (m = s >> 3, n = s & 7: the A fragment stays in srcB for
-    8 MFMAs) or B-outer (n = s >> 3, m = s & 7: the B fragment stays in srcA for 8 MFMAs). Each
-    accumulator m*8+n gets the same k sequence either way, so the results are identical."""
+def mfma(i: int, zero_c: bool = False) -> str:
+    """MFMA slot i: k-half i >> 6, A-outer (m = s >> 3, n = s & 7: the A fragment stays in srcB for
+    8 MFMAs)."""
     r, s = (0, i) if i < 64 else (1, i - 64)
-    m, n = (s & 7, s >> 3) if bout else (s >> 3, s & 7)
+    m, n = s >> 3, s & 7
     acc = m * 8 + n
     c = "0" if zero_c and r == 0 else f"a[{4 * acc}:{4 * acc + 3}]"     # zero_c: a tile's first k-half
     return (f"v_mfma_f32_16x16x32_bf16 a[{4 * acc}:{4 * acc + 3}], {frag_regs(r, True, n)}, "
@@ -79,9 +78,8 @@ def mfma(i: int, bout: bool = False, zero_c: bool = False) -> str:
 class Schedule:
     """Slot positions of one K-tile (see the module docstring)."""
 
-    def __init__(self, name, r1, w1, b1, dma, m0_lead, w2, b2, r0, vk, w3, bout=False):
+    def __init__(self, name, r1, w1, b1, dma, m0_lead, w2, b2, r0, vk, w3):
         self.name = name
-        self.bout = bout        # B-outer MFMA order (see mfma())
         self.r1 = r1            # slot of R1 read j (k-half 1 of tile t), j = 0..15
         self.w1, self.b1 = w1, b1   # lgkmcnt(0) slot, free barrier slot
         self.dma = dma          # slot of DMA piece p (p = 0..15)
@@ -99,7 +97,7 @@ class Schedule:
         return sum(1 for s in self.dma if s <= self.w2)
 
 
-def make(name, r1=(0, 1), dma=(19, 5), w2=79, r0=(81, 2), w3=126, vk=None, bout=False, w1_gap=1):
+def make(name, r1=(0, 1), dma=(19, 5), w2=79, r0=(81, 2), w3=126, vk=None, w1_gap=1):
     """A schedule from arithmetic progressions: R1 reads j at r1[0] + j*r1[1] (then lgkmcnt(0) and
     the free barrier right after the last one), DMA piece p at dma[0] + p*dma[1], the landing wait at
     w2 and its barrier at w2 + 1, R0 reads j at r0[0] + j*r0[1].
@@ -111,7 +109,7 @@ def make(name, r1=(0, 1), dma=(19, 5), w2=79, r0=(81, 2), w3=126, vk=None, bout=
     ds = [dma[0] + p * dma[1] for p in range(16)]
     r0s = [r0[0] + j * r0[1] for j in range(16)]
     sc = Schedule(name, r1=r1s, w1=w1, b1=w1 + 1, dma=ds, m0_lead=1, w2=w2, b2=None if w2 is None else w2 + 1, r0=r0s,
-                  vk=vk if vk is not None else ds[-1] + 2, w3=w3, bout=bout)
+                  vk=vk if vk is not None else ds[-1] + 2, w3=w3)
     validate(sc)
     return sc
 
@@ -147,9 +145,6 @@ SCHEDULES = {
     "v18_d6": make("v18_d6", dma=(19, 6), w2=98, r0=(100, 1)),
     "v18_d6b": make("v18_d6b", dma=(19, 6), w2=80, r0=(82, 2)),
     "v18_d5_late": make("v18_d5_late", w2=96, r0=(98, 1)),
-    # the same placements with the B fragment held in srcA across 8 MFMAs (hipBLASLt's order)
-    "v18_d6b_bout": make("v18_d6b_bout", dma=(19, 6), w2=80, r0=(82, 2), bout=True),
-    "v18_d5_late_bout": make("v18_d5_late_bout", w2=96, r0=(98, 1), bout=True),
     # the R1 reads' lgkmcnt(0) a few MFMAs after the last read (the LDS latency under the read
     # burst of all four waves), then the free barrier and the DMA
     "g4": make("g4", w1_gap=4, dma=(22, 5), w2=98, r0=(100, 1)),
@@ -168,8 +163,9 @@ SCHEDULES = {
 }
 
 
-# schedules the persistent kernel is generated for (its SC index = position here)
-PERSISTENT = ["v18", "v18_d6b", "v18_d5_late", "v18_d6b_bout", "v18_d5_late_bout", "g4", "g6", "g8", "sp2g6",
+# schedules the persistent kernel is generated for (its SC index = position here; None: a retired
+# schedule's index, left free so that the others keep theirs)
+PERSISTENT = ["v18", "v18_d6b", "v18_d5_late", None, None, "g4", "g6", "g8", "sp2g6",
               "g6d6", "g4d6", "g2d6", "sp2g4d5", "m4", "m4d4", "m4d3", "m6d4", "g4_rw", "g6d6_rw", "g4_zc",
               "g6d6_zc"]
 # a name ending in _zc: kloop_persistent_zc (first K-tile with src C = 0; frame EPI 8)
@@ -209,7 +205,7 @@ def body(sc: Schedule, cur: int, dma: bool, nx: bool, nxt_tile: bool = False, w2
         gap[i] += ops
     out = []
     for i in range(SLOTS):
-        out.append(mfma(i, sc.bout, zero_c))
+        out.append(mfma(i, zero_c))
         out += gap[i]
     return out
 
@@ -567,7 +563,6 @@ def body_ef(sc: Schedule, cur: int, dma: bool, nx: bool, nxt_tile: bool = False,
     """body() for the EF kernel: permuted B reads, optional src-C-zero first K-tile, extra landing-wait
     count, and (last) the fused epilogue with the spread-final MFMA order. Returns (lines, stores issued
     after the last DMA piece)."""
-    assert not sc.bout
     rA, rB, voff, kstep = ("%[nA]", "%[nB]", "%[nvoff]", "%[nkstep]") if nxt_tile else \
         ("%[rA]", "%[rB]", "%[voff]", "%[kstep]")
     nxt = 1 - cur
@@ -753,13 +748,15 @@ def render() -> str:
     parts.append("")
     parts.append("// " + ", ".join(f"{i} = {n}" for i, n in enumerate(SCHEDULES)))
     parts.append("")
-    psel = [f"if constexpr (SC == {i}) W4AP_LOOP(W4AP_ASM_{n.upper()});" for i, n in enumerate(PERSISTENT)]
+    psel = [f"if constexpr (SC == {i}) W4AP_LOOP(W4AP_ASM_{n.upper()});" for i, n in enumerate(PERSISTENT) if n]
     parts.append("// persistent kernel (gemm_bf16_256x256_w4ap): schedule index -> asm text")
     parts.append("#define W4AP_LOOP_SELECT(SC) \\")
     parts.append("  " + " else \\\n  ".join(psel))
-    parts.append("// " + ", ".join(f"{i} = {n}" for i, n in enumerate(PERSISTENT)))
+    parts.append("// " + ", ".join(f"{i} = {n}" for i, n in enumerate(PERSISTENT) if n))
     parts.append("// by name (the production dispatch refers to schedules this way)")
     for i, n in enumerate(PERSISTENT):
+        if n is None:
+            continue
         parts.append(f"#define W4AP_SC_{n.upper()} {i}")
     parts.append("")
     esel = [f"if constexpr (SC == {i}) W4EF_LOOP(W4EF_ASM_{n.upper()});" for i, n in enumerate(EF)]
@@ -808,7 +805,7 @@ def render() -> str:
             parts.append(f'  "{ln}\\n\\t" \\')
         parts.append('  ""')
         parts.append("")
-    for name in PERSISTENT:
+    for name in filter(None, PERSISTENT):
         lines = ap_lines(name)
         parts.append(f"#define W4AP_ASM_{name.upper()} \\")
         for ln in lines:
