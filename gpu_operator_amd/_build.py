@@ -62,8 +62,12 @@ class Target:
         srcs = [str(NATIVE_SRC / s) for s in self.sources]
         inc = [f"-I{NATIVE_SRC / 'include'}"]
         if self.kind.startswith("hip"):
+            # no packed fp32 VALU (v_pk_fma_f32 and its kin): hipcc makes them from plain float code, and
+            # some of their forms have given wrong results (its host pass does not know the feature
+            # and says so: harmless)
             base = [hipcc(), f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-Wall",
-                    "-Wno-unused-function", "-Wno-unused-result"] + inc
+                    "-Wno-unused-function", "-Wno-unused-result",
+                    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + inc
             if self.kind == "hip-shared":
                 base += ["-fPIC", "-shared"]
             else:
