@@ -96,12 +96,15 @@ def _pyext_name(stem: str) -> str:
 GEMM_HEADERS = ["include/gemm_tile_common.h", "hip/gemm_bf16_kernels.h", "hip/gemm_bf16_asm_loop.h",
                 "hip/gemm_fp8_kernels.h", "hip/gemm_fp8_asm_loop.h", "hip/gemm_w4ap.h", "hip/gemm_small.h",
                 "hip/gemm_small_host.h", "hip/gemm_raster_host.h"]
+GROUP_HEADERS = ["include/gemm_tile_common.h", "hip/group_common.h", "hip/group_tile.h"]
 LAB_HEADERS = GEMM_HEADERS + ["hip/gemm_bf16_asm_loop_lab.h", "hip/gemm_fp8_asm_loop_lab.h"]
 
 TARGETS: List[Target] = [
     # GPU compute: validator workloads (GEMM, smoke). Loaded via ctypes by ops/.
     Target("libamdgo_hip.so", ["hip/gemm_bf16.hip", "hip/gemm_fp8.hip", "hip/gemm_abft.hip", "hip/smoke.hip"], "hip-shared",
            headers=GEMM_HEADERS),
+    # Grouped and block-scaled matrix products and their quantiser. Loaded via ctypes by ops/.
+    Target("libamdgo_group.so", ["hip/gemm_group.hip", "hip/quant_block.hip"], "hip-shared", headers=GROUP_HEADERS),
     # Node agent library (sysfs/KFD topology, partitions, telemetry, inotify barriers).
     Target(_pyext_name("_amdnode"), ["node/pybind.cpp", "node/amdnode.cpp"], "pyext",
            headers=["include/amdnode.h"]),

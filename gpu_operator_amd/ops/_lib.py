@@ -1,6 +1,7 @@
-"""Loader for the in-tree HIP shared library (``_native/libamdgo_hip.so``).
+"""Loader for the in-tree HIP shared libraries: ``_native/libamdgo_hip.so`` (validator workloads) and
+``_native/libamdgo_group.so`` (grouped and block-scaled matrix products).
 
-The library is built by :mod:`gpu_operator_amd._build` for gfx950. On a machine with a GPU the
+The libraries are built by :mod:`gpu_operator_amd._build` for gfx950. On a machine with a GPU the
 ops refuse to fall back silently: if the library is missing they raise, so a GPU test can
 never pass on an eager PyTorch path by accident.
 """
@@ -16,6 +17,7 @@ from typing import Optional
 _NATIVE = Path(__file__).resolve().parent.parent / "_native"
 _LOCK = threading.Lock()
 _LIB: Optional[ctypes.CDLL] = None
+_GROUP_LIB: Optional[ctypes.CDLL] = None
 
 
 class NativeLibraryMissing(RuntimeError):
@@ -96,6 +98,47 @@ def load() -> ctypes.CDLL:
             getattr(lib, f).restype = i
         _LIB = lib
         return lib
+
+
+class GroupArgs(ctypes.Structure):
+    """``GroupArgs`` of native/hip/group_common.h: one grouped or block-scaled product."""
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("a", "b", "c", "a_scale", "b_scale", "offsets")]
+                + [(f, ctypes.c_longlong) for f in ("lda", "ldb", "ldc", "b_expert", "c_expert", "as_row", "as_k",
+                                                    "bs_expert", "bs_row", "bs_k")]
+                + [(f, ctypes.c_int) for f in ("rows", "cols", "red", "experts", "mode", "dtype", "scale", "zero_rest")])
+
+
+class QuantArgs(ctypes.Structure):
+    """``QuantArgs`` of native/hip/quant_block.hip: one quantisation by blocks."""
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("x", "q", "s")]
+                + [(f, ctypes.c_longlong) for f in ("ld", "batch_stride")]
+                + [(f, ctypes.c_int) for f in ("batches", "rows", "cols", "dtype", "block_rows", "e8")])
+
+
+def group_lib_path() -> Path:
+    return _NATIVE / "libamdgo_group.so"
+
+
+def load_group() -> ctypes.CDLL:
+    """The grouped / block-scaled products' library (like :func:`load`, it never falls back)."""
+    global _GROUP_LIB
+    if _GROUP_LIB is not None:
+        return _GROUP_LIB
+    with _LOCK:
+        if _GROUP_LIB is None:
+            p = group_lib_path()
+            if not p.exists():
+                raise NativeLibraryMissing(
+                    f"{p} not found: build it with `python -m gpu_operator_amd._build` (hipcc, gfx950)")
+            import torch  # noqa: F401  (its HIP runtime first: see load())
+
+            lib = ctypes.CDLL(str(p))
+            lib.amdgo_gemm_group.argtypes = [ctypes.POINTER(GroupArgs), ctypes.c_void_p]
+            lib.amdgo_gemm_group.restype = ctypes.c_int
+            lib.amdgo_quantize_fp8_block.argtypes = [ctypes.POINTER(QuantArgs), ctypes.c_void_p]
+            lib.amdgo_quantize_fp8_block.restype = ctypes.c_int
+            _GROUP_LIB = lib
+    return _GROUP_LIB
 
 
 def check(err: int, what: str) -> None:

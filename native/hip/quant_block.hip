@@ -1,0 +1,250 @@
+// fp8 e4m3 operands of the block-scaled products: one scale for each block of 128 columns of one row
+// (activations) or of 128 rows (weights).
+//
+//   amax = max |x| over the block's finite values, at least 448 * 2^-126
+//   float32 scale   s = amax / 448                              q = e4m3(x * 448 / amax)
+//   e8m0 scale      s = the least 2^e with amax <= 448 * 2^e    q = e4m3(x / s)
+//
+// e4m3() rounds the exact quotient to the nearest value, ties to even; 448 is e4m3's largest, so nothing
+// saturates. An infinity or NaN becomes NaN (e4m3 has no infinity) and leaves its block's scale alone.
+//
+// The quotient with a float32 scale is formed from x and amax brought to amax's binade, by a reciprocal
+// with an error of a few units in the last place. That can only change the e4m3 value where the quotient is
+// within that error of a border between two of them, and every border has 5 significant bits: those rare
+// values (the test below) are compared with the border exactly, in float64.
+//
+// Bound by the memory: 2 (4) bytes read and 1 written for each element.
+#include "gemm_tile_common.h"
+
+enum : int { kInBf16 = 0, kInFp16 = 1, kInFp32 = 2 };
+
+struct QuantArgs {
+  const void* x;
+  unsigned char* q;
+  void* s;
+  long long ld, batch_stride;      // elements
+  int batches, rows, cols;
+  int dtype, block_rows, e8;
+};
+
+namespace {
+
+typedef unsigned int qu4 __attribute__((ext_vector_type(4)));
+typedef unsigned int qu2 __attribute__((ext_vector_type(2)));
+
+constexpr int QT = 256;                // threads
+
+// 8 consecutive elements as loaded
+template <int DT>
+struct Raw8 {
+  static constexpr int W = DT == kInFp32 ? 8 : 4;
+  unsigned int w[W];
+};
+
+template <int DT>
+__device__ __forceinline__ float raw_get(const Raw8<DT>& r, int i) {
+  if constexpr (DT == kInFp32) return __builtin_bit_cast(float, r.w[i]);
+  const unsigned int h = (r.w[i >> 1] >> ((i & 1) * 16)) & 0xffff;
+  if constexpr (DT == kInBf16) return __builtin_bit_cast(float, h << 16);
+  return (float)__builtin_bit_cast(_Float16, (unsigned short)h);
+}
+
+// elements [c, c + 8) of a row, zeros from `cols` on; WIDE: whole and 16-byte aligned
+template <int DT>
+__device__ __forceinline__ Raw8<DT> raw_load(const char* row, int c, int cols, bool wide) {
+  constexpr int ES = DT == kInFp32 ? 4 : 2;
+  Raw8<DT> r;
+  if (wide && c + 8 <= cols) {
+    const qu4* p = (const qu4*)(row + (size_t)c * ES);
+#pragma unroll
+    for (int i = 0; i < Raw8<DT>::W / 4; ++i) {
+      const qu4 v = p[i];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) r.w[4 * i + k] = v[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw8<DT>::W; ++i) r.w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) {
+        if constexpr (ES == 4) r.w[i] = ((const unsigned int*)row)[c + i];
+        else r.w[i >> 1] |= (unsigned int)((const unsigned short*)row)[c + i] << ((i & 1) * 16);
+      }
+  }
+  return r;
+}
+
+// |x|'s bits where x is finite, else 0: ordered as the magnitudes are
+__device__ __forceinline__ unsigned int finite_bits(float x) {
+  const unsigned int b = __builtin_bit_cast(unsigned int, x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+constexpr unsigned int kLeastAmax = ((unsigned)(127 - 118) << 23) | 0x600000u;   // 448 * 2^-126 = 1.75 * 2^-118
+
+struct Scale {
+  float f;            // float32: the scale; e8m0: 2^e
+  int e;              // float32: amax's exponent; e8m0: e
+  float d, r;         // float32: amax * 2^-e in [1, 2) and 448 / d nearly
+};
+
+template <bool E8>
+__device__ __forceinline__ Scale make_scale(unsigned int amax) {
+  amax = max(amax, kLeastAmax);
+  Scale s;
+  if constexpr (E8) {
+    s.e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+    s.f = __builtin_bit_cast(float, (unsigned)(s.e + 127) << 23);
+    s.d = s.r = 0.f;
+  } else {
+    s.f = __builtin_bit_cast(float, amax) / 448.0f;
+    s.e = (int)(amax >> 23) - 127;
+    s.d = __builtin_bit_cast(float, (amax & 0x7fffffu) | 0x3f800000u);
+    s.r = 448.0f * __builtin_amdgcn_rcpf(s.d);
+  }
+  return s;
+}
+
+template <bool E8>
+__device__ __forceinline__ float quotient(float x, const Scale& s) {
+  const float xs = ldexpf(x, -s.e);           // exact wherever the result does not round to zero
+  float y;
+  if constexpr (E8) {
+    y = xs;
+  } else {
+    y = xs * s.r;                              // within 4 units in the last place of 448 x / amax
+    const unsigned int b = __builtin_bit_cast(unsigned int, y);
+    if (((b + 8) & 0x7ffffu) < 16) {           // maybe a border: compare with it exactly
+      const unsigned int tb = (b + 8) & ~0x7ffffu;
+      const double t = (double)__builtin_bit_cast(float, tb) * (double)s.d, n = 448.0 * (double)xs;
+      const double at = fabs(t), an = fabs(n);
+      y = __builtin_bit_cast(float, tb + (an > at ? 1u : an < at ? 0xffffffffu : 0u));
+    }
+  }
+  return finite_bits(x) == 0 && x != 0.f ? __builtin_nanf("") : y;
+}
+
+template <int DT, bool E8>
+__device__ __forceinline__ qu2 quantize8(const Raw8<DT>& r, const Scale& s) {
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = quotient<E8>(raw_get<DT>(r, i), s);
+  qu2 o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h], y[4 * h + 1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * h + 2], y[4 * h + 3], w, true);
+    o[h] = (unsigned)w;
+  }
+  return o;
+}
+
+__device__ __forceinline__ void store8(unsigned char* row, int c, int cols, bool wide, qu2 v) {
+  if (wide && c + 8 <= cols) {
+    *(qu2*)(row + c) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < cols) row[c + i] = (unsigned char)(v[i >> 2] >> ((i & 3) * 8));
+  }
+}
+
+template <bool E8>
+__device__ __forceinline__ void store_scale(void* s, size_t at, const Scale& v) {
+  if constexpr (E8) ((unsigned char*)s)[at] = (unsigned char)(v.e + 127);
+  else ((float*)s)[at] = v.f;
+}
+
+template <int DT>
+__device__ __forceinline__ unsigned int amax8(const Raw8<DT>& r) {
+  unsigned int m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, finite_bits(raw_get<DT>(r, i)));
+  return m;
+}
+
+// One row's block a quarter wave: 16 lanes of 8 elements; a wave takes 4 blocks of one row.
+template <int DT, bool E8>
+__global__ void __launch_bounds__(QT) quantize_row_blocks(const QuantArgs a) {
+  constexpr int ES = DT == kInFp32 ? 4 : 2;
+  const int lane = threadIdx.x & 63, kb_count = (a.cols + 127) / 128, per_row = (kb_count + 3) / 4;
+  const long long id = (long long)blockIdx.x * (QT / 64) + (threadIdx.x >> 6);
+  const long long row = id / per_row;
+  if (row >= (long long)a.batches * a.rows) return;
+  const int kb = (int)(id - row * per_row) * 4 + (lane >> 4);
+  const int batch = (int)(row / a.rows), r = (int)(row - (long long)batch * a.rows);
+  const char* x = (const char*)a.x + ((size_t)batch * a.batch_stride + (size_t)r * a.ld) * ES;
+  const bool wide_in = (((uintptr_t)a.x | (uintptr_t)(a.ld * ES) | (uintptr_t)(a.batch_stride * ES)) & 15) == 0;
+  const bool wide_out = (((uintptr_t)a.q | (uintptr_t)a.cols) & 7) == 0;
+  const int c = kb * 128 + (lane & 15) * 8;
+  const Raw8<DT> v = raw_load<DT>(x, c, a.cols, wide_in);
+  unsigned int m = amax8<DT>(v);
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+  if (kb >= kb_count) return;
+  const Scale s = make_scale<E8>(m);
+  store8(a.q + (size_t)row * a.cols, c, a.cols, wide_out, quantize8<DT, E8>(v, s));
+  if ((lane & 15) == 0) store_scale<E8>(a.s, (size_t)row * kb_count + kb, s);
+}
+
+// A block of 128 rows a workgroup: thread t holds chunk t & 15 of rows t / 16 + 16 i.
+template <int DT, bool E8>
+__global__ void __launch_bounds__(QT) quantize_square_blocks(const QuantArgs a) {
+  constexpr int ES = DT == kInFp32 ? 4 : 2;
+  __shared__ unsigned int part[QT / 64];
+  const int kb_count = (a.cols + 127) / 128, rb_count = (a.rows + 127) / 128;
+  const int kb = blockIdx.x % kb_count;
+  const int rest = blockIdx.x / kb_count, rb = rest % rb_count, batch = rest / rb_count;
+  const char* x = (const char*)a.x + (size_t)batch * a.batch_stride * ES;
+  const bool wide_in = (((uintptr_t)a.x | (uintptr_t)(a.ld * ES) | (uintptr_t)(a.batch_stride * ES)) & 15) == 0;
+  const bool wide_out = (((uintptr_t)a.q | (uintptr_t)a.cols) & 7) == 0;
+  const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
+  Raw8<DT> v[8];
+  unsigned int m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i;
+    v[i] = raw_load<DT>(x + (size_t)(r < a.rows ? r : 0) * a.ld * ES, c, r < a.rows ? a.cols : 0, wide_in);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, amax8<DT>(v[i]));
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+  __syncthreads();
+  m = max(max(part[0], part[1]), max(part[2], part[3]));
+  const Scale s = make_scale<E8>(m);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int r = r0 + 16 * i;
+    if (r < a.rows) store8(a.q + ((size_t)batch * a.rows + r) * a.cols, c, a.cols, wide_out, quantize8<DT, E8>(v[i], s));
+  }
+  if (threadIdx.x == 0) store_scale<E8>(a.s, blockIdx.x, s);
+}
+
+template <int DT, bool E8>
+int launch_quant(const QuantArgs& a, hipStream_t s) {
+  const long long kb = ((long long)a.cols + 127) / 128;
+  const long long grid = a.block_rows == 1 ? ((long long)a.batches * a.rows * ((kb + 3) / 4) + QT / 64 - 1) / (QT / 64)
+                                           : a.batches * (((long long)a.rows + 127) / 128) * kb;
+  if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
+  if (a.block_rows == 1) hipLaunchKernelGGL((quantize_row_blocks<DT, E8>), dim3((unsigned)grid), dim3(QT), 0, s, a);
+  else hipLaunchKernelGGL((quantize_square_blocks<DT, E8>), dim3((unsigned)grid), dim3(QT), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" int amdgo_quantize_fp8_block(const QuantArgs* args, hipStream_t s) {
+  if (!args) return (int)hipErrorInvalidValue;
+  const QuantArgs& a = *args;
+  if (a.batches < 0 || a.rows < 0 || a.cols < 0 || (a.block_rows != 1 && a.block_rows != 128)) return (int)hipErrorInvalidValue;
+  if (a.batches == 0 || a.rows == 0 || a.cols == 0) return 0;
+  switch (a.dtype) {
+    case kInBf16: return a.e8 ? launch_quant<kInBf16, true>(a, s) : launch_quant<kInBf16, false>(a, s);
+    case kInFp16: return a.e8 ? launch_quant<kInFp16, true>(a, s) : launch_quant<kInFp16, false>(a, s);
+    case kInFp32: return a.e8 ? launch_quant<kInFp32, true>(a, s) : launch_quant<kInFp32, false>(a, s);
+  }
+  return (int)hipErrorInvalidValue;
+}

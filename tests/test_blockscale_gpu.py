@@ -1,0 +1,237 @@
+"""The block quantiser and the block-scaled fp8 products against a 64-bit plain form."""
+
+import pytest
+import torch
+
+import group_helpers as H
+
+pytestmark = pytest.mark.gpu
+
+SCALES = [torch.float32, torch.float8_e8m0fnu]
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def _same_codes(q, want):
+    """Equal values, NaN where NaN is due, and the sign of zeros."""
+    got = q.double()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    bad = (got != want) & ~torch.isnan(want)
+    assert not bad.any(), (int(bad.sum()), got[bad][:4].tolist(), want[bad][:4].tolist())
+
+
+def _check_quantized(x, block_rows, scale_dtype):
+    from gpu_operator_amd.ops import blockscale as B
+
+    q, s = B.quantize_fp8_block(x, block_rows, scale_dtype=scale_dtype)
+    want, sw = H.quantize64(x, block_rows, scale_dtype != torch.float32)
+    assert s.dtype == scale_dtype and s.shape == sw.shape
+    # the scale is the 64-bit quotient rounded once to float32 (half a step), or the power of two itself
+    assert ((s.float().double() - sw).abs() <= (0.0 if scale_dtype != torch.float32 else 2.0 ** -24) * sw).all()
+    _same_codes(q, want)
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 128), (3, 127), (5, 129), (17, 1000), (128, 512), (130, 257), (300, 640), (257, 2056)])
+def test_quantize(cuda_device, rows, cols, block_rows, dtype, scale_dtype):
+    g = torch.Generator(device=cuda_device).manual_seed(rows * 7 + cols)
+    x = torch.randn((rows, cols), generator=g, device=cuda_device)
+    x = x * torch.exp(4 * torch.randn((rows, 1), generator=g, device=cuda_device)).clamp(1e-3, 1e3)
+    _check_quantized(x.to(dtype), block_rows, scale_dtype)
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("dtype", TYPES)
+def test_quantize_borders(cuda_device, dtype, scale_dtype):
+    """Quotients on and next to the borders between two e4m3 values, for many amax: ties go to the even one."""
+    rows = []
+    for seed in range(512):
+        g = torch.Generator().manual_seed(seed)
+        amax = (torch.rand(1, generator=g) * 3 + 0.01).to(dtype).double()
+        mid = (torch.randint(16, 32, (126,), generator=g).double() + 0.5) / 16 * 2.0 ** torch.randint(-9, 8, (126,), generator=g)
+        v = (mid.clamp_max(1.0 * 448) * amax / 448).to(dtype).double()
+        v = v + torch.randint(-1, 2, (126,), generator=g) * v * torch.finfo(dtype).eps
+        rows.append(torch.cat([amax, torch.minimum(v, amax), torch.zeros(1, dtype=torch.float64)]).to(dtype))
+    _check_quantized(torch.stack(rows).to(cuda_device), 1, scale_dtype)
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_extremes(cuda_device, block_rows, scale_dtype):
+    """Zeros, the least and the largest values, infinities and NaN: they are NaN and leave their block's scale alone."""
+    x = torch.randn((256, 384), generator=torch.Generator().manual_seed(2)).to(cuda_device)
+    x[:128, :128] = 0.0
+    x[:128, 128:256] *= 1e-38
+    x[:128, 256:] *= 1e38
+    x[130, 5], x[131, 6], x[132, 140] = float("inf"), float("nan"), float("-inf")
+    x[140, 256:] = float("nan")
+    x[0, 130] = 1e-45
+    _check_quantized(x, block_rows, scale_dtype)
+    _check_quantized(x.bfloat16(), block_rows, scale_dtype)
+
+
+def test_quantize_strides_batches_and_outputs(cuda_device):
+    from gpu_operator_amd.ops import blockscale as B
+
+    g = torch.Generator(device=cuda_device).manual_seed(1)
+    x = torch.randn((3, 200, 300), generator=g, device=cuda_device).bfloat16()
+    for br in (1, 128):
+        q, s = B.quantize_fp8_block(x, br)
+        for i in range(3):
+            qi, si = B.quantize_fp8_block(x[i], br)
+            assert torch.equal(q[i].view(torch.uint8), qi.view(torch.uint8)) and torch.equal(s[i], si)
+        wide = torch.full((3, 201, 331), float("nan"), dtype=torch.bfloat16, device=cuda_device)
+        view = wide[:, 1:, 7:307]
+        view.copy_(x)
+        out, scale_out = torch.empty_like(q), torch.empty_like(s)
+        q2, s2 = B.quantize_fp8_block(view, br, out=out, scale_out=scale_out)
+        assert q2 is out and s2 is scale_out
+        assert torch.equal(q.view(torch.uint8), out.view(torch.uint8)) and torch.equal(s, scale_out)
+    assert B.quantize_fp8_block(x[:, :0])[0].shape == (3, 0, 300)
+
+
+def _operands(dev, m, n, k, scale_dtype, e=0, seed=0):
+    """Random codes (all of them but NaN) and scales over several binades."""
+    g = torch.Generator(device=dev).manual_seed(seed + 3 * m + 5 * n + 7 * k)
+
+    def codes(*shape):
+        c = torch.randint(0, 256, shape, generator=g, device=dev, dtype=torch.int32)
+        return torch.where((c & 0x7F) == 0x7F, c ^ 1, c).to(torch.uint8).view(torch.float8_e4m3fn)
+
+    def scales(*shape):
+        s = torch.exp2(torch.randint(-12, 3, shape, generator=g, device=dev).float())
+        if scale_dtype == torch.float32:
+            return s * (1 + torch.rand(shape, generator=g, device=dev))
+        return s.to(scale_dtype)
+
+    kb, nb = -(-k // 128), -(-n // 128)
+    lead = (e,) if e else ()
+    return codes(m, k), scales(m, kb), codes(*lead, n, k), scales(*lead, nb, kb)
+
+
+GEMMS = [(1, 1, 1), (1, 128, 128), (3, 17, 16), (16, 256, 1024), (17, 130, 144), (33, 100, 257), (64, 640, 384), (127, 129, 127),
+         (128, 256, 512), (200, 384, 1000), (257, 512, 640), (300, 264, 2064), (1, 1000, 4096), (512, 512, 1)]
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("m,n,k", GEMMS)
+def test_gemm(cuda_device, m, n, k, scale_dtype):
+    from gpu_operator_amd.ops import blockscale as B
+
+    a, sa, bt, sb = _operands(cuda_device, m, n, k, scale_dtype)
+    x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
+    H.check(B.gemm_fp8_block(a, sa, bt, sb), x @ w.t(), x.abs() @ w.abs().t(), k + 3 * -(-k // 128),
+            H.fp8_slack(x, w))
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("sizes,n,k", [([1], 16, 128), ([0, 3, 0, 1], 40, 136), ([1, 2] * 30, 256, 256), ([16, 17, 0, 15], 130, 70),
+                                       ([127, 0, 128, 129], 384, 512), ([300, 5], 520, 1040)])
+def test_grouped_gemm(cuda_device, sizes, n, k, scale_dtype):
+    from gpu_operator_amd.ops import blockscale as B
+
+    tail = 4
+    a, sa, bt, sb = _operands(cuda_device, sum(sizes) + tail, n, k, scale_dtype, e=len(sizes))
+    a[-tail:] = float("nan")
+    off = H.offsets_of(sizes, device=cuda_device)
+    x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
+    ref, mag = H.forward64(x, w, off)
+    got = B.gemm_grouped_fp8_block(a, sa, bt, sb, off)
+    H.check(got, ref, mag, k + 3 * -(-k // 128), H.grouped_fp8_slack(x, w, off))
+    out = torch.full_like(got, 5.0)
+    B.gemm_grouped_fp8_block(a, sa, bt, sb, off, out)
+    assert torch.equal(out[:-tail], got[:-tail]) and (out[-tail:] == 5.0).all()
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+def test_strided_operands_and_scales(cuda_device, scale_dtype):
+    """Row strides off 16 bytes, scales stored column by column or apart: the packed operands' bits."""
+    from gpu_operator_amd.ops import blockscale as B
+
+    a, sa, bt, sb = _operands(cuda_device, 150, 272, 400, scale_dtype)
+    want = B.gemm_fp8_block(a, sa, bt, sb)
+
+    def apart(x, pad, lead):
+        flat = torch.empty(lead + x.shape[0] * (x.shape[1] + pad), dtype=torch.uint8, device=x.device).fill_(0x7F)
+        v = flat[lead:].view(x.shape[0], x.shape[1] + pad)[:, : x.shape[1]]
+        v.copy_(x.view(torch.uint8))
+        return v.view(torch.float8_e4m3fn)
+
+    def columns(s):
+        u = s.view(torch.uint8) if scale_dtype != torch.float32 else s
+        return (u.t().contiguous().t()).view(scale_dtype)
+
+    for pad, lead in ((16, 0), (1, 0), (0, 3), (48, 16)):
+        assert torch.equal(B.gemm_fp8_block(apart(a, pad, lead), columns(sa), apart(bt, pad, lead), columns(sb)), want)
+    out = torch.zeros((150, 300), dtype=torch.bfloat16, device=cuda_device)
+    B.gemm_fp8_block(a, sa, bt, sb, out[:, 5:277])
+    assert torch.equal(out[:, 5:277], want) and (out[:, :5] == 0).all() and (out[:, 277:] == 0).all()
+
+
+def test_a_nan_stays_in_its_row(cuda_device):
+    from gpu_operator_amd.ops import blockscale as B
+
+    a, sa, bt, sb = _operands(cuda_device, 70, 200, 300, torch.float32)
+    want = B.gemm_fp8_block(a, sa, bt, sb)
+    a.view(torch.uint8)[7, 299] = 0x7F
+    sa[9, 1] = float("nan")
+    got = B.gemm_fp8_block(a, sa, bt, sb)
+    keep = [r for r in range(70) if r not in (7, 9)]
+    assert torch.isnan(got[[7, 9]]).all() and torch.equal(got[keep], want[keep])
+
+
+def test_power_of_two_scales_are_float32_ones(cuda_device):
+    """The same powers of two in either type stand for the same operands; only the sums' roundings may differ."""
+    from gpu_operator_amd.ops import blockscale as B
+
+    a, sa, bt, sb = _operands(cuda_device, 130, 256, 512, torch.float8_e8m0fnu)
+    x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
+    for s, t in ((sa, sb), (sa.float(), sb.float())):
+        H.check(B.gemm_fp8_block(a, s, bt, t), x @ w.t(), x.abs() @ w.abs().t(), 512 + 12, H.fp8_slack(x, w))
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+def test_serving_path(cuda_device, scale_dtype):
+    """As a server runs them: weights quantised once, activations per step, two grouped products with a gate between
+    them, in a graph that is replayed over new tokens."""
+    from gpu_operator_amd.ops import blockscale as B
+
+    e, h, f, t = 6, 256, 384, 40
+    g = torch.Generator(device=cuda_device).manual_seed(0)
+    w1 = torch.randn((e, 2 * f, h), generator=g, device=cuda_device) * h ** -0.5
+    w2 = torch.randn((e, h, f), generator=g, device=cuda_device) * f ** -0.5
+    q1, s1 = B.quantize_fp8_block(w1, 128, scale_dtype=scale_dtype)
+    q2, s2 = B.quantize_fp8_block(w2, 128, scale_dtype=scale_dtype)
+    x = torch.zeros((t, h), dtype=torch.bfloat16, device=cuda_device)
+    off = torch.zeros(e + 1, dtype=torch.int32, device=cuda_device)
+
+    def step():
+        qx, sx = B.quantize_fp8_block(x, scale_dtype=scale_dtype)
+        up = B.gemm_grouped_fp8_block(qx, sx, q1, s1, off)
+        y = torch.nn.functional.silu(up[:, :f]) * up[:, f:]
+        qy, sy = B.quantize_fp8_block(y, scale_dtype=scale_dtype)
+        return up, y, B.gemm_grouped_fp8_block(qy, sy, q2, s2, off)
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        up, y, out = step()
+    for seed in range(4):
+        x.copy_(torch.randn((t, h), generator=g, device=cuda_device))
+        off.copy_(H.offsets_of(H.random_sizes(t - seed, e, seed, empty=(seed,)), device=cuda_device))
+        graph.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip((up, y, out), eager))
+        # each product against 64 bits on the operands it was given
+        vx, sv = H.quantize64(x, 1, scale_dtype != torch.float32)
+        x64 = vx * sv.float().double().repeat_interleave(128, 1)[:, :h]
+        w64 = H.dequantize64(q1, s1, 128)
+        ref, mag = H.forward64(x64, w64, off)
+        H.check(up, ref, mag, h + 6, H.grouped_fp8_slack(x64, w64, off))
+        vy, sv = H.quantize64(y, 1, scale_dtype != torch.float32)
+        y64 = vy * sv.float().double().repeat_interleave(128, 1)[:, :f]
+        w64 = H.dequantize64(q2, s2, 128)
+        ref, mag = H.forward64(y64, w64, off)
+        H.check(out, ref, mag, f + 9, H.grouped_fp8_slack(y64, w64, off))
