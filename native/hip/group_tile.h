@@ -1,36 +1,46 @@
-// The tiled kernel of the grouped products: a BM x BN output tile per workgroup, WM x WN waves, operand panels
-// of 128 bytes along the reduction (64 elements of 16 bits, 128 of fp8: one scale block) staged through LDS.
+// The tiled kernels of the grouped products: a BM x BN output tile per workgroup, WM x WN waves, operand panels
+// of PB bytes along the reduction (128: 64 elements of 16 bits, or 128 of fp8, one scale block) staged through
+// LDS.
 #pragma once
 
 #include "group_common.h"
 
-template <int DT_, int SC_, bool ATR_, bool BTR_, int BM_, int BN_, int WM_, int WN_>
+template <int DT_, int SC_, bool ATR_, bool BTR_, int BM_, int BN_, int WM_, int WN_, int PB_ = 128, int NBUF_ = 1>
 struct TileCfg {
   static constexpr int DT = DT_, SC = SC_, BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr bool ATR = ATR_, BTR = BTR_;
   static constexpr int ES = DT == kFp8 ? 1 : 2;          // bytes an element
-  static constexpr int KT = 128 / ES;                     // reduction steps a panel
+  static constexpr int PB = PB_, NBUF = NBUF_;            // bytes a panel is wide; panels in the ring
+  static constexpr int KT = PB / ES;                      // reduction steps a panel
   static constexpr int THREADS = 64 * WM * WN;
   static constexpr int TM = BM / WM, TN = BN / WN;        // a wave's part
   static constexpr int NI = TM / 16, NJ = TN / 16;
-  static constexpr int OPA = BM * 128, OPB = BN * 128;    // bytes of a panel
-  static constexpr int SCB = SC == kScaleNone ? 0 : (BM + 4) * 4;
+  static constexpr int OPA = BM * PB, OPB = BN * PB;      // bytes of a panel
+  static constexpr int SCB = SC == kScaleNone ? 0 : THREADS * 4;
+
   static constexpr int STAGE = OPA + OPB + SCB;
+  static constexpr int LDS = NBUF * STAGE;
+  static_assert(LDS <= 160 * 1024, "one CU's LDS");
+  static constexpr int EU = WM * WN / 4 * (160 * 1024 / LDS >= 2 ? 2 : 1);   // waves a SIMD that the ring leaves room for
   static_assert(!(DT == kFp8 && (ATR || BTR)), "fp8 operands are K-major");
   static_assert((DT == kFp8) == (SC != kScaleNone), "fp8 has scales");
+  static_assert(PB == 128 || (PB == 64 && DT != kFp8), "an fp8 panel is one scale block");
 };
 
-// Byte of 16-byte chunk q of row r in a K-major panel: rows of 128 bytes, chunks permuted by the row so that
+// Byte of 16-byte chunk q of row r in a K-major panel: rows of PB bytes, chunks permuted by the row so that
 // the fragment reads (16 rows, one chunk) spread over the banks.
-__device__ __forceinline__ int km_at(int r, int q) { return r * 128 + ((q ^ (r & 7)) << 4); }
+template <int PB>
+__device__ __forceinline__ int km_swizzle(int r) { return PB == 128 ? r & 7 : (r >> 1) & 3; }
+template <int PB>
+__device__ __forceinline__ int km_at(int r, int q) { return r * PB + ((q ^ km_swizzle<PB>(r)) << 4); }
 
 // Byte of 16-byte chunk q of row r in a reduction-major panel of W columns (2 W bytes a row): 32-byte slots
 // permuted by the row. A transposing read takes 16 columns (one slot) of rows 8 g + 4 h + 0..3, so the rows
 // that one read touches together are told apart by r & 3 and by bit 3 of r.
+__device__ __forceinline__ int rm_swizzle(int r) { return (r & 3) | (((r >> 3) & 1) << 2); }
 template <int W>
 __device__ __forceinline__ int rm_at(int r, int q) {
-  const int f = (r & 3) | (((r >> 3) & 1) << 2);
-  return r * (2 * W) + (((q >> 1) ^ f) << 5) + ((q & 1) << 4);
+  return r * (2 * W) + (((q >> 1) ^ rm_swizzle(r)) << 5) + ((q & 1) << 4);
 }
 
 // 16 bytes of a row from element `from`, elements at or past `upto` as zeros; any alignment.
@@ -67,7 +77,7 @@ struct TileOperands {
   const char* bs;
 };
 
-// One reduction step of 128 bytes: acc += A panel x B panel^T (fp8: times the scales of the panel's block).
+// One panel: acc += A panel x B panel^T (fp8: times the scales of the panel's block).
 template <class C>
 __device__ __forceinline__ void tile_compute(const char* lds, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
   const int lane = threadIdx.x & 63, j16 = lane & 15, g = lane >> 4;
@@ -78,7 +88,7 @@ __device__ __forceinline__ void tile_compute(const char* lds, int wm, int wn, gf
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) {
       const int r = wn * C::TN + j * 16 + j16;
-      const gi4 x = *(const gi4*)(lb + km_at(r, g)), y = *(const gi4*)(lb + km_at(r, g + 4));
+      const gi4 x = *(const gi4*)(lb + km_at<C::PB>(r, g)), y = *(const gi4*)(lb + km_at<C::PB>(r, g + 4));
       bf[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     }
     const char* ls = lds + C::OPA + C::OPB;
@@ -87,7 +97,7 @@ __device__ __forceinline__ void tile_compute(const char* lds, int wm, int wn, gf
 #pragma unroll
       for (int i = 0; i < C::NI; ++i) {
         const int r = wm * C::TM + i * 16 + j16;
-        const gi4 x = *(const gi4*)(la + km_at(r, g)), y = *(const gi4*)(la + km_at(r, g + 4));
+        const gi4 x = *(const gi4*)(la + km_at<C::PB>(r, g)), y = *(const gi4*)(la + km_at<C::PB>(r, g + 4));
         const gi8 af = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         const float s = *(const float*)(ls + r * 4) * sb;
 #pragma unroll
@@ -102,7 +112,7 @@ __device__ __forceinline__ void tile_compute(const char* lds, int wm, int wn, gf
 #pragma unroll
       for (int i = 0; i < C::NI; ++i) {
         const int r = wm * C::TM + i * 16 + j16;
-        const gi4 x = *(const gi4*)(la + km_at(r, g)), y = *(const gi4*)(la + km_at(r, g + 4));
+        const gi4 x = *(const gi4*)(la + km_at<C::PB>(r, g)), y = *(const gi4*)(la + km_at<C::PB>(r, g + 4));
         const gi8 af = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
         const int sa = *(const int*)(ls + r * 4);
 #pragma unroll
@@ -121,13 +131,13 @@ __device__ __forceinline__ void tile_compute(const char* lds, int wm, int wn, gf
         const gi2 l2 = __builtin_bit_cast(gi2, lo), h2 = __builtin_bit_cast(gi2, hi);
         return gi4{l2[0], l2[1], h2[0], h2[1]};
       } else {
-        return *(const gi4*)(base + km_at(row0 + j16, s * 4 + g));
+        return *(const gi4*)(base + km_at<C::PB>(row0 + j16, s * 4 + g));
       }
     };
     constexpr std::integral_constant<int, C::ATR ? C::BM : 0> ta;
     constexpr std::integral_constant<int, C::BTR ? C::BN : 0> tb;
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < C::PB / 64; ++s) {
       gi4 bf[C::NJ];
 #pragma unroll
       for (int j = 0; j < C::NJ; ++j) bf[j] = frag(tb, lb, wn * C::TN + j * 16, s);
@@ -162,11 +172,12 @@ __device__ __forceinline__ void stage_regs(char* lds, const char* base, long lon
       *(gi4*)(lds + rm_at<ROWS>(r, q)) = v;
     }
   } else {
-    for (int i = threadIdx.x; i < ROWS * 8; i += C::THREADS) {
-      const int r = i >> 3, q = i & 7;
+    constexpr int CPR = C::PB / 16;
+    for (int i = threadIdx.x; i < ROWS * CPR; i += C::THREADS) {
+      const int r = i / CPR, q = i % CPR;
       gi4 v = {0, 0, 0, 0};
       if (r < rows) v = load_chunk<ES>(base + (size_t)r * ld_b, kt * C::KT + q * (16 / ES), red);
-      *(gi4*)(lds + km_at(r, q)) = v;
+      *(gi4*)(lds + km_at<C::PB>(r, q)) = v;
     }
   }
 }
@@ -268,6 +279,161 @@ __device__ __forceinline__ void tile_store(const GroupArgs& g, char* c_tile, int
       }
     }
   }
+}
+
+// What an LDS-DMA lane that has nothing to load asks for: past every buffer's end, so it gets zeros.
+constexpr unsigned kNowhere = 0x80000000u;
+
+typedef __attribute__((address_space(3))) void* g_lds_ptr;
+
+// One operand's panels by LDS-DMA (buffer_load ... lds): a wave instruction fills 1 KiB of LDS in lane order,
+// so the permutation of the chunks goes on the addresses that the lanes read. Each lane keeps the offsets of its
+// pieces; the panel's place is the descriptor's base. Rows or columns that do not exist, and in the last panel
+// the reduction steps past the end, are offsets past the buffer: zeros, whatever lies there.
+template <class C, bool TR, int ROWS>
+struct PanelDma {
+  static constexpr int WAVES = C::THREADS / 64;
+  static constexpr int PIECES = ROWS * C::PB / 1024 / WAVES;
+  static_assert(PIECES * WAVES * 1024 == ROWS * C::PB, "whole pieces");
+  unsigned off[PIECES];
+
+  __device__ __forceinline__ static int row_of(int piece, int wave, int lane) {
+    if constexpr (TR) return (piece * WAVES + wave) * (1024 / (2 * ROWS)) + lane / (ROWS / 8);
+    else return (piece * WAVES + wave) * (1024 / C::PB) + lane / (C::PB / 16);
+  }
+  // the 16-byte chunk of its row that the lane reads
+  __device__ __forceinline__ static int chunk_of(int row, int lane) {
+    if constexpr (TR) {
+      const int q = lane % (ROWS / 8);
+      return (((q >> 1) ^ rm_swizzle(row)) << 1) | (q & 1);
+    } else {
+      return (lane % (C::PB / 16)) ^ km_swizzle<C::PB>(row);
+    }
+  }
+  __device__ __forceinline__ void init(int wave, int lane, unsigned ld, int rows, int col0, int cols) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int r = row_of(i, wave, lane), q = chunk_of(r, lane);
+      if constexpr (TR) off[i] = col0 + q * 8 < cols ? (unsigned)r * ld + (unsigned)(col0 + q * 8) * 2 : kNowhere;
+      else off[i] = r < rows ? (unsigned)r * ld + q * 16 : kNowhere;
+    }
+  }
+  // the last panel: `left` reduction steps of it exist
+  __device__ __forceinline__ void cut(int wave, int lane, int left) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int r = row_of(i, wave, lane);
+      if constexpr (TR) off[i] = r < left ? off[i] : kNowhere;
+      else off[i] = chunk_of(r, lane) * 16 < left * C::ES ? off[i] : kNowhere;
+    }
+  }
+  __device__ __forceinline__ void load(char* lds, const char* panel, int wave) const {
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)panel, 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (g_lds_ptr)(lds + (i * WAVES + wave) * 1024), 16, off[i], 0, 0, 0);
+  }
+};
+
+template <int N>
+__device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// One panel's work: the next panel's DMA goes into `into` while `from` is multiplied. Two pointers that do not
+// alias, so that the compiler puts no wait for the DMA before the fragment reads.
+template <class C, class F>
+__device__ __forceinline__ void tile_step(char* __restrict__ into, const char* __restrict__ from, int wm, int wn,
+                                          gf4 (&acc)[C::NI][C::NJ], F&& issue) {
+  issue(into);
+  tile_compute<C>(from, wm, wn, acc);
+}
+
+// The same tile with its panels in a ring of NBUF, NBUF - 1 of them in flight. At panel t a counted wait
+// retires t's pieces only, a bare s_barrier publishes them, and panel t + NBUF - 1 goes into the buffer that
+// every wave left at t - 1.
+template <class C>
+__global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::EU, C::EU)))
+group_tile_dma(const GroupArgs g) {
+  __shared__ __attribute__((aligned(16))) char lds[C::LDS];     // the only LDS object: see tile_step
+  zero_rest_rows(g, g.cols, blockIdx.x, gridDim.x, C::THREADS);
+  TileOperands t;
+  char* c_tile;
+  int c_rows, c_cols;
+  if (!tile_setup<C>(g, blockIdx.x, t, c_tile, c_rows, c_cols)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WN, wn = wave % C::WN;
+  using DmaA = PanelDma<C, C::ATR, C::BM>;
+  using DmaB = PanelDma<C, C::BTR, C::BN>;
+  DmaA da;
+  DmaB db;
+  da.init(wave, lane, (unsigned)t.lda_b, t.a_rows, t.a_col0, t.a_cols);
+  db.init(wave, lane, (unsigned)t.ldb_b, t.b_rows, t.b_col0, t.b_cols);
+  const size_t step_a = C::ATR ? (size_t)C::KT * t.lda_b : C::PB, step_b = C::BTR ? (size_t)C::KT * t.ldb_b : C::PB;
+  // scales: waves 0 .. BM / 64 - 1 fetch a row's each lane, the next wave the columns', the others nothing
+  constexpr int SB = C::SC == kScaleF32 ? 4 : 1;
+  unsigned soff = kNowhere;
+  const char* sbase = t.as;
+  long long sstep = 0;
+  if constexpr (C::SC != kScaleNone) {
+    if (wave < C::BM / 64) {
+      const int r = wave * 64 + lane;
+      if (r < t.a_rows) soff = (unsigned)r * (unsigned)(g.as_row * SB);
+      sstep = g.as_k * SB;
+    } else if (wave == C::BM / 64) {
+      if (lane < C::BN / kScaleBlock && lane * kScaleBlock < t.b_rows) soff = (unsigned)lane * (unsigned)(g.bs_row * SB);
+      sbase = t.bs;
+      sstep = g.bs_k * SB;
+    }
+  }
+  constexpr int PT = DmaA::PIECES + DmaB::PIECES + (C::SC != kScaleNone ? 1 : 0);
+  const int nk = (t.red + C::KT - 1) / C::KT, left = t.red - (nk - 1) * C::KT;
+  const char *pa = t.a, *pb = t.b;
+  auto issue = [&](int kt, char* base) {
+    if (kt == nk - 1 && left < C::KT) {
+      da.cut(wave, lane, left);
+      db.cut(wave, lane, left);
+    }
+    da.load(base, pa, wave);
+    db.load(base + C::OPA, pb, wave);
+    if constexpr (C::SC != kScaleNone) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sbase, 0, 0x7fffffff, 0x00020000);
+      g_lds_ptr const at = (g_lds_ptr)(base + C::OPA + C::OPB + wave * 256);
+      if constexpr (C::SC == kScaleF32) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 4, soff, 0, 0, 0);
+      else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 1, soff, 0, 0, 0);      // a byte to a word each
+      sbase += sstep;
+    }
+    pa += step_a;
+    pb += step_b;
+  };
+  gf4 acc[C::NI][C::NJ];
+#pragma unroll
+  for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int p = 0; p < C::NBUF - 1; ++p)
+    if (p < nk) issue(p, lds + p * C::STAGE);
+  int buf = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    const int ahead = nk - 1 - kt;
+    if constexpr (C::NBUF >= 4) {
+      if (ahead >= C::NBUF - 2) wait_vm<PT * (C::NBUF - 2)>();
+      else if (ahead == 1) wait_vm<PT>();
+      else if (ahead == 0) wait_vm<0>();
+      else wait_vm<2 * PT>();
+    } else if constexpr (C::NBUF == 3) {
+      if (ahead >= 1) wait_vm<PT>();
+      else wait_vm<0>();
+    } else {
+      wait_vm<0>();
+    }
+    bar();
+    tile_step<C>(lds + (buf == 0 ? C::NBUF - 1 : buf - 1) * C::STAGE, lds + buf * C::STAGE, wm, wn, acc,
+                 [&](char* into) {
+                   if (kt + C::NBUF - 1 < nk) issue(kt + C::NBUF - 1, into);
+                 });
+    buf = buf == C::NBUF - 1 ? 0 : buf + 1;
+  }
+  tile_store<C>(g, c_tile, c_rows, c_cols, wm, wn, acc);
 }
 
 template <class C>
