@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 from typing import Optional
@@ -100,19 +101,14 @@ def load() -> ctypes.CDLL:
         return lib
 
 
-class GroupArgs(ctypes.Structure):
-    """``GroupArgs`` of native/hip/group_common.h: one grouped or block-scaled product."""
-    _fields_ = ([(f, ctypes.c_void_p) for f in ("a", "b", "c", "a_scale", "b_scale", "offsets")]
-                + [(f, ctypes.c_longlong) for f in ("lda", "ldb", "ldc", "b_expert", "c_expert", "as_row", "as_k",
-                                                    "bs_expert", "bs_row", "bs_k")]
-                + [(f, ctypes.c_int) for f in ("rows", "cols", "red", "experts", "mode", "dtype", "scale", "zero_rest")])
-
-
-class QuantArgs(ctypes.Structure):
-    """``QuantArgs`` of native/hip/quant_block.hip: one quantisation by blocks."""
-    _fields_ = ([(f, ctypes.c_void_p) for f in ("x", "q", "s")]
-                + [(f, ctypes.c_longlong) for f in ("ld", "batch_stride")]
-                + [(f, ctypes.c_int) for f in ("batches", "rows", "cols", "dtype", "block_rows", "e8")])
+# The argument structs of native/hip/group_common.h (GroupArgs) and quant_block.hip (QuantArgs), packed in one call:
+# building a ctypes.Structure field by field costs more than the launch.
+GROUP_FIELDS = ("a", "b", "c", "a_scale", "b_scale", "offsets",
+                "lda", "ldb", "ldc", "b_expert", "c_expert", "as_row", "as_k", "bs_expert", "bs_row", "bs_k",
+                "rows", "cols", "red", "experts", "mode", "dtype", "scale", "zero_rest")
+pack_group = struct.Struct("=6Q10q8i").pack
+QUANT_FIELDS = ("x", "q", "s", "ld", "batch_stride", "batches", "rows", "cols", "dtype", "block_rows", "e8")
+pack_quant = struct.Struct("=3Q2q6i").pack
 
 
 def group_lib_path() -> Path:
@@ -133,9 +129,9 @@ def load_group() -> ctypes.CDLL:
             import torch  # noqa: F401  (its HIP runtime first: see load())
 
             lib = ctypes.CDLL(str(p))
-            lib.amdgo_gemm_group.argtypes = [ctypes.POINTER(GroupArgs), ctypes.c_void_p]
+            lib.amdgo_gemm_group.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
             lib.amdgo_gemm_group.restype = ctypes.c_int
-            lib.amdgo_quantize_fp8_block.argtypes = [ctypes.POINTER(QuantArgs), ctypes.c_void_p]
+            lib.amdgo_quantize_fp8_block.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
             lib.amdgo_quantize_fp8_block.restype = ctypes.c_int
             _GROUP_LIB = lib
     return _GROUP_LIB

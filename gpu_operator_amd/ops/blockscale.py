@@ -15,10 +15,8 @@ two scales (a float32: scales whose product leaves float32's range are not suppo
 
 from __future__ import annotations
 
-import ctypes
-
 from . import _lib
-from .grouped import MODE_FORWARD, _matrix, _offsets, _on, _row_stride, _shape, _written, launch
+from .grouped import MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, launch
 
 BLOCK = 128
 
@@ -40,23 +38,22 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
     scale_dtype = scale_dtype or torch.float32
     codes = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
     _shape(isinstance(x, torch.Tensor) and x.dim() in (2, 3), "x must be a tensor of 2 or 3 dimensions")
-    _matrix(x, "x", x.dim(), tuple(codes))
+    shape = tuple(x.shape)
+    strides = _matrix(x, "x", len(shape), codes)
     if block_rows not in (1, BLOCK):
         raise ValueError(f"block_rows must be 1 or {BLOCK}, got {block_rows}")
     if scale_dtype not in (torch.float32, torch.float8_e8m0fnu):
         raise TypeError(f"scale_dtype must be torch.float32 or torch.float8_e8m0fnu, got {scale_dtype}")
-    batch, (rows, cols) = (x.shape[0] if x.dim() == 3 else 1), x.shape[-2:]
-    scale_shape = (*x.shape[:-2], rows if block_rows == 1 else _blocks(rows), _blocks(cols))
-    q = _result(out, "out", tuple(x.shape), torch.float8_e4m3fn, x)
+    rows, cols = shape[-2:]
+    scale_shape = (*shape[:-2], rows if block_rows == 1 else _blocks(rows), _blocks(cols))
+    q = _result(out, "out", shape, torch.float8_e4m3fn, x)
     s = _result(scale_out, "scale_out", scale_shape, scale_dtype, x)
     if x.numel():
-        args = _lib.QuantArgs(x=x.data_ptr(), q=q.data_ptr(), s=s.data_ptr(), ld=_row_stride(x),
-                              batch_stride=x.stride(0) if x.dim() == 3 else 0, batches=batch, rows=rows, cols=cols,
-                              dtype=codes[x.dtype], block_rows=block_rows, e8=int(scale_dtype == torch.float8_e8m0fnu))
-        with _on(x.device):
-            err = _lib.load_group().amdgo_quantize_fp8_block(ctypes.byref(args),
-                                                             torch.cuda.current_stream(x.device).cuda_stream)
-        _lib.check(err, "amdgo_quantize_fp8_block")
+        batched = len(shape) == 3
+        launch(x.device, "amdgo_quantize_fp8_block", _lib.load_group().amdgo_quantize_fp8_block, _lib.pack_quant,
+               x.data_ptr(), q.data_ptr(), s.data_ptr(), _row_stride(shape, strides), strides[0] if batched else 0,
+               shape[0] if batched else 1, rows, cols, codes[x.dtype], block_rows,
+               0 if scale_dtype == torch.float32 else 1)
     return q, s
 
 
@@ -85,32 +82,26 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
 
     f8 = (torch.float8_e4m3fn,)
     dims = 2 if offsets is None else 3
-    _matrix(a, "a", 2, f8)
-    _matrix(bt, "bt", dims, f8, a.device)
-    m, k = a.shape
-    n = bt.shape[-2]
-    e = bt.shape[0] if dims == 3 else 1
-    _shape(bt.shape[-1] == k, f"a is [{m},{k}], bt is {tuple(bt.shape)}: their last dimensions differ")
+    sa = _matrix(a, "a", 2, f8)
+    device = a.device
+    sb = _matrix(bt, "bt", dims, f8, device)
+    (m, k), shape_b = a.shape, tuple(bt.shape)
+    n, e = shape_b[-2], shape_b[0] if dims == 3 else 1
+    _shape(shape_b[-1] == k, f"a is [{m},{k}], bt is {shape_b}: their last dimensions differ")
     _shape(e >= 1, "bt has no experts")
-    _scale(a_scale, "a_scale", (m, _blocks(k)), (torch.float32, torch.float8_e8m0fnu), a.device)
-    _scale(bt_scale, "bt_scale", (*bt.shape[:-2], _blocks(n), _blocks(k)), (a_scale.dtype,), a.device)
+    _scale(a_scale, "a_scale", (m, _blocks(k)), (torch.float32, torch.float8_e8m0fnu), device)
+    _scale(bt_scale, "bt_scale", (*shape_b[:-2], _blocks(n), _blocks(k)), (a_scale.dtype,), device)
     if offsets is not None:
-        _offsets(offsets, e, a.device)
-    rest = 0
-    if out is None:
-        out, rest = torch.empty((m, n), dtype=torch.bfloat16, device=a.device), int(offsets is not None)
-    else:
-        _matrix(out, "out", 2, (torch.bfloat16,), a.device)
-        _shape(tuple(out.shape) == (m, n), f"out must be [{m},{n}], got {tuple(out.shape)}")
-        _written(out, "out")
+        _offsets(offsets, e, device)
+    out, ldc, rest = _out(out, (m, n), torch.bfloat16, device)
     if m and n:
-        launch(a.device, "amdgo_gemm_group(fp8)", a=a.data_ptr(), b=bt.data_ptr(), c=out.data_ptr(),
-               a_scale=a_scale.data_ptr(), b_scale=bt_scale.data_ptr(),
-               offsets=None if offsets is None else offsets.data_ptr(), lda=_row_stride(a), ldb=_row_stride(bt),
-               ldc=_row_stride(out), b_expert=bt.stride(0) if dims == 3 else 0, as_row=a_scale.stride(0),
-               as_k=a_scale.stride(1), bs_expert=bt_scale.stride(0) if dims == 3 else 0, bs_row=bt_scale.stride(-2),
-               bs_k=bt_scale.stride(-1), rows=m, cols=n, red=k, experts=e, mode=MODE_FORWARD, dtype=2,
-               scale=1 if a_scale.dtype == torch.float32 else 2, zero_rest=rest)
+        ssa, ssb = a_scale.stride(), bt_scale.stride()
+        launch(device, "amdgo_gemm_group(fp8)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+               a.data_ptr(), bt.data_ptr(), out.data_ptr(), a_scale.data_ptr(), bt_scale.data_ptr(),
+               0 if offsets is None else offsets.data_ptr(),
+               _row_stride((m, k), sa), _row_stride((n, k), sb), ldc, sb[0] if dims == 3 else 0, 0,
+               ssa[0], ssa[1], ssb[0] if dims == 3 else 0, ssb[-2], ssb[-1],
+               m, n, k, e, MODE_FORWARD, 2, 1 if a_scale.dtype == torch.float32 else 2, rest)
     return out
 
 

@@ -17,49 +17,53 @@ stride; only the last dimension has to be contiguous.
 
 from __future__ import annotations
 
-import contextlib
-import ctypes
+import struct
 
 from . import _lib
 
 MODE_FORWARD, MODE_DGRAD, MODE_WGRAD = 0, 1, 2
-_INT_MAX = 2 ** 31 - 1
 
 
 def _matrix(t, name: str, dims: int, dtypes, device=None):
-    """A GPU tensor of `dims` dimensions whose last one is contiguous and whose rows do not overlap."""
-    import torch
-
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+    """A GPU tensor of `dims` dimensions whose last one is contiguous; its strides."""
+    try:
+        strides = t.stride()
+        if t.dtype in dtypes and len(strides) == dims and t.is_cuda and (device is None or t.device == device) \
+                and (strides[-1] == 1 or t.shape[-1] <= 1 or t.numel() == 0):
+            return strides
+    except AttributeError:
+        raise TypeError(f"{name} must be a tensor, got {type(t).__name__}") from None
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if t.dim() != dims:
+    if len(strides) != dims:
         raise ValueError(f"{name} must have {dims} dimensions, got shape {tuple(t.shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor")
     if device is not None and t.device != device:
         raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
-    if max(t.shape, default=0) > _INT_MAX:
-        raise ValueError(f"{name} has a dimension over 2^31 - 1: {tuple(t.shape)}")
-    if t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}'s last dimension must be contiguous, got strides {t.stride()}")
-    if any(s < 0 for s in t.stride()):
-        raise ValueError(f"{name} has a negative stride")
+    raise ValueError(f"{name}'s last dimension must be contiguous, got strides {strides}")
 
 
-def _row_stride(t) -> int:
+def _row_stride(shape, strides) -> int:
     """Elements between two rows (a single row's own stride says nothing)."""
-    return t.stride(-2) if t.shape[-2] > 1 else t.shape[-1]
+    return strides[-2] if shape[-2] > 1 else shape[-1]
 
 
-def _written(t, name: str) -> None:
-    """An output's rows (and matrices) may be apart, but not overlap."""
-    rows, cols = t.shape[-2:]
-    if t.numel() and rows > 1 and t.stride(-2) < cols:
-        raise ValueError(f"{name}'s rows overlap: strides {t.stride()}")
-    if t.numel() and t.dim() == 3 and t.shape[0] > 1 and t.stride(0) < (rows - 1) * _row_stride(t) + cols:
-        raise ValueError(f"{name}'s matrices overlap: strides {t.stride()}")
+def _out(out, shape, dtype, device):
+    """(tensor to write, its row stride, whether rows that no expert owns have to be cleared). The rows (and matrices)
+    of an output may be apart, but not overlap."""
+    import torch
+
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device), shape[-1], 1
+    strides = _matrix(out, "out", len(shape), (dtype,), device)
+    _shape(tuple(out.shape) == shape, f"out must be {shape}, got {tuple(out.shape)}")
+    ld = _row_stride(shape, strides)
+    if out.numel():
+        _shape(ld >= shape[-1], f"out's rows overlap: strides {strides}")
+        if len(shape) == 3 and shape[0] > 1:
+            _shape(strides[0] >= (shape[1] - 1) * ld + shape[2], f"out's matrices overlap: strides {strides}")
+    return out, ld, 0
 
 
 def _offsets(offsets, experts: int, device) -> None:
@@ -78,20 +82,22 @@ def _shape(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _on(device):
-    """The device that a launch on one of its streams needs current."""
+def launch(device, what: str, entry, pack, *fields) -> None:
+    """One launch on the device's current stream; `entry`: a function of the library, `pack`: its arguments' packer."""
     import torch
 
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
-def launch(device, what: str, **fields) -> None:
-    import torch
-
-    args = _lib.GroupArgs(**fields)
-    with _on(device):
-        err = _lib.load_group().amdgo_gemm_group(ctypes.byref(args), torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(err, what)
+    try:
+        args = pack(*fields)
+    except struct.error:
+        raise ValueError(f"{what}: a dimension over 2^31 - 1 or a stride over 2^63 - 1") from None
+    index = device.index
+    if torch.cuda.current_device() == index:
+        err = entry(args, torch.cuda.current_stream(index).cuda_stream)
+    else:                                    # a launch on a device's stream needs that device current
+        with torch.cuda.device(index):
+            err = entry(args, torch.cuda.current_stream(index).cuda_stream)
+    if err:
+        _lib.check(err, what)
 
 
 def _dtype_code(dtype) -> int:
@@ -106,50 +112,39 @@ def _halves():
     return (torch.bfloat16, torch.float16)
 
 
-def _out(out, shape, like, name="out"):
-    """(tensor to write, whether rows that no expert owns have to be cleared)"""
-    import torch
-
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device), 1
-    _matrix(out, name, len(shape), (like.dtype,), like.device)
-    _shape(tuple(out.shape) == tuple(shape), f"{name} must be {tuple(shape)}, got {tuple(out.shape)}")
-    _written(out, name)
-    return out, 0
-
-
 def gemm_grouped(a, bt, offsets, out=None):
     """``out[t] = a[t] @ bt[e(t)].T``. ``a``: [T,K], ``bt``: [E,N,K], bf16 or fp16; ``out``: [T,N] of their type."""
-    _matrix(a, "a", 2, _halves())
-    _matrix(bt, "bt", 3, (a.dtype,), a.device)
-    t, k = a.shape
-    e, n, kb = bt.shape
+    sa = _matrix(a, "a", 2, _halves())
+    device, dtype = a.device, a.dtype
+    sb = _matrix(bt, "bt", 3, (dtype,), device)
+    (t, k), (e, n, kb) = a.shape, bt.shape
     _shape(kb == k, f"a is [{t},{k}], bt is [{e},{n},{kb}]: their last dimensions differ")
     _shape(e >= 1, "bt has no experts")
-    _offsets(offsets, e, a.device)
-    out, rest = _out(out, (t, n), a)
+    _offsets(offsets, e, device)
+    out, ldc, rest = _out(out, (t, n), dtype, device)
     if t and n:
-        launch(a.device, "amdgo_gemm_group", a=a.data_ptr(), b=bt.data_ptr(), c=out.data_ptr(), offsets=offsets.data_ptr(),
-               lda=_row_stride(a), ldb=_row_stride(bt), ldc=_row_stride(out), b_expert=bt.stride(0), rows=t, cols=n, red=k,
-               experts=e, mode=MODE_FORWARD, dtype=_dtype_code(a.dtype), zero_rest=rest)
+        launch(device, "amdgo_gemm_group", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+               a.data_ptr(), bt.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
+               _row_stride((t, k), sa), _row_stride((n, k), sb), ldc, sb[0], 0, 0, 0, 0, 0, 0,
+               t, n, k, e, MODE_FORWARD, _dtype_code(dtype), 0, rest)
     return out
 
 
 def gemm_grouped_dgrad(dc, bt, offsets, out=None):
     """The product's gradient for its rows: ``out[t] = dc[t] @ bt[e(t)]``. ``dc``: [T,N], ``bt``: [E,N,K]; ``out``: [T,K]."""
-    _matrix(dc, "dc", 2, _halves())
-    _matrix(bt, "bt", 3, (dc.dtype,), dc.device)
-    t, n = dc.shape
-    e, nb, k = bt.shape
+    sd = _matrix(dc, "dc", 2, _halves())
+    device, dtype = dc.device, dc.dtype
+    sb = _matrix(bt, "bt", 3, (dtype,), device)
+    (t, n), (e, nb, k) = dc.shape, bt.shape
     _shape(nb == n, f"dc is [{t},{n}], bt is [{e},{nb},{k}]: the middle dimension of bt is not dc's last")
     _shape(e >= 1, "bt has no experts")
-    _offsets(offsets, e, dc.device)
-    out, rest = _out(out, (t, k), dc)
+    _offsets(offsets, e, device)
+    out, ldc, rest = _out(out, (t, k), dtype, device)
     if t and k:
-        launch(dc.device, "amdgo_gemm_group(dgrad)", a=dc.data_ptr(), b=bt.data_ptr(), c=out.data_ptr(),
-               offsets=offsets.data_ptr(), lda=_row_stride(dc), ldb=_row_stride(bt), ldc=_row_stride(out),
-               b_expert=bt.stride(0), rows=t, cols=k, red=n, experts=e, mode=MODE_DGRAD, dtype=_dtype_code(dc.dtype),
-               zero_rest=rest)
+        launch(device, "amdgo_gemm_group(dgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+               dc.data_ptr(), bt.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
+               _row_stride((t, n), sd), _row_stride((n, k), sb), ldc, sb[0], 0, 0, 0, 0, 0, 0,
+               t, k, n, e, MODE_DGRAD, _dtype_code(dtype), 0, rest)
     return out
 
 
@@ -158,19 +153,20 @@ def gemm_grouped_wgrad(dc, a, offsets, out=None):
     has none). ``dc``: [T,N], ``a``: [T,K]; ``out``: [E,N,K] of their type, rounded once from the fp32 sum."""
     import torch
 
-    _matrix(dc, "dc", 2, _halves())
-    _matrix(a, "a", 2, (dc.dtype,), dc.device)
-    t, n = dc.shape
-    ta, k = a.shape
+    sd = _matrix(dc, "dc", 2, _halves())
+    device, dtype = dc.device, dc.dtype
+    sa = _matrix(a, "a", 2, (dtype,), device)
+    (t, n), (ta, k) = dc.shape, a.shape
     _shape(ta == t, f"dc has {t} rows, a has {ta}")
     _shape(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.shape[0] >= 2, "offsets must be [E + 1]")
     e = offsets.shape[0] - 1
-    _offsets(offsets, e, dc.device)
-    out, _ = _out(out, (e, n, k), dc)
+    _offsets(offsets, e, device)
+    out, ldc, _ = _out(out, (e, n, k), dtype, device)
     if n and k:
-        launch(dc.device, "amdgo_gemm_group(wgrad)", a=dc.data_ptr(), b=a.data_ptr(), c=out.data_ptr(),
-               offsets=offsets.data_ptr(), lda=_row_stride(dc), ldb=_row_stride(a), ldc=_row_stride(out),
-               c_expert=out.stride(0), rows=n, cols=k, red=t, experts=e, mode=MODE_WGRAD, dtype=_dtype_code(dc.dtype))
+        launch(device, "amdgo_gemm_group(wgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+               dc.data_ptr(), a.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
+               _row_stride((t, n), sd), _row_stride((t, k), sa), ldc, 0, out.stride(0), 0, 0, 0, 0, 0,
+               n, k, t, e, MODE_WGRAD, _dtype_code(dtype), 0, 0)
     return out
 
 
@@ -193,7 +189,7 @@ def _function():
             @torch.autograd.function.once_differentiable
             def backward(ctx, dc):
                 a, bt, offsets = ctx.saved_tensors
-                if dc.dim() == 2 and dc.numel() and (dc.stride(-1) != 1 or _row_stride(dc) < dc.shape[-1]):
+                if dc.stride(-1) != 1:
                     dc = dc.contiguous()            # a gradient broadcast by a sum has strides of zero
                 da = gemm_grouped_dgrad(dc, bt, offsets) if ctx.needs_input_grad[0] else None
                 dbt = gemm_grouped_wgrad(dc, a, offsets) if ctx.needs_input_grad[1] else None

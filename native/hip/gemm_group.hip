@@ -1,6 +1,6 @@
 // Grouped (ragged by expert) and block-scaled fp8 matrix products: the dispatch and the C entry.
-// The mathematics and the modes: group_common.h. Kernels: group_tile.h.
-#include "group_tile.h"
+// The mathematics and the modes: group_common.h. Kernels: group_tile.h, group_skinny.h.
+#include "group_skinny.h"
 
 namespace {
 
@@ -30,10 +30,44 @@ bool dma_ready(const GroupArgs& g) {
   const bool a_tr = g.mode == kModeWgrad, b_tr = g.mode != kModeForward;
   const auto fits = [&](const void* p, long long ld, long long batch, bool tr, long long width) {
     return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(batch * es) | (uintptr_t)((tr ? width : g.red) * es)) & 15) == 0 &&
-           ld * es * 256 + width * es < 0x7fffffffll;
+           ld * es * 256 + (width + g.red) * es < 0x7fffffffll;
   };
   if (!fits(g.a, g.lda, 0, a_tr, g.rows) || !fits(g.b, g.ldb, g.b_expert, b_tr, g.cols)) return false;
-  return g.scale == kScaleNone || (g.as_row * 4 * 256 < 0x7fffffffll && g.bs_row * 4 * 4 < 0x7fffffffll);
+  const long long kb = g.red / kScaleBlock + 1;
+  return g.scale == kScaleNone || ((g.as_row * 256 + g.as_k * kb) * 4 < 0x7fffffffll &&
+                                   (g.bs_row * 4 + g.bs_k * kb) * 4 < 0x7fffffffll);
+}
+
+template <class C>
+int launch_skinny(const GroupArgs& g, long long tiles_m, hipStream_t s) {
+  const long long grid = tiles_m * (((long long)g.cols + C::COLS - 1) / C::COLS);
+  if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
+  hipLaunchKernelGGL((group_skinny<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, g);
+  return (int)hipGetLastError();
+}
+
+// MT 16-row tiles a workgroup. 64 columns and 4 waves where that leaves more than two workgroups a CU, else
+// narrower columns and the reduction over more waves (8192 x 8192 fp8, 16 rows: 128 workgroups of 64 columns
+// 23.0 us, 256 of 32 with 8 waves 17.5; 1024 x 2048 bf16 over 4 experts: 32 columns 7.5, 16 columns 6.5; 64 experts of
+// 4096 x 2048 fp8: 64 columns and 4 waves 54.3, 32 and 8 58.0; the weights at a copy's rate: 13.3, 2.2, 58.0).
+template <int DT, int SC, int MT>
+int skinny_columns(const GroupArgs& g, hipStream_t s) {
+  const long long tiles_m = group_tile_bound(g.rows, g.experts, g.offsets != nullptr, 16 * MT);
+  if (tiles_m * ((g.cols + 63) / 64) > 512) return launch_skinny<SkinnyCfg<DT, SC, MT, 4, 4, 1>>(g, tiles_m, s);
+  if constexpr (MT == 1)
+    if (tiles_m * ((g.cols + 31) / 32) < 256) return launch_skinny<SkinnyCfg<DT, SC, 1, 1, 8, 1>>(g, tiles_m, s);
+  if constexpr (MT <= 2) return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1>>(g, tiles_m, s);
+  else return skinny_columns<DT, SC, 2>(g, s);
+}
+
+// Few rows a busy group: the skinny kernel, its tile as high as the groups are on average (they are uneven, so not
+// much higher: 64 experts of 8 rows on average run 93.8 us with 16-row tiles, 100.9 with 32; 16 of 32 rows 95, 73.6 and
+// with 64-row tiles 66.5; the tiled kernel 76.4). 0: not for this shape.
+int skinny_rows(const GroupArgs& g) {
+  if (g.mode != kModeForward) return 0;
+  if (g.offsets == nullptr) return g.rows <= 16 ? 1 : g.rows <= 64 ? 2 : 0;
+  const long long busy = g.experts < g.rows ? g.experts : g.rows;
+  return g.rows <= 10 * busy ? 1 : g.rows <= 20 * busy ? 2 : g.rows <= 48 * busy ? 4 : 0;
 }
 
 // 256 x 256 tiles (one workgroup a CU) once the groups fill them and the grid fills the CUs, else 128 x 128
@@ -43,6 +77,13 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
   using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
   if (!dma_ready(g)) return launch_tile<TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2>, false>(g, s);
+  if constexpr (!ATR && !BTR) {
+    switch (skinny_rows(g)) {
+      case 1: return skinny_columns<DT, SC, 1>(g, s);
+      case 2: return skinny_columns<DT, SC, 2>(g, s);
+      case 4: return skinny_columns<DT, SC, 4>(g, s);
+    }
+  }
   const long long per_group = g.mode == kModeWgrad ? g.rows : g.rows / g.experts;
   if (per_group > 128 && tile_grid<Large>(g) >= 256) return launch_tile<Large, true>(g, s);
   return launch_tile<Small, true>(g, s);
