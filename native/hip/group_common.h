@@ -109,6 +109,23 @@ __device__ __forceinline__ bool group_find_tile(const GroupArgs& g, int total, i
   return false;
 }
 
+// The expert with the `want`-th most rows (ties in order), up to 64 experts; above that the experts in order. A
+// weight gradient's tiles take as long as their expert has rows: started with the longest, the last ones to end are
+// short.
+__device__ __forceinline__ int group_by_size(const GroupArgs& g, int total, int want) {
+  if (g.offsets == nullptr || g.experts > 64) return want;
+  const int lane = threadIdx.x & 63;
+  int b = 0, x = -1;
+  if (lane < g.experts) group_rows(g.offsets, lane, total, b, x);
+  const int n = x - b;                               // -1 in lanes without an expert
+  int rank = 0;
+  for (int e = 0; e < g.experts; ++e) {
+    const int other = __builtin_amdgcn_readlane(n, e);
+    rank += other > n || (other == n && e < lane) ? 1 : 0;
+  }
+  return __builtin_ctzll(__ballot(lane < g.experts && rank == want));
+}
+
 // Most row tiles that `experts` groups of `total` rows together can have: every busy expert adds at most one
 // that is not full. The host sizes the grid with it, since the offsets live on the device.
 __host__ inline long long group_tile_bound(long long total, int experts, bool grouped, int bm) {

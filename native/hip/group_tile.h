@@ -208,10 +208,10 @@ __device__ __forceinline__ bool tile_setup(const GroupArgs& g, int block, TileOp
   const int tiles_n = (g.cols + C::BN - 1) / C::BN;
   if (g.mode == kModeWgrad) {
     const int tiles_m = (g.rows + C::BM - 1) / C::BM, per = tiles_m * tiles_n;
-    const int id = xcd_remap(block, per * g.experts);
-    const int e = id / per;
+    // an expert's tiles over all XCDs: whole experts to an XCD would leave those with the short ones idle
+    const int place = block / per, e = group_by_size(g, g.red, place);
     int tm, tn, begin = 0, end = g.red;
-    tile_coords(id - e * per, tiles_m, tiles_n, tm, tn);
+    tile_coords(xcd_remap(block - place * per, per), tiles_m, tiles_n, tm, tn);
     if (g.offsets) group_rows(g.offsets, e, g.red, begin, end);
     t.a = (const char*)g.a + (size_t)begin * g.lda * C::ES;
     t.b = (const char*)g.b + (size_t)begin * g.ldb * C::ES;
