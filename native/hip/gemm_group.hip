@@ -2,6 +2,8 @@
 // The mathematics and the modes: group_common.h. Kernels: group_tile.h, group_skinny.h.
 #include "group_skinny.h"
 
+#include <stddef.h>
+
 namespace {
 
 template <class C>
@@ -14,11 +16,14 @@ long long tile_grid(const GroupArgs& g) {
 
 template <class C, bool DMA>
 int launch_tile(const GroupArgs& g, hipStream_t s) {
-  const long long grid = tile_grid<C>(g);
+  GroupArgs a = g;
+  // the DMA kernel cuts the last tiles into parts: at most one more round of workgroups
+  a.slots = DMA && g.mode != kModeWgrad ? device_cu_count(s) * (160 * 1024 / C::LDS) : 0;
+  const long long grid = tile_grid<C>(g) + a.slots;
   if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
   if (grid == 0) return 0;
-  if constexpr (DMA) hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, g);
-  else hipLaunchKernelGGL((group_tile_regs<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, g);
+  if constexpr (DMA) hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
+  else hipLaunchKernelGGL((group_tile_regs<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
   return (int)hipGetLastError();
 }
 
@@ -103,9 +108,10 @@ int dispatch16(const GroupArgs& g, hipStream_t s) {
 
 extern "C" {
 
-int amdgo_gemm_group(const GroupArgs* args, hipStream_t s) {
+int amdgo_gemm_group(const void* args, hipStream_t s) {
   if (!args) return (int)hipErrorInvalidValue;
-  const GroupArgs& g = *args;
+  GroupArgs g = {};
+  __builtin_memcpy(&g, args, offsetof(GroupArgs, slots));       // packed by the caller up to there
   if (g.rows < 0 || g.cols < 0 || g.red < 0 || g.experts < 1) return (int)hipErrorInvalidValue;
   if (g.rows == 0 || g.cols == 0) return 0;
   if (g.dtype == kFp8) {

@@ -13,8 +13,8 @@ struct TileCfg {
   static constexpr int PB = PB_, NBUF = NBUF_;            // bytes a panel is wide; panels in the ring
   static constexpr int KT = PB / ES;                      // reduction steps a panel
   static constexpr int THREADS = 64 * WM * WN;
-  static constexpr int TM = BM / WM, TN = BN / WN;        // a wave's part
-  static constexpr int NI = TM / 16, NJ = TN / 16;
+  // a wave's part: TN columns, and of the 16-row blocks every WM-th, so that all waves share what rows there are
+  static constexpr int TN = BN / WN, NI = BM / WM / 16, NJ = TN / 16;
   static constexpr int OPA = BM * PB, OPB = BN * PB;      // bytes of a panel
   static constexpr int SCB = SC == kScaleNone ? 0 : THREADS * 4;
 
@@ -77,83 +77,120 @@ struct TileOperands {
   const char* bs;
 };
 
+typedef const __attribute__((address_space(3))) char* lds_in;      // a panel to read: 32-bit addresses, constant offsets
+__device__ __forceinline__ gi4 lds_chunk(lds_in p) { return *(const __attribute__((address_space(3))) gi4*)p; }
+__device__ __forceinline__ int lds_word(lds_in p) { return *(const __attribute__((address_space(3))) int*)p; }
+
+// A 64-byte step's fragments of a wave (16-bit operands), and its matrix instructions.
+template <class C>
+struct TileFrags {
+  gi4 a[C::NI], b[C::NJ];
+};
+
+template <class C, int W>     // 16-row block `blk`; W: a reduction-major panel's columns, 0: K-major
+__device__ __forceinline__ gi4 tile_frag(lds_in base, int blk0, int blk, int s) {
+  const int lane = threadIdx.x & 63, j16 = lane & 15, g = lane >> 4;
+  if constexpr (W > 0) {
+    // rows s 32 + 8 g + 4 h + 0..3 of the panel: their swizzle depends on the lane alone
+    const int r = g * 8 + (j16 >> 2), slot = (blk0 + blk) ^ rm_swizzle(r);
+    const lds_in at = base + r * (2 * W) + (slot << 5) + (j16 & 3) * 8 + s * 32 * 2 * W;
+    const gs4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gs4_lds)at);
+    const gs4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gs4_lds)(at + 4 * 2 * W));
+    const gi2 l2 = __builtin_bit_cast(gi2, lo), h2 = __builtin_bit_cast(gi2, hi);
+    return gi4{l2[0], l2[1], h2[0], h2[1]};
+  } else {
+    return lds_chunk(base + blk0 * 16 * C::PB + km_at<C::PB>(j16, s * 4 + g) + blk * 16 * C::PB);
+  }
+}
+
+template <class C>
+__device__ __forceinline__ gf4 tile_mfma(const gi4& b, const gi4& a, const gf4& c) {
+  if constexpr (C::DT == kFp16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gh8, b), __builtin_bit_cast(gh8, a), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gbf8, b), __builtin_bit_cast(gbf8, a), c, 0, 0, 0);
+}
+
+// NA of the wave's NI row blocks exist.
+template <class C, int NA>
+__device__ __forceinline__ void tile_read(lds_in lds, int wm, int wn, int s, TileFrags<C>& f) {
+#pragma unroll
+  for (int j = 0; j < C::NJ; ++j) f.b[j] = tile_frag<C, C::BTR ? C::BN : 0>(lds + C::OPA, wn * C::NJ, j, s);
+#pragma unroll
+  for (int i = 0; i < NA; ++i) f.a[i] = tile_frag<C, C::ATR ? C::BM : 0>(lds, wm, i * C::WM, s);
+}
+
+template <class C, int NA>
+__device__ __forceinline__ void tile_mul(const TileFrags<C>& f, gf4 (&acc)[C::NI][C::NJ]) {
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) acc[i][j] = tile_mfma<C>(f.b[j], f.a[i], acc[i][j]);
+}
+
 // One panel: acc += A panel x B panel^T (fp8: times the scales of the panel's block).
 template <class C>
-__device__ __forceinline__ void tile_compute(const char* lds, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+__device__ __forceinline__ gi8 tile_frag8(lds_in base, int blk0, int blk) {
   const int lane = threadIdx.x & 63, j16 = lane & 15, g = lane >> 4;
-  const char* la = lds;
-  const char* lb = lds + C::OPA;
-  if constexpr (C::DT == kFp8) {
-    gi8 bf[C::NJ];
+  const gi4 x = lds_chunk(base + blk0 * 2048 + km_at<128>(j16, g) + blk * 2048);
+  const gi4 y = lds_chunk(base + blk0 * 2048 + km_at<128>(j16, g + 4) + blk * 2048);
+  return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// fp8: one matrix instruction of 128 steps for each accumulator, weighted with the block's scales. e8m0 scales
+// go into the instruction. float32 ones need its sum apart (16 x 16 of it: 4 registers) and 4 multiply-adds, which
+// take half its time on the vector unit: the sums of 16 rows are kept while the next 16 rows' instructions run, so the
+// vector unit works under the matrix unit (one scale for a lane's 4 values, since they lie along a row of A).
+template <class C, int NA>
+__device__ __forceinline__ void tile_compute8(lds_in lds, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+  const int j16 = threadIdx.x & 15;
+  const lds_in la = lds, lb = lds + C::OPA, ls = lds + C::OPA + C::OPB;
+  gi8 bf[C::NJ];
 #pragma unroll
-    for (int j = 0; j < C::NJ; ++j) {
-      const int r = wn * C::TN + j * 16 + j16;
-      const gi4 x = *(const gi4*)(lb + km_at<C::PB>(r, g)), y = *(const gi4*)(lb + km_at<C::PB>(r, g + 4));
-      bf[j] = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-    const char* ls = lds + C::OPA + C::OPB;
-    if constexpr (C::SC == kScaleF32) {
-      const float sb = *(const float*)(ls + C::BM * 4 + (wn * C::TN / kScaleBlock) * 4);
+  for (int j = 0; j < C::NJ; ++j) bf[j] = tile_frag8<C>(lb, wn * C::NJ, j);
+  const int sb = lds_word(ls + C::BM * 4 + (wn * C::TN / kScaleBlock) * 4);
+  const lds_in lsa = ls + (wm * 16 + j16) * 4;
+  if constexpr (C::SC == kScaleE8) {
 #pragma unroll
-      for (int i = 0; i < C::NI; ++i) {
-        const int r = wm * C::TM + i * 16 + j16;
-        const gi4 x = *(const gi4*)(la + km_at<C::PB>(r, g)), y = *(const gi4*)(la + km_at<C::PB>(r, g + 4));
-        const gi8 af = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        const float s = *(const float*)(ls + r * 4) * sb;
+    for (int i = 0; i < NA; ++i) {
+      const gi8 af = tile_frag8<C>(la, wm, i * C::WM);
+      const int sa = lds_word(lsa + i * C::WM * 64);
 #pragma unroll
-        for (int j = 0; j < C::NJ; ++j) {
-          const gf4 p = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af, gf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) acc[i][j][q] = fmaf(p[q], s, acc[i][j][q]);
-        }
-      }
-    } else {
-      const int sb = *(const int*)(ls + C::BM * 4 + (wn * C::TN / kScaleBlock) * 4);
-#pragma unroll
-      for (int i = 0; i < C::NI; ++i) {
-        const int r = wm * C::TM + i * 16 + j16;
-        const gi4 x = *(const gi4*)(la + km_at<C::PB>(r, g)), y = *(const gi4*)(la + km_at<C::PB>(r, g + 4));
-        const gi8 af = __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
-        const int sa = *(const int*)(ls + r * 4);
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af, acc[i][j], 0, 0, 0, sb, 0, sa);
-      }
+      for (int j = 0; j < C::NJ; ++j)
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af, acc[i][j], 0, 0, 0, sb, 0, sa);
     }
   } else {
-    auto frag = [&](auto TR, const char* base, int row0, int s) -> gi4 {
-      if constexpr (decltype(TR)::value > 0) {
-        constexpr int W = decltype(TR)::value;
-        const int r = s * 32 + g * 8 + (j16 >> 2);
-        const int at = rm_at<W>(r, row0 >> 3) + (j16 & 3) * 8;
-        const gs4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gs4_lds)(base + at));
-        const gs4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((gs4_lds)(base + at + 4 * 2 * W));
-        const gi2 l2 = __builtin_bit_cast(gi2, lo), h2 = __builtin_bit_cast(gi2, hi);
-        return gi4{l2[0], l2[1], h2[0], h2[1]};
-      } else {
-        return *(const gi4*)(base + km_at<C::PB>(row0 + j16, s * 4 + g));
+    gf4 part[2][C::NJ];
+    float s[2];
+#pragma unroll
+    for (int i = 0; i <= NA; ++i) {
+      if (i < NA) {
+        const gi8 af = tile_frag8<C>(la, wm, i * C::WM);
+        s[i & 1] = __builtin_bit_cast(float, lds_word(lsa + i * C::WM * 64)) * __builtin_bit_cast(float, sb);
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j)
+          part[i & 1][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(bf[j], af, gf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
       }
-    };
-    constexpr std::integral_constant<int, C::ATR ? C::BM : 0> ta;
-    constexpr std::integral_constant<int, C::BTR ? C::BN : 0> tb;
+      if (i > 0) {
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) acc[i - 1][j][q] = fmaf(part[(i - 1) & 1][j][q], s[(i - 1) & 1], acc[i - 1][j][q]);
+      }
+    }
+  }
+}
+
+template <class C, int NA>
+__device__ __forceinline__ void tile_compute(lds_in lds, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+  if constexpr (C::DT == kFp8) {
+    tile_compute8<C, NA>(lds, wm, wn, acc);
+  } else {
 #pragma unroll
     for (int s = 0; s < C::PB / 64; ++s) {
-      gi4 bf[C::NJ];
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j) bf[j] = frag(tb, lb, wn * C::TN + j * 16, s);
-#pragma unroll
-      for (int i = 0; i < C::NI; ++i) {
-        const gi4 af = frag(ta, la, wm * C::TM + i * 16, s);
-#pragma unroll
-        for (int j = 0; j < C::NJ; ++j) {
-          if constexpr (C::DT == kFp16)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(gh8, bf[j]), __builtin_bit_cast(gh8, af),
-                                                                acc[i][j], 0, 0, 0);
-          else
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(gbf8, bf[j]), __builtin_bit_cast(gbf8, af),
-                                                                acc[i][j], 0, 0, 0);
-        }
-      }
+      TileFrags<C> f;
+      tile_read<C, NA>(lds, wm, wn, s, f);
+      tile_mul<C, NA>(f, acc);
     }
   }
 }
@@ -224,12 +261,29 @@ __device__ __forceinline__ bool tile_setup(const GroupArgs& g, int block, TileOp
     c_cols = min(C::BN, g.cols - tn * C::BN);
     c_tile = (char*)g.c + 2 * ((size_t)e * g.c_expert + (size_t)tm * C::BM * g.ldc + (size_t)tn * C::BN);
   } else {
-    const int tiles_m = group_tile_count(g, g.rows, C::BM);
-    if (block >= tiles_m * tiles_n) return false;
-    int tm, tn;
-    tile_coords(xcd_remap(block, tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
+    const int tiles_m = group_tile_count(g, g.rows, C::BM), tiles = tiles_m * tiles_n;
+    // The tiles past the last whole round of the `slots` workgroups that run at once would keep few of them busy for a
+    // whole tile's time: they are cut into 2 or 4 parts by rows, as many as still fit one round.
+    const int over = g.slots > 0 ? tiles % g.slots : 0, whole = tiles - over;
+    const int parts = over == 0 ? 1 : 4 * over <= g.slots ? 4 : 2 * over <= g.slots ? 2 : 1;
+    int tm, tn, tile, part = 0;
+    if (block < whole) {
+      tile = xcd_remap(block, whole);
+    } else {
+      if (block - whole >= over * parts) return false;
+      const int item = xcd_remap(block - whole, over * parts);
+      tile = whole + item / parts;
+      part = item % parts;
+    }
+    tile_coords(tile, tiles_m, tiles_n, tm, tn);
     RowTile rt;
     if (!group_find_tile(g, g.rows, C::BM, tm, rt)) return false;
+    if (parts > 1 && block >= whole) {
+      const int rows = C::BM / parts;
+      rt.row0 += part * rows;
+      rt.row_end = min(rt.row_end, rt.row0 + rows);
+      if (rt.row0 >= rt.row_end) return false;
+    }
     t.a = (const char*)g.a + (size_t)rt.row0 * g.lda * C::ES;
     t.a_rows = min(C::BM, rt.row_end - rt.row0);
     t.b_rows = min(C::BN, g.cols - tn * C::BN);
@@ -261,7 +315,7 @@ __device__ __forceinline__ void tile_store(const GroupArgs& g, char* c_tile, int
   const bool wide = ((uintptr_t)g.c & 7) == 0 && (g.ldc & 3) == 0 && (g.c_expert & 3) == 0;
 #pragma unroll
   for (int i = 0; i < C::NI; ++i) {
-    const int r = wm * C::TM + i * 16 + (lane & 15);
+    const int r = (i * C::WM + wm) * 16 + (lane & 15);
     if (r >= c_rows) continue;
     unsigned short* row = (unsigned short*)c_tile + (size_t)r * g.ldc;
 #pragma unroll
@@ -277,6 +331,47 @@ __device__ __forceinline__ void tile_store(const GroupArgs& g, char* c_tile, int
         for (int q = 0; q < 4; ++q)
           if (c + q < c_cols) row[c + q] = v[q];
       }
+    }
+  }
+}
+
+// The same through LDS, which the loop has left: whole rows of the tile at a time, 16 bytes a lane, where the direct
+// form writes 32 bytes of each of 16 rows. 16-byte chunk c of row r lies at c ^ (r & 15): neither side conflicts.
+template <class C>
+__device__ __forceinline__ void tile_store_rows(const GroupArgs& g, char* lds, char* c_tile, int c_rows, int c_cols, int wm, int wn,
+                                                const gf4 (&acc)[C::NI][C::NJ]) {
+  static_assert(C::BM * C::BN * 2 <= C::LDS, "the tile fits the ring");
+  constexpr int OUT = C::DT == kFp16 ? kFp16 : kBf16;
+  const bool wide = (((uintptr_t)g.c | (uintptr_t)(g.ldc * 2) | (uintptr_t)(g.c_expert * 2)) & 15) == 0;
+  if (!wide) return tile_store<C>(g, c_tile, c_rows, c_cols, wm, wn, acc);
+  const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
+  bar();                                                 // every wave has read its last fragments
+#pragma unroll
+  for (int i = 0; i < C::NI; ++i) {
+    const int r = (i * C::WM + wm) * 16 + l16;
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+      unsigned short v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = to_out<OUT>(acc[i][j][e]);
+      const int c = (wn * C::TN + j * 16) / 8 + (q >> 1);
+      *(uint2*)(lds + r * (C::BN * 2) + ((c ^ l16) << 4) + (q & 1) * 8) =
+          make_uint2(v[0] | (unsigned)v[1] << 16, v[2] | (unsigned)v[3] << 16);
+    }
+  }
+  __syncthreads();
+  constexpr int CPR = C::BN / 8, RPI = C::THREADS / CPR;  // chunks a row, rows a step of the workgroup
+  const int c = threadIdx.x % CPR;
+  for (int r = threadIdx.x / CPR; r < c_rows; r += RPI) {
+    const uint4 v = *(const uint4*)(lds + r * (C::BN * 2) + ((c ^ (r & 15)) << 4));
+    unsigned short* at = (unsigned short*)c_tile + (size_t)r * g.ldc + c * 8;
+    if (c * 8 + 8 <= c_cols) {
+      store_c16(at, v);
+    } else {
+      const unsigned w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c * 8 + e < c_cols) at[e] = (unsigned short)(w[e >> 1] >> ((e & 1) * 16));
     }
   }
 }
@@ -335,16 +430,86 @@ struct PanelDma {
   }
 };
 
+// A tile's panels by LDS-DMA, one after the other: PT pieces a wave for each.
+template <class C>
+struct TileLoader {
+  using DmaA = PanelDma<C, C::ATR, C::BM>;
+  using DmaB = PanelDma<C, C::BTR, C::BN>;
+  static constexpr int PT = DmaA::PIECES + DmaB::PIECES + (C::SC != kScaleNone ? 1 : 0);
+  static constexpr int SB = C::SC == kScaleF32 ? 4 : 1;
+  DmaA da;
+  DmaB db;
+  const char *pa, *pb, *ps;
+  size_t step_a, step_b;
+  long long step_s;
+  unsigned soff;
+  int wave, lane, nk, left;
+
+  __device__ __forceinline__ TileLoader(const GroupArgs& g, const TileOperands& t, int wave_, int lane_)
+      : pa(t.a), pb(t.b), ps(t.as), step_a(C::ATR ? (size_t)C::KT * t.lda_b : C::PB),
+        step_b(C::BTR ? (size_t)C::KT * t.ldb_b : C::PB), step_s(0), soff(kNowhere), wave(wave_), lane(lane_) {
+    nk = (t.red + C::KT - 1) / C::KT;
+    left = t.red - (nk - 1) * C::KT;
+    da.init(wave, lane, (unsigned)t.lda_b, t.a_rows, t.a_col0, t.a_cols);
+    db.init(wave, lane, (unsigned)t.ldb_b, t.b_rows, t.b_col0, t.b_cols);
+    // scales: waves 0 .. BM / 64 - 1 fetch a row's each lane, the next wave the columns', the others nothing
+    if constexpr (C::SC != kScaleNone) {
+      if (wave < C::BM / 64) {
+        const int r = wave * 64 + lane;
+        if (r < t.a_rows) soff = (unsigned)r * (unsigned)(g.as_row * SB);
+        step_s = g.as_k * SB;
+      } else if (wave == C::BM / 64) {
+        if (lane < C::BN / kScaleBlock && lane * kScaleBlock < t.b_rows) soff = (unsigned)lane * (unsigned)(g.bs_row * SB);
+        ps = t.bs;
+        step_s = g.bs_k * SB;
+      }
+    }
+  }
+  // panel kt (the next one) into `base`
+  __device__ __forceinline__ void issue(int kt, char* base) {
+    if (kt == nk - 1 && left < C::KT) {
+      da.cut(wave, lane, left);
+      db.cut(wave, lane, left);
+    }
+    da.load(base, pa, wave);
+    db.load(base + C::OPA, pb, wave);
+    if constexpr (C::SC != kScaleNone) {
+      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)ps, 0, 0x7fffffff, 0x00020000);
+      g_lds_ptr const at = (g_lds_ptr)(base + C::OPA + C::OPB + wave * 256);
+      if constexpr (C::SC == kScaleF32) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 4, soff, 0, 0, 0);
+      else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 1, soff, 0, 0, 0);      // a byte to a word each
+      ps += step_s;
+    }
+    pa += step_a;
+    pb += step_b;
+  }
+};
+
 template <int N>
 __device__ __forceinline__ void wait_vm() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// One panel's work: the next panel's DMA goes into `into` while `from` is multiplied. Two pointers that do not
-// alias, so that the compiler puts no wait for the DMA before the fragment reads.
-template <class C, class F>
-__device__ __forceinline__ void tile_step(char* __restrict__ into, const char* __restrict__ from, int wm, int wn,
-                                          gf4 (&acc)[C::NI][C::NJ], F&& issue) {
-  issue(into);
-  tile_compute<C>(from, wm, wn, acc);
+// One panel's work: panel kt goes into `into` (if there is one) while `from` is multiplied. Two pointers that do
+// not alias, so that the compiler puts no wait for the DMA before the fragment reads.
+template <class C, int NA>
+__device__ __forceinline__ void tile_step(char* __restrict__ into, const __attribute__((address_space(3))) char* __restrict__ from,
+                                          TileLoader<C>& ld, int kt, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+  if (kt < ld.nk) ld.issue(kt, into);
+  tile_compute<C, NA>(from, wm, wn, acc);
+}
+
+// The loop over the panels with NA of a wave's row blocks.
+template <class C, int NA>
+__device__ __forceinline__ void tile_loop(char* lds, TileLoader<C>& ld, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+  constexpr int PT = TileLoader<C>::PT;
+  int buf = 0;
+  for (int kt = 0; kt < ld.nk; ++kt) {
+    if (C::NBUF == 3 && ld.nk - 1 - kt >= 1) wait_vm<PT>();
+    else wait_vm<0>();
+    bar();
+    tile_step<C, NA>(lds + (buf == 0 ? C::NBUF - 1 : buf - 1) * C::STAGE, (lds_in)lds + buf * C::STAGE, ld, kt + C::NBUF - 1,
+                     wm, wn, acc);
+    buf = buf == C::NBUF - 1 ? 0 : buf + 1;
+  }
 }
 
 // The same tile with its panels in a ring of NBUF, NBUF - 1 of them in flight. At panel t a counted wait
@@ -361,49 +526,7 @@ group_tile_dma(const GroupArgs g) {
   if (!tile_setup<C>(g, blockIdx.x, t, c_tile, c_rows, c_cols)) return;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WN, wn = wave % C::WN;
-  using DmaA = PanelDma<C, C::ATR, C::BM>;
-  using DmaB = PanelDma<C, C::BTR, C::BN>;
-  DmaA da;
-  DmaB db;
-  da.init(wave, lane, (unsigned)t.lda_b, t.a_rows, t.a_col0, t.a_cols);
-  db.init(wave, lane, (unsigned)t.ldb_b, t.b_rows, t.b_col0, t.b_cols);
-  const size_t step_a = C::ATR ? (size_t)C::KT * t.lda_b : C::PB, step_b = C::BTR ? (size_t)C::KT * t.ldb_b : C::PB;
-  // scales: waves 0 .. BM / 64 - 1 fetch a row's each lane, the next wave the columns', the others nothing
-  constexpr int SB = C::SC == kScaleF32 ? 4 : 1;
-  unsigned soff = kNowhere;
-  const char* sbase = t.as;
-  long long sstep = 0;
-  if constexpr (C::SC != kScaleNone) {
-    if (wave < C::BM / 64) {
-      const int r = wave * 64 + lane;
-      if (r < t.a_rows) soff = (unsigned)r * (unsigned)(g.as_row * SB);
-      sstep = g.as_k * SB;
-    } else if (wave == C::BM / 64) {
-      if (lane < C::BN / kScaleBlock && lane * kScaleBlock < t.b_rows) soff = (unsigned)lane * (unsigned)(g.bs_row * SB);
-      sbase = t.bs;
-      sstep = g.bs_k * SB;
-    }
-  }
-  constexpr int PT = DmaA::PIECES + DmaB::PIECES + (C::SC != kScaleNone ? 1 : 0);
-  const int nk = (t.red + C::KT - 1) / C::KT, left = t.red - (nk - 1) * C::KT;
-  const char *pa = t.a, *pb = t.b;
-  auto issue = [&](int kt, char* base) {
-    if (kt == nk - 1 && left < C::KT) {
-      da.cut(wave, lane, left);
-      db.cut(wave, lane, left);
-    }
-    da.load(base, pa, wave);
-    db.load(base + C::OPA, pb, wave);
-    if constexpr (C::SC != kScaleNone) {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)sbase, 0, 0x7fffffff, 0x00020000);
-      g_lds_ptr const at = (g_lds_ptr)(base + C::OPA + C::OPB + wave * 256);
-      if constexpr (C::SC == kScaleF32) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 4, soff, 0, 0, 0);
-      else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 1, soff, 0, 0, 0);      // a byte to a word each
-      sbase += sstep;
-    }
-    pa += step_a;
-    pb += step_b;
-  };
+  TileLoader<C> ld(g, t, wave, lane);
   gf4 acc[C::NI][C::NJ];
 #pragma unroll
   for (int i = 0; i < C::NI; ++i)
@@ -411,29 +534,12 @@ group_tile_dma(const GroupArgs g) {
     for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int p = 0; p < C::NBUF - 1; ++p)
-    if (p < nk) issue(p, lds + p * C::STAGE);
-  int buf = 0;
-  for (int kt = 0; kt < nk; ++kt) {
-    const int ahead = nk - 1 - kt;
-    if constexpr (C::NBUF >= 4) {
-      if (ahead >= C::NBUF - 2) wait_vm<PT * (C::NBUF - 2)>();
-      else if (ahead == 1) wait_vm<PT>();
-      else if (ahead == 0) wait_vm<0>();
-      else wait_vm<2 * PT>();
-    } else if constexpr (C::NBUF == 3) {
-      if (ahead >= 1) wait_vm<PT>();
-      else wait_vm<0>();
-    } else {
-      wait_vm<0>();
-    }
-    bar();
-    tile_step<C>(lds + (buf == 0 ? C::NBUF - 1 : buf - 1) * C::STAGE, lds + buf * C::STAGE, wm, wn, acc,
-                 [&](char* into) {
-                   if (kt + C::NBUF - 1 < nk) issue(kt + C::NBUF - 1, into);
-                 });
-    buf = buf == C::NBUF - 1 ? 0 : buf + 1;
-  }
-  tile_store<C>(g, c_tile, c_rows, c_cols, wm, wn, acc);
+    if (p < ld.nk) ld.issue(p, lds + p * C::STAGE);
+  // a group's last tile, or a part of a tile, is as long as its rows, in quarters
+  if (c_rows > C::BM / 2) tile_loop<C, C::NI>(lds, ld, wm, wn, acc);
+  else if (c_rows > C::BM / 4) tile_loop<C, C::NI / 2>(lds, ld, wm, wn, acc);
+  else tile_loop<C, C::NI / 4>(lds, ld, wm, wn, acc);
+  tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
 }
 
 template <class C>
@@ -456,7 +562,7 @@ __global__ void __launch_bounds__(C::THREADS) group_tile_regs(const GroupArgs g)
     stage_regs<C, C::BTR, C::BN>(lds + C::OPA, t.b, t.ldb_b, t.b_rows, t.b_col0, t.b_cols, t.red, kt);
     stage_scales<C>(lds + C::OPA + C::OPB, g, t, kt);
     __syncthreads();
-    tile_compute<C>(lds, wm, wn, acc);
+    tile_compute<C, C::NI>((lds_in)lds, wm, wn, acc);
     __syncthreads();
   }
   tile_store<C>(g, c_tile, c_rows, c_cols, wm, wn, acc);
