@@ -14,15 +14,18 @@ long long tile_grid(const GroupArgs& g) {
   return tiles_m * tiles_n;
 }
 
-template <class C, bool DMA>
+enum TileKernel { kTileRegs, kTileDma, kTilePingPong };
+
+template <class C, TileKernel KERNEL>
 int launch_tile(const GroupArgs& g, hipStream_t s) {
   GroupArgs a = g;
-  // the DMA kernel cuts the last tiles into parts: at most one more round of workgroups
-  a.slots = DMA && g.mode != kModeWgrad ? device_cu_count(s) * (160 * 1024 / C::LDS) : 0;
+  // the DMA kernels cut the last tiles into parts: at most one more round of workgroups
+  a.slots = KERNEL != kTileRegs && g.mode != kModeWgrad ? device_cu_count(s) * (160 * 1024 / C::LDS) : 0;
   const long long grid = tile_grid<C>(g) + a.slots;
   if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
   if (grid == 0) return 0;
-  if constexpr (DMA) hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
+  if constexpr (KERNEL == kTilePingPong) hipLaunchKernelGGL((group_tile_pp<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
+  else if constexpr (KERNEL == kTileDma) hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
   else hipLaunchKernelGGL((group_tile_regs<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
   return (int)hipGetLastError();
 }
@@ -81,7 +84,7 @@ template <int DT, int SC, bool ATR, bool BTR>
 int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
   using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
-  if (!dma_ready(g)) return launch_tile<TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2>, false>(g, s);
+  if (!dma_ready(g)) return launch_tile<TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2>, kTileRegs>(g, s);
   if constexpr (!ATR && !BTR) {
     switch (skinny_rows(g)) {
       case 1: return skinny_columns<DT, SC, 1>(g, s);
@@ -90,8 +93,8 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
     }
   }
   const long long per_group = g.mode == kModeWgrad ? g.rows : g.rows / g.experts;
-  if (per_group > 128 && tile_grid<Large>(g) >= 256) return launch_tile<Large, true>(g, s);
-  return launch_tile<Small, true>(g, s);
+  if (per_group > 128 && tile_grid<Large>(g) >= 256) return launch_tile<Large, kTilePingPong>(g, s);
+  return launch_tile<Small, kTileDma>(g, s);
 }
 
 template <int DT>

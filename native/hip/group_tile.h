@@ -430,13 +430,38 @@ struct PanelDma {
   }
 };
 
+// The scales of a panel by LDS-DMA: waves 0 .. BM / 64 - 1 fetch a row's each lane, the next wave the columns', the
+// others nothing.
+template <class C>
+__device__ __forceinline__ void scale_lanes(const GroupArgs& g, const TileOperands& t, int wave, int lane, unsigned& soff,
+                                            const char*& base, long long& step) {
+  constexpr int SB = C::SC == kScaleF32 ? 4 : 1;
+  if (wave < C::BM / 64) {
+    const int r = wave * 64 + lane;
+    if (r < t.a_rows) soff = (unsigned)r * (unsigned)(g.as_row * SB);
+    base = t.as;
+    step = g.as_k * SB;
+  } else if (wave == C::BM / 64) {
+    if (lane < C::BN / kScaleBlock && lane * kScaleBlock < t.b_rows) soff = (unsigned)lane * (unsigned)(g.bs_row * SB);
+    base = t.bs;
+    step = g.bs_k * SB;
+  }
+}
+
+template <class C>
+__device__ __forceinline__ void scale_load(char* lds, const char* base, int wave, unsigned soff) {
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000);
+  g_lds_ptr const at = (g_lds_ptr)(lds + wave * 256);
+  if constexpr (C::SC == kScaleF32) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 4, soff, 0, 0, 0);
+  else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 1, soff, 0, 0, 0);      // a byte to a word each
+}
+
 // A tile's panels by LDS-DMA, one after the other: PT pieces a wave for each.
 template <class C>
 struct TileLoader {
   using DmaA = PanelDma<C, C::ATR, C::BM>;
   using DmaB = PanelDma<C, C::BTR, C::BN>;
   static constexpr int PT = DmaA::PIECES + DmaB::PIECES + (C::SC != kScaleNone ? 1 : 0);
-  static constexpr int SB = C::SC == kScaleF32 ? 4 : 1;
   DmaA da;
   DmaB db;
   const char *pa, *pb, *ps;
@@ -452,18 +477,7 @@ struct TileLoader {
     left = t.red - (nk - 1) * C::KT;
     da.init(wave, lane, (unsigned)t.lda_b, t.a_rows, t.a_col0, t.a_cols);
     db.init(wave, lane, (unsigned)t.ldb_b, t.b_rows, t.b_col0, t.b_cols);
-    // scales: waves 0 .. BM / 64 - 1 fetch a row's each lane, the next wave the columns', the others nothing
-    if constexpr (C::SC != kScaleNone) {
-      if (wave < C::BM / 64) {
-        const int r = wave * 64 + lane;
-        if (r < t.a_rows) soff = (unsigned)r * (unsigned)(g.as_row * SB);
-        step_s = g.as_k * SB;
-      } else if (wave == C::BM / 64) {
-        if (lane < C::BN / kScaleBlock && lane * kScaleBlock < t.b_rows) soff = (unsigned)lane * (unsigned)(g.bs_row * SB);
-        ps = t.bs;
-        step_s = g.bs_k * SB;
-      }
-    }
+    if constexpr (C::SC != kScaleNone) scale_lanes<C>(g, t, wave, lane, soff, ps, step_s);
   }
   // panel kt (the next one) into `base`
   __device__ __forceinline__ void issue(int kt, char* base) {
@@ -474,10 +488,7 @@ struct TileLoader {
     da.load(base, pa, wave);
     db.load(base + C::OPA, pb, wave);
     if constexpr (C::SC != kScaleNone) {
-      const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)ps, 0, 0x7fffffff, 0x00020000);
-      g_lds_ptr const at = (g_lds_ptr)(base + C::OPA + C::OPB + wave * 256);
-      if constexpr (C::SC == kScaleF32) __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 4, soff, 0, 0, 0);
-      else __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, at, 1, soff, 0, 0, 0);      // a byte to a word each
+      scale_load<C>(base + C::OPA + C::OPB, ps, wave, soff);
       ps += step_s;
     }
     pa += step_a;
@@ -539,6 +550,278 @@ group_tile_dma(const GroupArgs g) {
   if (c_rows > C::BM / 2) tile_loop<C, C::NI>(lds, ld, wm, wn, acc);
   else if (c_rows > C::BM / 4) tile_loop<C, C::NI / 2>(lds, ld, wm, wn, acc);
   else tile_loop<C, C::NI / 4>(lds, ld, wm, wn, acc);
+  tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
+}
+
+// The ping-pong form of the 256 x 256 tile. Its 8 waves are two groups of 4 (a SIMD has one wave of each), one
+// interval apart: while one group runs matrix instructions, the other reads its next fragments from LDS and issues
+// DMA; a barrier ends every interval. A panel takes a group four of them:
+//
+//   read B and the upper half's A | multiply the upper half | read the lower half's A | multiply the lower half
+//
+// (the wave's 64 columns of B are kept for both halves: 64 registers of fragments, 128 of sums). With two panels in
+// LDS the parts of a buffer are refilled as soon as they are free: B, the upper half of A and the scales of panel t
+// have been read by both groups when the first one reads the lower half, and there it issues those of panel
+// t + 2; the lower half of panel t + 1 is issued where panel t's first read is. So a piece has 4 to 5 intervals (about
+// 2500 cycles) to land, where the plain ring of two gives it 4 at most and leaves the matrix pipes idle while
+// all waves read.
+template <class C>
+struct PingPong {
+  static constexpr int HM = C::BM / 2, NH = C::NI / 2;                    // rows and a wave's blocks in a half
+  static constexpr int HALF = HM * C::PB;
+  static constexpr int LO = 0, HI = HALF, B = 2 * HALF, STAGE = B + C::OPB;      // where they are in a stage
+  static constexpr int SCALES = 2 * STAGE, LDS = SCALES + 4 * C::SCB;             // the scales' ring
+  using DmaA = PanelDma<C, C::ATR, HM>;
+  using DmaB = PanelDma<C, C::BTR, C::BN>;
+  static constexpr int P1 = DmaA::PIECES + DmaB::PIECES + (C::SC != kScaleNone ? 1 : 0), P2 = DmaA::PIECES;
+  static_assert(C::WM == 2 && C::WN == 4 && C::NBUF == 2 && C::PB == 128, "two groups of four waves, two panels");
+};
+
+template <class C>
+struct PingPongLoader {
+  using P = PingPong<C>;
+  typename P::DmaA lo, hi;
+  typename P::DmaB b;
+  const char *pa, *pb, *ps;
+  size_t step_a, step_b;
+  long long step_s;
+  unsigned soff;
+  int wave, lane, nk, left;
+
+  __device__ __forceinline__ PingPongLoader(const GroupArgs& g, const TileOperands& t, int wave_, int lane_)
+      : pa(t.a), pb(t.b), ps(t.as), step_a(C::ATR ? (size_t)C::KT * t.lda_b : C::PB),
+        step_b(C::BTR ? (size_t)C::KT * t.ldb_b : C::PB), step_s(0), soff(kNowhere), wave(wave_), lane(lane_) {
+    nk = (t.red + C::KT - 1) / C::KT;
+    left = t.red - (nk - 1) * C::KT;
+    lo.init(wave, lane, (unsigned)t.lda_b, t.a_rows, t.a_col0, t.a_cols);
+    if constexpr (C::ATR) {
+      hi.init(wave, lane, (unsigned)t.lda_b, 0, t.a_col0 + P::HM, t.a_cols);
+    } else {
+      hi.init(wave, lane, (unsigned)t.lda_b, t.a_rows - P::HM, 0, 0);
+#pragma unroll
+      for (int i = 0; i < P::DmaA::PIECES; ++i)
+        if (hi.off[i] != kNowhere) hi.off[i] += (unsigned)P::HM * (unsigned)t.lda_b;
+    }
+    b.init(wave, lane, (unsigned)t.ldb_b, t.b_rows, t.b_col0, t.b_cols);
+    if constexpr (C::SC != kScaleNone) scale_lanes<C>(g, t, wave, lane, soff, ps, step_s);
+  }
+  // B, A's upper half and the scales of panel kt into the stage at `base`
+  __device__ __forceinline__ void issue_lo(int kt, char* base, char* ring) {
+    if (kt == nk - 1 && left < C::KT) {
+      lo.cut(wave, lane, left);
+      b.cut(wave, lane, left);
+    }
+    b.load(base + P::B, pb + (size_t)kt * step_b, wave);
+    lo.load(base + P::LO, pa + (size_t)kt * step_a, wave);
+    if constexpr (C::SC != kScaleNone) scale_load<C>(ring + (kt & 3) * C::SCB, ps + kt * step_s, wave, soff);
+  }
+  __device__ __forceinline__ void issue_hi(int kt, char* base) {
+    if (kt == nk - 1 && left < C::KT) hi.cut(wave, lane, left);
+    hi.load(base + P::HI, pa + (size_t)kt * step_a, wave);
+  }
+};
+
+// A wave's fragments of 16 rows or columns of a whole panel: 8 registers, for fp8 one matrix instruction's operand, for
+// 16 bits two steps'.
+template <class C, int W>
+__device__ __forceinline__ gi8 panel_frag(lds_in base, int blk0, int blk) {
+  if constexpr (C::DT == kFp8) {
+    return tile_frag8<C>(base, blk0, blk);
+  } else {
+    const gi4 x = tile_frag<C, W>(base, blk0, blk, 0), y = tile_frag<C, W>(base, blk0, blk, 1);
+    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+}
+
+template <class C>
+struct PingPongFrags {
+  gi8 a[PingPong<C>::NH], b[C::NJ];
+  int s[C::SC == kScaleNone ? 1 : PingPong<C>::NH];    // float32: the product of the scales; e8m0: the row's byte
+  int sb;
+};
+
+// The scales of a half's rows. They have a ring of four panels apart, so that both halves can read them while the
+// stage's next ones land.
+template <class C, int NA, int HALF>
+__device__ __forceinline__ void pp_scales(lds_in ring, int kt, int wm, int wn, PingPongFrags<C>& f) {
+  if constexpr (C::SC != kScaleNone) {
+    const lds_in at = ring + (kt & 3) * C::SCB;
+    f.sb = lds_word(at + C::BM * 4 + (wn * C::TN / kScaleBlock) * 4);
+    const lds_in rows = at + (HALF * PingPong<C>::HM + wm * 16 + (threadIdx.x & 15)) * 4;
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      f.s[i] = lds_word(rows + i * C::WM * 64);
+      if constexpr (C::SC == kScaleF32)
+        f.s[i] = __builtin_bit_cast(int, __builtin_bit_cast(float, f.s[i]) * __builtin_bit_cast(float, f.sb));
+    }
+  }
+}
+
+// B and the upper half's A (NA of the wave's blocks).
+template <class C, int NA>
+__device__ __forceinline__ void pp_frags_lo(lds_in from, int wm, int wn, PingPongFrags<C>& f) {
+  using P = PingPong<C>;
+#pragma unroll
+  for (int j = 0; j < C::NJ; ++j) f.b[j] = panel_frag<C, C::BTR ? C::BN : 0>(from + P::B, wn * C::NJ, j);
+#pragma unroll
+  for (int i = 0; i < NA; ++i) f.a[i] = panel_frag<C, C::ATR ? P::HM : 0>(from + P::LO, wm, i * C::WM);
+}
+
+// (Two pointers that do not alias, as in tile_step.)
+template <class C>
+__device__ __forceinline__ void pp_read_lo(char* __restrict__ into, const __attribute__((address_space(3))) char* __restrict__ from,
+                                           lds_in ring, PingPongLoader<C>& ld, int kt, int wm, int wn, PingPongFrags<C>& f) {
+  pp_frags_lo<C, PingPong<C>::NH>(from, wm, wn, f);
+  pp_scales<C, PingPong<C>::NH, 0>(ring, kt, wm, wn, f);
+  if (kt + 1 < ld.nk) ld.issue_hi(kt + 1, into);
+}
+
+template <class C>
+__device__ __forceinline__ void pp_read_hi(char* __restrict__ into, const __attribute__((address_space(3))) char* __restrict__ from,
+                                           char* ring, PingPongLoader<C>& ld, int kt, int wm, int wn, PingPongFrags<C>& f) {
+  using P = PingPong<C>;
+#pragma unroll
+  for (int i = 0; i < P::NH; ++i) f.a[i] = panel_frag<C, C::ATR ? P::HM : 0>(from + P::HI, wm, i * C::WM);
+  pp_scales<C, P::NH, 1>((lds_in)ring, kt, wm, wn, f);
+  if (kt + 2 < ld.nk) ld.issue_lo(kt + 2, into, ring);
+}
+
+// The products of NA blocks of the wave, from its block I0 on.
+template <class C, int I0, int NA>
+__device__ __forceinline__ void pp_mul(const PingPongFrags<C>& f, gf4 (&acc)[C::NI][C::NJ]) {
+  if constexpr (C::SC == kScaleF32) {
+    // two accumulators' sums are weighted while the next two's instructions run
+    constexpr int STEPS = NA * C::NJ / 2;
+    gf4 part[2][2];
+#pragma unroll
+    for (int k = 0; k <= STEPS; ++k) {
+      if (k < STEPS) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          part[k & 1][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.b[(2 * k + h) % C::NJ], f.a[2 * k / C::NJ],
+                                                                           gf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
+      }
+      if (k > 0) {
+        const int i = 2 * (k - 1) / C::NJ;
+        const float s = __builtin_bit_cast(float, f.s[i]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          gf4& a = acc[I0 + i][(2 * (k - 1) + h) % C::NJ];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) a[q] = fmaf(part[(k - 1) & 1][h][q], s, a[q]);
+        }
+      }
+    }
+  } else if constexpr (C::SC == kScaleE8) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j)
+        acc[I0 + i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.b[j], f.a[i], acc[I0 + i][j], 0, 0, 0, f.sb, 0, f.s[i]);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j) {
+          const gi8 b = f.b[j], a = f.a[i];
+          acc[I0 + i][j] = h == 0 ? tile_mfma<C>(__builtin_shufflevector(b, b, 0, 1, 2, 3), __builtin_shufflevector(a, a, 0, 1, 2, 3), acc[I0 + i][j])
+                                  : tile_mfma<C>(__builtin_shufflevector(b, b, 4, 5, 6, 7), __builtin_shufflevector(a, a, 4, 5, 6, 7), acc[I0 + i][j]);
+        }
+  }
+  // the sums are done here: the compiler may not sink work past the barrier that follows
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) asm volatile("" : "+v"(acc[I0 + i][j]));
+}
+
+template <class C>
+__device__ __forceinline__ void pp_loop(char* lds, PingPongLoader<C>& ld, int wave, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+  using P = PingPong<C>;
+  const int nk = ld.nk;
+  if (nk == 0) return;
+  char* const ring = lds + P::SCALES;
+  ld.issue_lo(0, lds, ring);
+  ld.issue_hi(0, lds);
+  if (nk > 1) {
+    ld.issue_lo(1, lds + P::STAGE, ring);
+    wait_vm<P::P1 + P::P2>();
+  } else {
+    wait_vm<P::P2>();
+  }
+  bar();
+  if (wave >= 4) bar();
+  for (int kt = 0; kt < nk; ++kt) {
+    char* const here = lds + (kt & 1) * P::STAGE;
+    char* const there = lds + (~kt & 1) * P::STAGE;
+    PingPongFrags<C> f;
+    pp_read_lo<C>(there, (lds_in)here, (lds_in)ring, ld, kt, wm, wn, f);
+    if (kt + 1 < nk) wait_vm<P::P1 + P::P2>();       // this wave's pieces of the lower half have landed
+    else wait_vm<0>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    bar();
+    __builtin_amdgcn_s_setprio(1);
+    pp_mul<C, 0, P::NH>(f, acc);
+    __builtin_amdgcn_s_setprio(0);
+    bar();
+    // (the stage's upper half, B and scales have been read by both groups: panel kt + 2's go there)
+    pp_read_hi<C>(here, (lds_in)here, ring, ld, kt, wm, wn, f);
+    if (kt + 2 < nk) wait_vm<P::P1 + P::P2>();       // and of the next panel's first part
+    else wait_vm<P::P2>();
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    bar();
+    __builtin_amdgcn_s_setprio(1);
+    pp_mul<C, P::NH, P::NH>(f, acc);
+    __builtin_amdgcn_s_setprio(0);
+    bar();
+  }
+  if (wave < 4) bar();
+}
+
+// A tile of at most half the rows: its upper half alone, NA of a wave's blocks, all waves in step.
+template <class C, int NA>
+__device__ __forceinline__ void pp_half_step(char* __restrict__ into, const __attribute__((address_space(3))) char* __restrict__ from,
+                                             char* ring, PingPongLoader<C>& ld, int kt, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+  if (kt + 1 < ld.nk) ld.issue_lo(kt + 1, into, ring);
+  PingPongFrags<C> f;
+  pp_frags_lo<C, NA>(from, wm, wn, f);
+  pp_scales<C, NA, 0>((lds_in)ring, kt, wm, wn, f);
+  pp_mul<C, 0, NA>(f, acc);
+}
+
+template <class C, int NA>
+__device__ __forceinline__ void pp_half_loop(char* lds, PingPongLoader<C>& ld, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+  using P = PingPong<C>;
+  char* const ring = lds + P::SCALES;
+  if (ld.nk > 0) ld.issue_lo(0, lds, ring);
+  for (int kt = 0; kt < ld.nk; ++kt) {
+    wait_vm<0>();
+    bar();
+    pp_half_step<C, NA>(lds + (~kt & 1) * P::STAGE, (lds_in)lds + (kt & 1) * P::STAGE, ring, ld, kt, wm, wn, acc);
+  }
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) group_tile_pp(const GroupArgs g) {
+  __shared__ __attribute__((aligned(16))) char lds[PingPong<C>::LDS];     // the only LDS object: see tile_step
+  zero_rest_rows(g, g.cols, blockIdx.x, gridDim.x, C::THREADS);
+  TileOperands t;
+  char* c_tile;
+  int c_rows, c_cols;
+  if (!tile_setup<C>(g, blockIdx.x, t, c_tile, c_rows, c_cols)) return;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WN, wn = wave % C::WN;
+  PingPongLoader<C> ld(g, t, wave, lane);
+  gf4 acc[C::NI][C::NJ];
+#pragma unroll
+  for (int i = 0; i < C::NI; ++i)
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
+  if (c_rows > C::BM / 2) pp_loop<C>(lds, ld, wave, wm, wn, acc);
+  else if (c_rows > C::BM / 4) pp_half_loop<C, PingPong<C>::NH>(lds, ld, wm, wn, acc);
+  else pp_half_loop<C, PingPong<C>::NH / 2>(lds, ld, wm, wn, acc);
   tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
 }
 
