@@ -690,27 +690,24 @@ __device__ __forceinline__ void pp_read_hi(char* __restrict__ into, const __attr
 template <class C, int I0, int NA>
 __device__ __forceinline__ void pp_mul(const PingPongFrags<C>& f, gf4 (&acc)[C::NI][C::NJ]) {
   if constexpr (C::SC == kScaleF32) {
-    // two accumulators' sums are weighted while the next two's instructions run
-    constexpr int STEPS = NA * C::NJ / 2;
-    gf4 part[2][2];
+    // Accumulator k's sum is weighted after instruction k + 2 has been issued: by then it is there without a wait
+    // (an instruction takes 32 cycles, its result 12 more), and 4 multiply-adds fit under each instruction. The
+    // order is pinned: the scheduler would gather them and wait.
+    constexpr int STEPS = NA * C::NJ;
+    gf4 part[3];
 #pragma unroll
-    for (int k = 0; k <= STEPS; ++k) {
-      if (k < STEPS) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          part[k & 1][h] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.b[(2 * k + h) % C::NJ], f.a[2 * k / C::NJ],
-                                                                           gf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0, 0, 0, 0);
-      }
-      if (k > 0) {
-        const int i = 2 * (k - 1) / C::NJ;
+    for (int k = 0; k < STEPS + 2; ++k) {
+      if (k < STEPS)
+        part[k % 3] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(f.b[k % C::NJ], f.a[k / C::NJ], gf4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0,
+                                                                     0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      if (k >= 2) {
+        const int i = (k - 2) / C::NJ, j = (k - 2) % C::NJ;
         const float s = __builtin_bit_cast(float, f.s[i]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          gf4& a = acc[I0 + i][(2 * (k - 1) + h) % C::NJ];
-#pragma unroll
-          for (int q = 0; q < 4; ++q) a[q] = fmaf(part[(k - 1) & 1][h][q], s, a[q]);
-        }
+        for (int q = 0; q < 4; ++q) acc[I0 + i][j][q] = fmaf(part[(k - 2) % 3][q], s, acc[I0 + i][j][q]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   } else if constexpr (C::SC == kScaleE8) {
 #pragma unroll
