@@ -78,23 +78,45 @@ int skinny_rows(const GroupArgs& g) {
   return g.rows <= 10 * busy ? 1 : g.rows <= 20 * busy ? 2 : g.rows <= 48 * busy ? 4 : 0;
 }
 
-// 256 x 256 tiles (one workgroup a CU) once the groups fill them and the grid fills the CUs, else 128 x 128
-// (two a CU, so that one's prologue and epilogue run under the other's loop).
+// The tile, by how many there are (`cus` workgroups run at once, or twice that) and how many rows a group has:
+//
+//   Large    256 x 256, ping-pong, one a CU: groups that fill it and a grid that nearly fills the CUs (16 groups of
+//            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1)
+//   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: grids of more than
+//            a round (32 fp8 groups of 64 rows, 4096 x 2048: 64.8 us, Low 71.6, Large 74.6)
+//   Deep     128 x 128, 8 waves, a ring of four: less than a round, where a workgroup's own latency is the time
+//            (fp8 256 x 8192 x 8192: 44.3 us, Low 54.9, Small 63.8)
+//   Low      64 x 128, a ring of three: few rows, or few tiles (fp8 128 x 4096 x 4096: 16.3 us, Deep 20.2, Small 23.1;
+//            20 groups of 30 rows, 1024 x 1024: 12.7, 13.7, 15.2)
+//
+// A weight gradient has whole tiles whatever the groups are; with short reductions the stores are the time, and two
+// workgroups a CU overlap them (20 groups of 30 rows, 1024 x 1024: Small 15.5 us, Large 19.8).
 template <int DT, int SC, bool ATR, bool BTR>
 int dispatch_tile(const GroupArgs& g, hipStream_t s) {
-  using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
   using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
+  using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
   if (!dma_ready(g)) return launch_tile<TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2>, kTileRegs>(g, s);
-  if constexpr (!ATR && !BTR) {
-    switch (skinny_rows(g)) {
-      case 1: return skinny_columns<DT, SC, 1>(g, s);
-      case 2: return skinny_columns<DT, SC, 2>(g, s);
-      case 4: return skinny_columns<DT, SC, 4>(g, s);
+  const int cus = device_cu_count(s);
+  const bool large_fills = 5 * tile_grid<Large>(g) >= 4 * cus;
+  if constexpr (ATR) {
+    if (large_fills && g.red >= 128ll * g.experts) return launch_tile<Large, kTilePingPong>(g, s);
+    return launch_tile<Small, kTileDma>(g, s);
+  } else {
+    using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 128, 4>;
+    using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 128, 3>;
+    if constexpr (!BTR) {
+      switch (skinny_rows(g)) {
+        case 1: return skinny_columns<DT, SC, 1>(g, s);
+        case 2: return skinny_columns<DT, SC, 2>(g, s);
+        case 4: return skinny_columns<DT, SC, 4>(g, s);
+      }
     }
+    const long long per_group = g.rows / g.experts, small = tile_grid<Small>(g);
+    if (large_fills && per_group > 128) return launch_tile<Large, kTilePingPong>(g, s);
+    if (small > cus) return launch_tile<Small, kTileDma>(g, s);
+    if (4 * small <= cus || per_group <= 64) return launch_tile<Low, kTileDma>(g, s);
+    return launch_tile<Deep, kTileDma>(g, s);
   }
-  const long long per_group = g.mode == kModeWgrad ? g.rows : g.rows / g.experts;
-  if (per_group > 128 && tile_grid<Large>(g) >= 256) return launch_tile<Large, kTilePingPong>(g, s);
-  return launch_tile<Small, kTileDma>(g, s);
 }
 
 template <int DT>

@@ -21,9 +21,12 @@ struct TileCfg {
   static constexpr int STAGE = OPA + OPB + SCB;
   static constexpr int LDS = NBUF * STAGE;
   static_assert(LDS <= 160 * 1024, "one CU's LDS");
-  static constexpr int EU = WM * WN / 4 * (160 * 1024 / LDS >= 2 ? 2 : 1);   // waves a SIMD that the ring leaves room for
+  static constexpr int RESIDENT = 160 * 1024 / LDS;                          // workgroups a CU that the ring leaves room for
+  static constexpr int EU = WM * WN / 4 * (RESIDENT < 2 ? 1 : RESIDENT > 3 ? 4 : RESIDENT);   // waves a SIMD to plan registers for
   static_assert(!(DT == kFp8 && (ATR || BTR)), "fp8 operands are K-major");
   static_assert((DT == kFp8) == (SC != kScaleNone), "fp8 has scales");
+  static_assert(NBUF <= 4, "the ring's counted waits");
+  static_assert(BN >= 128 && (!ATR || BM >= 128), "the chunk permutations reach over 256 bytes of a row");
   static_assert(PB == 128 || (PB == 64 && DT != kFp8), "an fp8 panel is one scale block");
 };
 
@@ -514,7 +517,9 @@ __device__ __forceinline__ void tile_loop(char* lds, TileLoader<C>& ld, int wm, 
   constexpr int PT = TileLoader<C>::PT;
   int buf = 0;
   for (int kt = 0; kt < ld.nk; ++kt) {
-    if (C::NBUF == 3 && ld.nk - 1 - kt >= 1) wait_vm<PT>();
+    const int ahead = ld.nk - 1 - kt;                 // panels younger than kt that may stay in flight
+    if (C::NBUF >= 4 && ahead >= 2) wait_vm<2 * PT>();
+    else if (C::NBUF >= 3 && ahead >= 1) wait_vm<PT>();
     else wait_vm<0>();
     bar();
     tile_step<C, NA>(lds + (buf == 0 ? C::NBUF - 1 : buf - 1) * C::STAGE, (lds_in)lds + buf * C::STAGE, ld, kt + C::NBUF - 1,
@@ -547,9 +552,9 @@ group_tile_dma(const GroupArgs g) {
   for (int p = 0; p < C::NBUF - 1; ++p)
     if (p < ld.nk) ld.issue(p, lds + p * C::STAGE);
   // a group's last tile, or a part of a tile, is as long as its rows, in quarters
-  if (c_rows > C::BM / 2) tile_loop<C, C::NI>(lds, ld, wm, wn, acc);
-  else if (c_rows > C::BM / 4) tile_loop<C, C::NI / 2>(lds, ld, wm, wn, acc);
-  else tile_loop<C, C::NI / 4>(lds, ld, wm, wn, acc);
+  if (C::NI < 4 || c_rows > C::BM / 2) tile_loop<C, C::NI>(lds, ld, wm, wn, acc);
+  else if (c_rows > C::BM / 4) tile_loop<C, (C::NI + 1) / 2>(lds, ld, wm, wn, acc);
+  else tile_loop<C, (C::NI + 3) / 4>(lds, ld, wm, wn, acc);
   tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
 }
 
