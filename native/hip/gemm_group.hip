@@ -64,30 +64,29 @@ int skinny_columns(const GroupArgs& g, hipStream_t s) {
   if (tiles_m * ((g.cols + 63) / 64) > 512) return launch_skinny<SkinnyCfg<DT, SC, MT, 4, 4, 1>>(g, tiles_m, s);
   if constexpr (MT == 1)
     if (tiles_m * ((g.cols + 31) / 32) < 256) return launch_skinny<SkinnyCfg<DT, SC, 1, 1, 8, 1>>(g, tiles_m, s);
-  if constexpr (MT <= 2) return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1>>(g, tiles_m, s);
-  else return skinny_columns<DT, SC, 2>(g, s);
+  return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1>>(g, tiles_m, s);
 }
 
-// Few rows a busy group: the skinny kernel, its tile as high as the groups are on average (they are uneven, so not
-// much higher: 64 experts of 8 rows on average run 93.8 us with 16-row tiles, 100.9 with 32; 16 of 32 rows 95, 73.6 and
-// with 64-row tiles 66.5; the tiled kernel 76.4). 0: not for this shape.
+// Few rows: the skinny kernel with tiles of 16 rows, or of 32 for a single group of 17 to 64 (8192 x 8192 fp8, 32 rows:
+// 16-row tiles 30 us, 32-row ones 22.5; 64 rows of 4096 x 4096: 15.6, 12.2). Groups of more than 12 rows on average
+// are for the tiled kernel (16 of 16 rows, 4096 x 2048: 65.5 us, Low 60.4; 64 of 8 rows: 93.8, Small 110.5). 0: not here.
 int skinny_rows(const GroupArgs& g) {
   if (g.mode != kModeForward) return 0;
   if (g.offsets == nullptr) return g.rows <= 16 ? 1 : g.rows <= 64 ? 2 : 0;
   const long long busy = g.experts < g.rows ? g.experts : g.rows;
-  return g.rows <= 10 * busy ? 1 : g.rows <= 20 * busy ? 2 : g.rows <= 48 * busy ? 4 : 0;
+  return g.rows <= 12 * busy ? 1 : 0;
 }
 
 // The tile, by how many there are (`cus` workgroups run at once, or twice that) and how many rows a group has:
 //
 //   Large    256 x 256, ping-pong, one a CU: groups that fill it and a grid that nearly fills the CUs (16 groups of
 //            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1)
-//   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: grids of more than
-//            a round (32 fp8 groups of 64 rows, 4096 x 2048: 64.8 us, Low 71.6, Large 74.6)
-//   Deep     128 x 128, 8 waves, a ring of four: less than a round, where a workgroup's own latency is the time
-//            (fp8 256 x 8192 x 8192: 44.3 us, Low 54.9, Small 63.8)
+//   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: grids of nearly two
+//            rounds or more (32 fp8 groups of 64 rows, 4096 x 2048: 64.8 us, Low 71.6, Large 74.6)
+//   Deep     128 x 128, 8 waves, a ring of four: smaller grids, where a workgroup's own latency is the time (fp8 256 x
+//            8192 x 8192: 44.3 us, Low 54.9, Small 63.8; 32 groups of 64 rows, 1024 x 2048: 37.2, 42.2, 45.9)
 //   Low      64 x 128, a ring of three: few rows, or few tiles (fp8 128 x 4096 x 4096: 16.3 us, Deep 20.2, Small 23.1;
-//            20 groups of 30 rows, 1024 x 1024: 12.7, 13.7, 15.2)
+//            20 groups of 30 rows, 1024 x 1024: 12.7, 13.7, 15.2; 32 fp8 groups of 32, 2048 x 2048: 32.1, 41.8, 34.6)
 //
 // A weight gradient has whole tiles whatever the groups are; with short reductions the stores are the time, and two
 // workgroups a CU overlap them (20 groups of 30 rows, 1024 x 1024: Small 15.5 us, Large 19.8).
@@ -108,13 +107,13 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
       switch (skinny_rows(g)) {
         case 1: return skinny_columns<DT, SC, 1>(g, s);
         case 2: return skinny_columns<DT, SC, 2>(g, s);
-        case 4: return skinny_columns<DT, SC, 4>(g, s);
       }
     }
     const long long per_group = g.rows / g.experts, small = tile_grid<Small>(g);
     if (large_fills && per_group > 128) return launch_tile<Large, kTilePingPong>(g, s);
-    if (small > cus) return launch_tile<Small, kTileDma>(g, s);
-    if (4 * small <= cus || per_group <= 64) return launch_tile<Low, kTileDma>(g, s);
+    const bool near_two_rounds = 4 * small > 7 * cus;
+    if (4 * small <= cus || per_group <= (near_two_rounds ? 48 : 32)) return launch_tile<Low, kTileDma>(g, s);
+    if (near_two_rounds) return launch_tile<Small, kTileDma>(g, s);
     return launch_tile<Deep, kTileDma>(g, s);
   }
 }
