@@ -94,7 +94,7 @@ template <int DT, int SC, bool ATR, bool BTR>
 int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
   using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
-  if (!dma_ready(g)) return launch_tile<TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2>, kTileRegs>(g, s);
+  if (!dma_ready(g)) return launch_tile<TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>, kTileRegs>(g, s);
   const int cus = device_cu_count(s);
   const bool large_fills = 5 * tile_grid<Large>(g) >= 4 * cus;
   if constexpr (ATR) {

@@ -199,28 +199,35 @@ __device__ __forceinline__ void tile_compute(lds_in lds, int wm, int wn, gf4 (&a
 }
 
 // A panel into LDS through registers: any alignment, any leading dimension, what lies outside reads as zero.
+// Loaded ahead, stored when its buffer is free.
 template <class C, bool TR, int ROWS>
-__device__ __forceinline__ void stage_regs(char* lds, const char* base, long long ld_b, int rows, int col0, int cols, int red,
-                                           int kt) {
-  constexpr int ES = C::ES;
-  if constexpr (TR) {
-    constexpr int CPR = ROWS * 2 / 16;                 // chunks a reduction row
-    for (int i = threadIdx.x; i < C::KT * CPR; i += C::THREADS) {
-      const int r = i / CPR, q = i % CPR, k = kt * C::KT + r;
-      gi4 v = {0, 0, 0, 0};
-      if (k < red) v = load_chunk<ES>(base + (size_t)k * ld_b, col0 + q * 8, cols);
-      *(gi4*)(lds + rm_at<ROWS>(r, q)) = v;
-    }
-  } else {
-    constexpr int CPR = C::PB / 16;
-    for (int i = threadIdx.x; i < ROWS * CPR; i += C::THREADS) {
-      const int r = i / CPR, q = i % CPR;
-      gi4 v = {0, 0, 0, 0};
-      if (r < rows) v = load_chunk<ES>(base + (size_t)r * ld_b, kt * C::KT + q * (16 / ES), red);
-      *(gi4*)(lds + km_at<C::PB>(r, q)) = v;
+struct PanelRegs {
+  static constexpr int ES = C::ES, CPR = TR ? ROWS / 8 : C::PB / 16;         // chunks a row
+  static constexpr int N = (TR ? C::KT : ROWS) * CPR / C::THREADS;
+  static_assert(N * C::THREADS == (TR ? C::KT : ROWS) * CPR, "whole chunks a thread");
+  gi4 v[N];
+
+  __device__ __forceinline__ void load(const char* base, long long ld_b, int rows, int col0, int cols, int red, int kt) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = i * C::THREADS + threadIdx.x, r = at / CPR, q = at % CPR;
+      v[i] = gi4{0, 0, 0, 0};
+      if constexpr (TR) {
+        const int k = kt * C::KT + r;
+        if (k < red) v[i] = load_chunk<ES>(base + (size_t)k * ld_b, col0 + q * 8, cols);
+      } else {
+        if (r < rows) v[i] = load_chunk<ES>(base + (size_t)r * ld_b, kt * C::KT + q * (16 / ES), red);
+      }
     }
   }
-}
+  __device__ __forceinline__ void store(char* lds) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = i * C::THREADS + threadIdx.x, r = at / CPR, q = at % CPR;
+      *(gi4*)(lds + (TR ? rm_at<ROWS>(r, q) : km_at<C::PB>(r, q))) = v[i];
+    }
+  }
+};
 
 // The scales of a panel's block into LDS: one 32-bit word for each row of the tile, then one for each 128
 // columns (float32, or the e8m0 byte). Rows and columns that do not exist get zero.
@@ -827,28 +834,42 @@ __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu
   tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
 }
 
+// The form for operands that LDS-DMA cannot take (16-byte chunks that are not whole or not aligned): panels go
+// through registers, the next one's loads in flight under the multiplication, into the other of two buffers.
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) group_tile_regs(const GroupArgs g) {
-  __shared__ __attribute__((aligned(16))) char lds[C::STAGE];
+  static_assert(C::NBUF == 2, "one barrier a panel");
+  __shared__ __attribute__((aligned(16))) char lds[C::LDS];
   zero_rest_rows(g, g.cols, blockIdx.x, gridDim.x, C::THREADS);
   TileOperands t;
   char* c_tile;
   int c_rows, c_cols;
   if (!tile_setup<C>(g, blockIdx.x, t, c_tile, c_rows, c_cols)) return;
-  const int wave = threadIdx.x >> 6, wm = wave / C::WN, wn = wave % C::WN;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WN, wn = wave % C::WN;
   gf4 acc[C::NI][C::NJ];
 #pragma unroll
   for (int i = 0; i < C::NI; ++i)
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
+  PanelRegs<C, C::ATR, C::BM> a;
+  PanelRegs<C, C::BTR, C::BN> b;
   const int nk = (t.red + C::KT - 1) / C::KT;
-  for (int kt = 0; kt < nk; ++kt) {
-    stage_regs<C, C::ATR, C::BM>(lds, t.a, t.lda_b, t.a_rows, t.a_col0, t.a_cols, t.red, kt);
-    stage_regs<C, C::BTR, C::BN>(lds + C::OPA, t.b, t.ldb_b, t.b_rows, t.b_col0, t.b_cols, t.red, kt);
-    stage_scales<C>(lds + C::OPA + C::OPB, g, t, kt);
-    __syncthreads();
-    tile_compute<C, C::NI>((lds_in)lds, wm, wn, acc);
-    __syncthreads();
+  for (int kt = -1; kt < nk; ++kt) {
+    char* const buf = lds + (kt & 1) * C::STAGE;
+    if (kt >= 0) {
+      a.store(buf);
+      b.store(buf + C::OPA);
+      stage_scales<C>(buf + C::OPA + C::OPB, g, t, kt);
+      __syncthreads();
+    }
+    if (kt + 1 < nk) {
+      a.load(t.a, t.lda_b, t.a_rows, t.a_col0, t.a_cols, t.red, kt + 1);
+      b.load(t.b, t.ldb_b, t.b_rows, t.b_col0, t.b_cols, t.red, kt + 1);
+    }
+    if (kt >= 0) {
+      if (c_rows > C::BM / 2) tile_compute<C, C::NI>((lds_in)buf, wm, wn, acc);
+      else tile_compute<C, C::NI / 2>((lds_in)buf, wm, wn, acc);
+    }
   }
   tile_store<C>(g, c_tile, c_rows, c_cols, wm, wn, acc);
 }

@@ -29,7 +29,6 @@ struct QuantArgs {
 
 namespace {
 
-typedef unsigned int qu4 __attribute__((ext_vector_type(4)));
 typedef unsigned int qu2 __attribute__((ext_vector_type(2)));
 
 constexpr int QT = 256;                // threads
@@ -49,19 +48,13 @@ __device__ __forceinline__ float raw_get(const Raw8<DT>& r, int i) {
   return (float)__builtin_bit_cast(_Float16, (unsigned short)h);
 }
 
-// elements [c, c + 8) of a row, zeros from `cols` on; WIDE: whole and 16-byte aligned
+// elements [c, c + 8) of a row, zeros from `cols` on; any alignment
 template <int DT>
-__device__ __forceinline__ Raw8<DT> raw_load(const char* row, int c, int cols, bool wide) {
+__device__ __forceinline__ Raw8<DT> raw_load(const char* row, int c, int cols) {
   constexpr int ES = DT == kInFp32 ? 4 : 2;
   Raw8<DT> r;
-  if (wide && c + 8 <= cols) {
-    const qu4* p = (const qu4*)(row + (size_t)c * ES);
-#pragma unroll
-    for (int i = 0; i < Raw8<DT>::W / 4; ++i) {
-      const qu4 v = p[i];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) r.w[4 * i + k] = v[k];
-    }
+  if (c + 8 <= cols) {
+    __builtin_memcpy(r.w, __builtin_assume_aligned(row + (size_t)c * ES, ES), sizeof(r.w));
   } else {
 #pragma unroll
     for (int i = 0; i < Raw8<DT>::W; ++i) r.w[i] = 0;
@@ -140,9 +133,9 @@ __device__ __forceinline__ qu2 quantize8(const Raw8<DT>& r, const Scale& s) {
   return o;
 }
 
-__device__ __forceinline__ void store8(unsigned char* row, int c, int cols, bool wide, qu2 v) {
-  if (wide && c + 8 <= cols) {
-    *(qu2*)(row + c) = v;
+__device__ __forceinline__ void store8(unsigned char* row, int c, int cols, qu2 v) {
+  if (c + 8 <= cols) {
+    __builtin_memcpy(row + c, &v, 8);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -175,16 +168,14 @@ __global__ void __launch_bounds__(QT) quantize_row_blocks(const QuantArgs a) {
   const int kb = (int)(id - row * per_row) * 4 + (lane >> 4);
   const int batch = (int)(row / a.rows), r = (int)(row - (long long)batch * a.rows);
   const char* x = (const char*)a.x + ((size_t)batch * a.batch_stride + (size_t)r * a.ld) * ES;
-  const bool wide_in = (((uintptr_t)a.x | (uintptr_t)(a.ld * ES) | (uintptr_t)(a.batch_stride * ES)) & 15) == 0;
-  const bool wide_out = (((uintptr_t)a.q | (uintptr_t)a.cols) & 7) == 0;
   const int c = kb * 128 + (lane & 15) * 8;
-  const Raw8<DT> v = raw_load<DT>(x, c, a.cols, wide_in);
+  const Raw8<DT> v = raw_load<DT>(x, c, a.cols);
   unsigned int m = amax8<DT>(v);
 #pragma unroll
   for (int d = 1; d < 16; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
   if (kb >= kb_count) return;
   const Scale s = make_scale<E8>(m);
-  store8(a.q + (size_t)row * a.cols, c, a.cols, wide_out, quantize8<DT, E8>(v, s));
+  store8(a.q + (size_t)row * a.cols, c, a.cols, quantize8<DT, E8>(v, s));
   if ((lane & 15) == 0) store_scale<E8>(a.s, (size_t)row * kb_count + kb, s);
 }
 
@@ -197,15 +188,13 @@ __global__ void __launch_bounds__(QT) quantize_square_blocks(const QuantArgs a) 
   const int kb = blockIdx.x % kb_count;
   const int rest = blockIdx.x / kb_count, rb = rest % rb_count, batch = rest / rb_count;
   const char* x = (const char*)a.x + (size_t)batch * a.batch_stride * ES;
-  const bool wide_in = (((uintptr_t)a.x | (uintptr_t)(a.ld * ES) | (uintptr_t)(a.batch_stride * ES)) & 15) == 0;
-  const bool wide_out = (((uintptr_t)a.q | (uintptr_t)a.cols) & 7) == 0;
   const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
   Raw8<DT> v[8];
   unsigned int m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + 16 * i;
-    v[i] = raw_load<DT>(x + (size_t)(r < a.rows ? r : 0) * a.ld * ES, c, r < a.rows ? a.cols : 0, wide_in);
+    v[i] = raw_load<DT>(x + (size_t)(r < a.rows ? r : 0) * a.ld * ES, c, r < a.rows ? a.cols : 0);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, amax8<DT>(v[i]));
@@ -218,7 +207,7 @@ __global__ void __launch_bounds__(QT) quantize_square_blocks(const QuantArgs a) 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + 16 * i;
-    if (r < a.rows) store8(a.q + ((size_t)batch * a.rows + r) * a.cols, c, a.cols, wide_out, quantize8<DT, E8>(v[i], s));
+    if (r < a.rows) store8(a.q + ((size_t)batch * a.rows + r) * a.cols, c, a.cols, quantize8<DT, E8>(v[i], s));
   }
   if (threadIdx.x == 0) store_scale<E8>(a.s, blockIdx.x, s);
 }
