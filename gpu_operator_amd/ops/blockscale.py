@@ -101,7 +101,7 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
                0 if offsets is None else offsets.data_ptr(),
                _row_stride((m, k), sa), _row_stride((n, k), sb), ldc, sb[0] if dims == 3 else 0, 0,
                ssa[0], ssa[1], ssb[0] if dims == 3 else 0, ssb[-2], ssb[-1],
-               m, n, k, e, MODE_FORWARD, 2, 1 if a_scale.dtype == torch.float32 else 2, rest)
+               m, n, k, e, MODE_FORWARD, 2, 1 if a_scale.dtype == torch.float32 else 2, rest, 0)
     return out
 
 

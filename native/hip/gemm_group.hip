@@ -14,36 +14,69 @@ long long tile_grid(const GroupArgs& g) {
   return tiles_m * tiles_n;
 }
 
-enum TileKernel { kTileRegs, kTileDma, kTilePingPong };
+enum TileKernel { kTileDma, kTilePingPong };
 
 template <class C, TileKernel KERNEL>
 int launch_tile(const GroupArgs& g, hipStream_t s) {
   GroupArgs a = g;
-  // the DMA kernels cut the last tiles into parts: at most one more round of workgroups
-  a.slots = KERNEL != kTileRegs && g.mode != kModeWgrad ? device_cu_count(s) * (160 * 1024 / C::LDS) : 0;
+  // the last tiles are cut into parts: at most one more round of workgroups
+  a.slots = g.mode != kModeWgrad ? device_cu_count(s) * (160 * 1024 / C::LDS) : 0;
   const long long grid = tile_grid<C>(g) + a.slots;
   if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
   if (grid == 0) return 0;
   if constexpr (KERNEL == kTilePingPong) hipLaunchKernelGGL((group_tile_pp<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
-  else if constexpr (KERNEL == kTileDma) hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
-  else hipLaunchKernelGGL((group_tile_regs<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
+  else hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
   return (int)hipGetLastError();
 }
 
-// Whether every 16-byte chunk that a tile reads is whole and aligned, and a tile's lane offsets fit a buffer's
-// 2 GiB: what LDS-DMA needs. (A K-major operand's chunks lie along the reduction, a reduction-major one's along
-// its rows.)
+// What amdgo_gemm_group answers, having launched nothing, where the operands have to be laid out first
+// (amdgo_group_pack): see dma_ready.
+constexpr int kNeedsPacking = -1;
+
+// Whether a tile's lane offsets fit a buffer's 2 GiB.
+bool offsets_fit(const GroupArgs& g) {
+  const long long es = g.dtype == kFp8 ? 1 : 2, kb = g.red / kScaleBlock + 1;
+  const long long across = ((long long)(g.rows > g.cols ? g.rows : g.cols) + g.red) * es;
+  return g.lda * es * 256 + across < 0x7fffffffll && g.ldb * es * 256 + across < 0x7fffffffll &&
+         (g.scale == kScaleNone || ((g.as_row * 256 + g.as_k * kb) * 4 < 0x7fffffffll &&
+                                    (g.bs_row * 4 + g.bs_k * kb) * 4 < 0x7fffffffll));
+}
+
+// Whether every 16-byte chunk that a tile reads is whole and aligned too: what LDS-DMA needs. (A K-major operand's
+// chunks lie along the reduction, a reduction-major one's along its rows.)
 bool dma_ready(const GroupArgs& g) {
   const long long es = g.dtype == kFp8 ? 1 : 2;
   const bool a_tr = g.mode == kModeWgrad, b_tr = g.mode != kModeForward;
-  const auto fits = [&](const void* p, long long ld, long long batch, bool tr, long long width) {
-    return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(batch * es) | (uintptr_t)((tr ? width : g.red) * es)) & 15) == 0 &&
-           ld * es * 256 + (width + g.red) * es < 0x7fffffffll;
+  const auto whole = [&](const void* p, long long ld, long long batch, bool tr, long long width) {
+    const long long along = tr ? (g.padded ? 0 : width) : g.red;
+    return (((uintptr_t)p | (uintptr_t)(ld * es) | (uintptr_t)(batch * es) | (uintptr_t)(along * es)) & 15) == 0;
   };
-  if (!fits(g.a, g.lda, 0, a_tr, g.rows) || !fits(g.b, g.ldb, g.b_expert, b_tr, g.cols)) return false;
-  const long long kb = g.red / kScaleBlock + 1;
-  return g.scale == kScaleNone || ((g.as_row * 256 + g.as_k * kb) * 4 < 0x7fffffffll &&
-                                   (g.bs_row * 4 + g.bs_k * kb) * 4 < 0x7fffffffll);
+  return whole(g.a, g.lda, 0, a_tr, g.rows) && whole(g.b, g.ldb, g.b_expert, b_tr, g.cols) && offsets_fit(g);
+}
+
+// A matrix [batches, rows, row_bytes] of any strides to [batches, to_rows, to_bytes] (to_bytes a multiple of 16), zeros
+// where the source has nothing. A workgroup takes whole rows, 16 bytes a lane.
+__global__ void __launch_bounds__(256) pack_rows(const char* __restrict__ from, char* __restrict__ to, long long ld_b,
+                                                 long long batch_b, int rows, long long row_bytes, int to_rows, long long to_bytes) {
+  const int batch = blockIdx.x / to_rows, r = blockIdx.x - batch * to_rows;
+  const char* src = from + (size_t)batch * batch_b + (size_t)r * ld_b;
+  char* dst = to + (size_t)blockIdx.x * to_bytes;
+  for (long long at = threadIdx.x * 16ll; at < to_bytes; at += 256 * 16) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (r < rows) {
+      if (at + 16 <= row_bytes) {
+        __builtin_memcpy(&v, src + at, 16);
+      } else {
+        union { unsigned char b[16]; uint4 v; } u;
+        u.v = v;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (at + i < row_bytes) u.b[i] = (unsigned char)src[at + i];
+        v = u.v;
+      }
+    }
+    *(uint4*)(dst + at) = v;
+  }
 }
 
 template <class C>
@@ -65,6 +98,14 @@ int skinny_columns(const GroupArgs& g, hipStream_t s) {
   if constexpr (MT == 1)
     if (tiles_m * ((g.cols + 31) / 32) < 256) return launch_skinny<SkinnyCfg<DT, SC, 1, 1, 8, 1>>(g, tiles_m, s);
   return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1>>(g, tiles_m, s);
+}
+
+// The same for operands without whole aligned chunks.
+template <int DT, int SC, int MT>
+int skinny_unaligned(const GroupArgs& g, hipStream_t s) {
+  if (!offsets_fit(g)) return kNeedsPacking;
+  const long long tiles_m = group_tile_bound(g.rows, g.experts, g.offsets != nullptr, 16 * MT);
+  return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1, false>>(g, tiles_m, s);
 }
 
 // Few rows: the skinny kernel with tiles of 16 rows, or of 32 for a single group of 17 to 64 (8192 x 8192 fp8, 32 rows:
@@ -94,7 +135,14 @@ template <int DT, int SC, bool ATR, bool BTR>
 int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
   using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
-  if (!dma_ready(g)) return launch_tile<TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>, kTileRegs>(g, s);
+  const bool ready = dma_ready(g);
+  if constexpr (!ATR && !BTR) {
+    switch (skinny_rows(g)) {
+      case 1: return ready ? skinny_columns<DT, SC, 1>(g, s) : skinny_unaligned<DT, SC, 1>(g, s);
+      case 2: return ready ? skinny_columns<DT, SC, 2>(g, s) : skinny_unaligned<DT, SC, 2>(g, s);
+    }
+  }
+  if (!ready) return kNeedsPacking;
   const int cus = device_cu_count(s);
   const bool large_fills = 5 * tile_grid<Large>(g) >= 4 * cus;
   if constexpr (ATR) {
@@ -103,12 +151,6 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   } else {
     using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 128, 4>;
     using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 128, 3>;
-    if constexpr (!BTR) {
-      switch (skinny_rows(g)) {
-        case 1: return skinny_columns<DT, SC, 1>(g, s);
-        case 2: return skinny_columns<DT, SC, 2>(g, s);
-      }
-    }
     const long long per_group = g.rows / g.experts, small = tile_grid<Small>(g);
     if (large_fills && per_group > 128) return launch_tile<Large, kTilePingPong>(g, s);
     const bool near_two_rounds = 4 * small > 7 * cus;
@@ -148,6 +190,18 @@ int amdgo_gemm_group(const void* args, hipStream_t s) {
   if (g.dtype == kBf16) return dispatch16<kBf16>(g, s);
   if (g.dtype == kFp16) return dispatch16<kFp16>(g, s);
   return (int)hipErrorInvalidValue;
+}
+
+// `to`: batches * to_rows rows of to_bytes, 16-byte aligned.
+int amdgo_group_pack(const void* from, void* to, long long ld_b, long long batch_b, int batches, int rows, long long row_bytes,
+                     int to_rows, long long to_bytes, hipStream_t s) {
+  const long long grid = (long long)batches * to_rows;
+  if (grid < 0 || grid > 0x7fffffff || to_rows < rows || to_bytes < row_bytes || (to_bytes & 15) || ((uintptr_t)to & 15))
+    return (int)hipErrorInvalidValue;
+  if (grid == 0 || to_bytes == 0) return 0;
+  hipLaunchKernelGGL(pack_rows, dim3((unsigned)grid), dim3(256), 0, s, (const char*)from, (char*)to, ld_b, batch_b, rows, row_bytes,
+                     to_rows, to_bytes);
+  return (int)hipGetLastError();
 }
 
 }  // extern "C"

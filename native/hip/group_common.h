@@ -34,7 +34,8 @@ struct GroupArgs {
   long long as_row, as_k, bs_expert, bs_row, bs_k;
   int rows, cols, red, experts;              // ragged extent: `rows` (forward, dgrad) or `red` (wgrad)
   int mode, dtype, scale, zero_rest;         // zero_rest: rows that no expert owns are written as zeros
-  int slots, reserved;                       // workgroups that run at once; set by the dispatch
+  int padded;                                // rows are readable to their next multiple of 16 bytes
+  int slots;                                 // workgroups that run at once; set by the dispatch
 };
 
 namespace {

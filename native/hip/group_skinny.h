@@ -10,8 +10,9 @@
 
 #include "group_tile.h"
 
-template <int DT_, int SC_, int MT_, int NJ_, int KW_, int U_>
+template <int DT_, int SC_, int MT_, int NJ_, int KW_, int U_, bool ALIGNED_ = true>
 struct SkinnyCfg {
+  static constexpr bool ALIGNED = ALIGNED_;      // whole, aligned 16-byte chunks (else they are loaded piece by piece)
   static constexpr int DT = DT_, SC = SC_, MT = MT_, NJ = NJ_, KW = KW_, U = U_;
   static constexpr int ES = DT == kFp8 ? 1 : 2;
   static constexpr int ROWS = 16 * MT, COLS = 16 * NJ, THREADS = 64 * KW;
@@ -106,11 +107,23 @@ __global__ void __launch_bounds__(C::THREADS) group_skinny(const GroupArgs g) {
   const unsigned as_k = (unsigned)(g.as_k * S), bs_k = (unsigned)(g.bs_k * S);
   const int nk = (g.red + 128 / C::ES - 1) / (128 / C::ES);
   // panel k: `at` is added to offsets that may already be past the end; they stay there (both under 2^31)
+  const char* const pa = (const char*)g.a + (size_t)rt.row0 * g.lda * C::ES;
+  const char* const pb = (const char*)g.b + ((size_t)rt.expert * g.b_expert + (size_t)n0 * g.ldb) * C::ES;
   const auto load = [&](SkinnyPanel<C>& p, int k) {
     const unsigned at = (unsigned)k * 128u;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const bool in = at + (unsigned)(q0 + 4 * h) * 16u < bytes;
+      if constexpr (!C::ALIGNED) {
+        const int from = (int)(at / C::ES) + (q0 + 4 * h) * (16 / C::ES);
+#pragma unroll
+        for (int m = 0; m < C::MT; ++m)
+          p.a[m][h] = load_chunk<C::ES>(pa + (size_t)(m * 16 + l16) * g.lda * C::ES, from, m * 16 + l16 < rows ? g.red : 0);
+#pragma unroll
+        for (int j = 0; j < C::NJ; ++j)
+          p.b[j][h] = load_chunk<C::ES>(pb + (size_t)(j * 16 + l16) * g.ldb * C::ES, from, j * 16 + l16 < cols ? g.red : 0);
+        continue;
+      }
 #pragma unroll
       for (int m = 0; m < C::MT; ++m) p.a[m][h] = buffer_chunk(ra, in ? oa[m] + at + h * 64u : kNowhere);
 #pragma unroll

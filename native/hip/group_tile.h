@@ -198,57 +198,6 @@ __device__ __forceinline__ void tile_compute(lds_in lds, int wm, int wn, gf4 (&a
   }
 }
 
-// A panel into LDS through registers: any alignment, any leading dimension, what lies outside reads as zero.
-// Loaded ahead, stored when its buffer is free.
-template <class C, bool TR, int ROWS>
-struct PanelRegs {
-  static constexpr int ES = C::ES, CPR = TR ? ROWS / 8 : C::PB / 16;         // chunks a row
-  static constexpr int N = (TR ? C::KT : ROWS) * CPR / C::THREADS;
-  static_assert(N * C::THREADS == (TR ? C::KT : ROWS) * CPR, "whole chunks a thread");
-  gi4 v[N];
-
-  __device__ __forceinline__ void load(const char* base, long long ld_b, int rows, int col0, int cols, int red, int kt) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = i * C::THREADS + threadIdx.x, r = at / CPR, q = at % CPR;
-      v[i] = gi4{0, 0, 0, 0};
-      if constexpr (TR) {
-        const int k = kt * C::KT + r;
-        if (k < red) v[i] = load_chunk<ES>(base + (size_t)k * ld_b, col0 + q * 8, cols);
-      } else {
-        if (r < rows) v[i] = load_chunk<ES>(base + (size_t)r * ld_b, kt * C::KT + q * (16 / ES), red);
-      }
-    }
-  }
-  __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = i * C::THREADS + threadIdx.x, r = at / CPR, q = at % CPR;
-      *(gi4*)(lds + (TR ? rm_at<ROWS>(r, q) : km_at<C::PB>(r, q))) = v[i];
-    }
-  }
-};
-
-// The scales of a panel's block into LDS: one 32-bit word for each row of the tile, then one for each 128
-// columns (float32, or the e8m0 byte). Rows and columns that do not exist get zero.
-template <class C>
-__device__ __forceinline__ void stage_scales(char* lds, const GroupArgs& g, const TileOperands& t, int kt) {
-  if constexpr (C::SC != kScaleNone) {
-    for (int i = threadIdx.x; i < C::BM + C::BN / kScaleBlock; i += C::THREADS) {
-      int v = 0;
-      if (i < C::BM) {
-        const long long at = i * g.as_row + kt * g.as_k;
-        if (i < t.a_rows) v = C::SC == kScaleF32 ? ((const int*)t.as)[at] : (int)((const unsigned char*)t.as)[at];
-      } else {
-        const int n = i - C::BM;
-        const long long at = n * g.bs_row + kt * g.bs_k;
-        if (n * kScaleBlock < t.b_rows) v = C::SC == kScaleF32 ? ((const int*)t.bs)[at] : (int)((const unsigned char*)t.bs)[at];
-      }
-      *(int*)(lds + i * 4) = v;
-    }
-  }
-}
-
 // The tile of this workgroup: what it reads and where it writes. False: nothing to do.
 template <class C>
 __device__ __forceinline__ bool tile_setup(const GroupArgs& g, int block, TileOperands& t, char*& c_tile, int& c_rows, int& c_cols) {
@@ -315,45 +264,17 @@ __device__ __forceinline__ bool tile_setup(const GroupArgs& g, int block, TileOp
   return true;
 }
 
-// Accumulator [i][j] of a lane: row 16 i + (lane & 15), columns 16 j + 4 (lane >> 4) + 0..3 of the wave's part
-// (B is the matrix instruction's first operand, so a lane's four values lie along a row of C).
-template <class C>
-__device__ __forceinline__ void tile_store(const GroupArgs& g, char* c_tile, int c_rows, int c_cols, int wm, int wn,
-                                           const gf4 (&acc)[C::NI][C::NJ]) {
-  constexpr int OUT = C::DT == kFp16 ? kFp16 : kBf16;
-  const int lane = threadIdx.x & 63;
-  const bool wide = ((uintptr_t)g.c & 7) == 0 && (g.ldc & 3) == 0 && (g.c_expert & 3) == 0;
-#pragma unroll
-  for (int i = 0; i < C::NI; ++i) {
-    const int r = (i * C::WM + wm) * 16 + (lane & 15);
-    if (r >= c_rows) continue;
-    unsigned short* row = (unsigned short*)c_tile + (size_t)r * g.ldc;
-#pragma unroll
-    for (int j = 0; j < C::NJ; ++j) {
-      const int c = wn * C::TN + j * 16 + (lane >> 4) * 4;
-      unsigned short v[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] = to_out<OUT>(acc[i][j][q]);
-      if (wide && c + 4 <= c_cols) {
-        *(uint2*)(row + c) = make_uint2(v[0] | (unsigned)v[1] << 16, v[2] | (unsigned)v[3] << 16);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          if (c + q < c_cols) row[c + q] = v[q];
-      }
-    }
-  }
-}
-
-// The same through LDS, which the loop has left: whole rows of the tile at a time, 16 bytes a lane, where the direct
-// form writes 32 bytes of each of 16 rows. 16-byte chunk c of row r lies at c ^ (r & 15): neither side conflicts.
+// The result through LDS, which the loop has left: whole rows of the tile at a time, 16 bytes a lane (straight from
+// the accumulators a store would write 32 bytes of each of 16 rows). Accumulator [i][j] of a lane holds row
+// 16 (i WM + wm) + (lane & 15), columns 16 j + 4 (lane >> 4) + 0..3 of the wave's part: B is the matrix instruction's
+// first operand, so a lane's four values lie along a row. 16-byte chunk c of row r lies at c ^ (r & 15): neither side
+// conflicts. Rows that do not start on 16 bytes are stored by the same unaligned vector stores.
 template <class C>
 __device__ __forceinline__ void tile_store_rows(const GroupArgs& g, char* lds, char* c_tile, int c_rows, int c_cols, int wm, int wn,
                                                 const gf4 (&acc)[C::NI][C::NJ]) {
   static_assert(C::BM * C::BN * 2 <= C::LDS, "the tile fits the ring");
   constexpr int OUT = C::DT == kFp16 ? kFp16 : kBf16;
   const bool wide = (((uintptr_t)g.c | (uintptr_t)(g.ldc * 2) | (uintptr_t)(g.c_expert * 2)) & 15) == 0;
-  if (!wide) return tile_store<C>(g, c_tile, c_rows, c_cols, wm, wn, acc);
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
   bar();                                                 // every wave has read its last fragments
 #pragma unroll
@@ -376,7 +297,8 @@ __device__ __forceinline__ void tile_store_rows(const GroupArgs& g, char* lds, c
     const uint4 v = *(const uint4*)(lds + r * (C::BN * 2) + ((c ^ (r & 15)) << 4));
     unsigned short* at = (unsigned short*)c_tile + (size_t)r * g.ldc + c * 8;
     if (c * 8 + 8 <= c_cols) {
-      store_c16(at, v);
+      if (wide) store_c16(at, v);
+      else __builtin_memcpy(at, &v, 16);
     } else {
       const unsigned w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -832,44 +754,4 @@ __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu
   else if (c_rows > C::BM / 4) pp_half_loop<C, PingPong<C>::NH>(lds, ld, wm, wn, acc);
   else pp_half_loop<C, PingPong<C>::NH / 2>(lds, ld, wm, wn, acc);
   tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
-}
-
-// The form for operands that LDS-DMA cannot take (16-byte chunks that are not whole or not aligned): panels go
-// through registers, the next one's loads in flight under the multiplication, into the other of two buffers.
-template <class C>
-__global__ void __launch_bounds__(C::THREADS) group_tile_regs(const GroupArgs g) {
-  static_assert(C::NBUF == 2, "one barrier a panel");
-  __shared__ __attribute__((aligned(16))) char lds[C::LDS];
-  zero_rest_rows(g, g.cols, blockIdx.x, gridDim.x, C::THREADS);
-  TileOperands t;
-  char* c_tile;
-  int c_rows, c_cols;
-  if (!tile_setup<C>(g, blockIdx.x, t, c_tile, c_rows, c_cols)) return;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WN, wn = wave % C::WN;
-  gf4 acc[C::NI][C::NJ];
-#pragma unroll
-  for (int i = 0; i < C::NI; ++i)
-#pragma unroll
-    for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
-  PanelRegs<C, C::ATR, C::BM> a;
-  PanelRegs<C, C::BTR, C::BN> b;
-  const int nk = (t.red + C::KT - 1) / C::KT;
-  for (int kt = -1; kt < nk; ++kt) {
-    char* const buf = lds + (kt & 1) * C::STAGE;
-    if (kt >= 0) {
-      a.store(buf);
-      b.store(buf + C::OPA);
-      stage_scales<C>(buf + C::OPA + C::OPB, g, t, kt);
-      __syncthreads();
-    }
-    if (kt + 1 < nk) {
-      a.load(t.a, t.lda_b, t.a_rows, t.a_col0, t.a_cols, t.red, kt + 1);
-      b.load(t.b, t.ldb_b, t.b_rows, t.b_col0, t.b_cols, t.red, kt + 1);
-    }
-    if (kt >= 0) {
-      if (c_rows > C::BM / 2) tile_compute<C, C::NI>((lds_in)buf, wm, wn, acc);
-      else tile_compute<C, C::NI / 2>((lds_in)buf, wm, wn, acc);
-    }
-  }
-  tile_store<C>(g, c_tile, c_rows, c_cols, wm, wn, acc);
 }
