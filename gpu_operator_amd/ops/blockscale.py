@@ -94,6 +94,7 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
     if offsets is not None:
         _offsets(offsets, e, device)
     out, ldc, rest = _out(out, (m, n), torch.bfloat16, device)
+    rest = 0 if offsets is None else rest
     if m and n:
         ssa, ssb = a_scale.stride(), bt_scale.stride()
         launch(device, "amdgo_gemm_group(fp8)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,

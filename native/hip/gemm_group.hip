@@ -21,7 +21,7 @@ int launch_tile(const GroupArgs& g, hipStream_t s) {
   GroupArgs a = g;
   // the last tiles are cut into parts: at most one more round of workgroups
   a.slots = g.mode != kModeWgrad ? device_cu_count(s) * (160 * 1024 / C::LDS) : 0;
-  const long long grid = tile_grid<C>(g) + a.slots;
+  const long long grid = tile_grid<C>(g) + a.slots + (g.zero_rest ? kRestBlocks : 0);
   if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
   if (grid == 0) return 0;
   if constexpr (KERNEL == kTilePingPong) hipLaunchKernelGGL((group_tile_pp<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(256) pack_rows(const char* __restrict__ from, 
 
 template <class C>
 int launch_skinny(const GroupArgs& g, long long tiles_m, hipStream_t s) {
-  const long long grid = tiles_m * (((long long)g.cols + C::COLS - 1) / C::COLS);
+  const long long grid = tiles_m * (((long long)g.cols + C::COLS - 1) / C::COLS) + (g.zero_rest ? kRestBlocks : 0);
   if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
   hipLaunchKernelGGL((group_skinny<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, g);
   return (int)hipGetLastError();
@@ -180,6 +180,7 @@ int amdgo_gemm_group(const void* args, hipStream_t s) {
   __builtin_memcpy(&g, args, offsetof(GroupArgs, slots));       // packed by the caller up to there
   if (g.rows < 0 || g.cols < 0 || g.red < 0 || g.experts < 1) return (int)hipErrorInvalidValue;
   if (g.rows == 0 || g.cols == 0) return 0;
+  if (g.offsets == nullptr || g.mode == kModeWgrad) g.zero_rest = 0;
   if (g.dtype == kFp8) {
     if (g.mode != kModeForward) return (int)hipErrorInvalidValue;
     if (g.scale == kScaleF32) return dispatch_tile<kFp8, kScaleF32, false, false>(g, s);

@@ -56,8 +56,9 @@ __device__ __forceinline__ void group_rows(const int* __restrict__ off, int e, i
   end = min(max(off[e + 1], begin), total);
 }
 
-// The row tile `t` of the ragged rows, counted over the experts' tiles of `bm` rows in order; false past the
-// last one. Every wave runs it redundantly over registers (64 experts a step), so no barrier is needed.
+// The tiles of `bm` rows of the ragged rows, expert by expert (whole tiles first and the experts' rests last costs
+// 4 %: the rests read their expert's weights again). Every wave works them out over its registers, 64 experts a step, so
+// no barrier is needed; the first step's offsets and sums stay in registers, and up to 64 experts need no other.
 struct RowTile {
   int expert, row0, row_end;
 };
@@ -72,44 +73,52 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
   return v;
 }
 
-__device__ __forceinline__ int group_tile_count(const GroupArgs& g, int total, int bm) {
-  if (g.offsets == nullptr) return (total + bm - 1) / bm;
-  int n = 0;
-  for (int e = threadIdx.x & 63; e < g.experts; e += 64) {
-    int b, x;
-    group_rows(g.offsets, e, total, b, x);
-    n += (x - b + bm - 1) / bm;
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) n += __shfl_xor(n, d);
-  return __builtin_amdgcn_readfirstlane(n);
-}
+struct RowTiles {
+  const int* off;
+  int experts, total, bm;
+  int begin, end, upto;                      // of expert (lane) of the current step; its tiles' sum with all before
+  int tiles;
 
-__device__ __forceinline__ bool group_find_tile(const GroupArgs& g, int total, int bm, int t, RowTile& out) {
-  if (g.offsets == nullptr) {
-    out = RowTile{0, t * bm, total};
-    return t * (long long)bm < total;
-  }
-  int base = 0;
-  for (int e0 = 0; e0 < g.experts; e0 += 64) {
+  __device__ __forceinline__ void step(int e0, int before) {
     const int e = e0 + (threadIdx.x & 63);
-    int b = 0, x = 0;
-    if (e < g.experts) group_rows(g.offsets, e, total, b, x);
-    const int mine = (x - b + bm - 1) / bm;
-    const int upto = wave_inclusive_sum(mine);
-    const unsigned long long past = __ballot(base + upto > t);
-    if (past != 0) {
-      const int lane = __builtin_ctzll(past);
-      const int first = base + __shfl(upto, lane) - __shfl(mine, lane);
-      out.expert = __builtin_amdgcn_readfirstlane(e0 + lane);
-      out.row0 = __builtin_amdgcn_readfirstlane(__shfl(b, lane) + (t - first) * bm);
-      out.row_end = __builtin_amdgcn_readfirstlane(__shfl(x, lane));
-      return true;
-    }
-    base += __shfl(upto, 63);
+    begin = end = 0;
+    if (e < experts) group_rows(off, e, total, begin, end);
+    upto = before + wave_inclusive_sum((end - begin + bm - 1) / bm);
   }
-  return false;
-}
+  __device__ __forceinline__ int last() const { return __builtin_amdgcn_readlane(upto, 63); }
+
+  __device__ __forceinline__ RowTiles(const GroupArgs& g, int total_, int bm_) : off(g.offsets), experts(g.experts), total(total_), bm(bm_) {
+    if (off == nullptr) {
+      tiles = (total + bm - 1) / bm;
+      return;
+    }
+    step(0, 0);
+    tiles = last();
+    for (int e0 = 64; e0 < experts; e0 += 64) {
+      RowTiles next = *this;
+      next.step(e0, tiles);
+      tiles = next.last();
+    }
+  }
+
+  // tile t < tiles
+  __device__ __forceinline__ RowTile find(int t) {
+    if (off == nullptr) return RowTile{0, t * bm, total};
+    for (int e0 = 0;;) {
+      const unsigned long long past = __ballot(upto > t);
+      if (past != 0) {
+        const int lane = __builtin_ctzll(past);
+        const int b = __builtin_amdgcn_readlane(begin, lane), x = __builtin_amdgcn_readlane(end, lane);
+        const int first = __builtin_amdgcn_readlane(upto, lane) - (x - b + bm - 1) / bm;
+        return RowTile{__builtin_amdgcn_readfirstlane(e0 + lane), b + (t - first) * bm, x};
+      }
+      const int before = last();
+      e0 += 64;
+      if (e0 >= experts) return RowTile{0, 0, 0};       // (not reached for t < tiles)
+      step(e0, before);
+    }
+  }
+};
 
 // The expert with the `want`-th most rows (ties in order), up to 64 experts; above that the experts in order. A
 // weight gradient's tiles take as long as their expert has rows: started with the longest, the last ones to end are
@@ -143,17 +152,26 @@ __device__ __forceinline__ unsigned short to_out(float v) {
   else return __builtin_bit_cast(unsigned short, (__bf16)v);
 }
 
-// Rows that no expert owns, as zeros: the whole grid walks them, each block whole rows.
-__device__ __forceinline__ void zero_rest_rows(const GroupArgs& g, int cols, int block, int blocks, int threads) {
-  if (!g.zero_rest || g.offsets == nullptr) return;
-  const int first = min(max(g.offsets[0], 0), g.rows), last = min(max(g.offsets[g.experts], 0), g.rows);
+// Rows that no expert owns, as zeros, by the launch's last kRestBlocks workgroups, which do nothing else (the others
+// would wait for the offsets once more). True: this is one of them.
+constexpr int kRestBlocks = 32;
+
+__device__ __forceinline__ bool zero_rest_rows(const GroupArgs& g, int threads) {
+  if (!g.zero_rest || g.offsets == nullptr) return false;
+  const int block = (int)blockIdx.x - ((int)gridDim.x - kRestBlocks);
+  if (block < 0) return false;
+  const int first = min(max(g.offsets[0], 0), g.rows), last = max(min(max(g.offsets[g.experts], 0), g.rows), first);
   unsigned short* c = (unsigned short*)g.c;
-  const int rest = first + (g.rows - max(last, first));
-  for (int i = block; i < rest; i += blocks) {
-    const int r = i < first ? i : max(last, first) + (i - first);
-    unsigned short* row = c + (size_t)r * g.ldc;
-    for (int j = threadIdx.x; j < cols; j += threads) row[j] = 0;
+  const int rest = first + (g.rows - last);
+  for (int i = block; i < rest; i += kRestBlocks) {
+    unsigned short* row = c + (size_t)(i < first ? i : last + (i - first)) * g.ldc;
+    // 16 bytes a lane between the row's first and last whole ones
+    const int head = min((int)((16 - ((uintptr_t)row & 15)) & 15) / 2, g.cols), body = (g.cols - head) / 8;
+    for (int j = threadIdx.x; j < body; j += threads) *(uint4*)(row + head + 8 * j) = make_uint4(0, 0, 0, 0);
+    if ((int)threadIdx.x < head) row[threadIdx.x] = 0;
+    for (int j = head + 8 * body + threadIdx.x; j < g.cols; j += threads) row[j] = 0;
   }
+  return true;
 }
 
 }  // namespace

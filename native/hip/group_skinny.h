@@ -74,11 +74,12 @@ __device__ __forceinline__ void skinny_mul(const SkinnyPanel<C>& p, gf4 (&acc)[C
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) group_skinny(const GroupArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[C::LDS];
-  zero_rest_rows(g, g.cols, blockIdx.x, gridDim.x, C::THREADS);
+  if (zero_rest_rows(g, C::THREADS)) return;
   const int tiles_n = (g.cols + C::COLS - 1) / C::COLS;
   const int tm = blockIdx.x / tiles_n, n0 = (blockIdx.x - tm * tiles_n) * C::COLS;
-  RowTile rt;
-  if (!group_find_tile(g, g.rows, C::ROWS, tm, rt)) return;
+  RowTiles row_tiles(g, g.rows, C::ROWS);
+  if (tm >= row_tiles.tiles) return;
+  const RowTile rt = row_tiles.find(tm);
   const int lane = threadIdx.x & 63, l16 = lane & 15, q0 = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int rows = min(C::ROWS, rt.row_end - rt.row0), cols = min(C::COLS, g.cols - n0);

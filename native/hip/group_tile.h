@@ -220,7 +220,8 @@ __device__ __forceinline__ bool tile_setup(const GroupArgs& g, int block, TileOp
     c_cols = min(C::BN, g.cols - tn * C::BN);
     c_tile = (char*)g.c + 2 * ((size_t)e * g.c_expert + (size_t)tm * C::BM * g.ldc + (size_t)tn * C::BN);
   } else {
-    const int tiles_m = group_tile_count(g, g.rows, C::BM), tiles = tiles_m * tiles_n;
+    RowTiles row_tiles(g, g.rows, C::BM);
+    const int tiles_m = row_tiles.tiles, tiles = tiles_m * tiles_n;
     // The tiles past the last whole round of the `slots` workgroups that run at once would keep few of them busy for a
     // whole tile's time: they are cut into 2 or 4 parts by rows, as many as still fit one round.
     const int over = g.slots > 0 ? tiles % g.slots : 0, whole = tiles - over;
@@ -235,8 +236,7 @@ __device__ __forceinline__ bool tile_setup(const GroupArgs& g, int block, TileOp
       part = item % parts;
     }
     tile_coords(tile, tiles_m, tiles_n, tm, tn);
-    RowTile rt;
-    if (!group_find_tile(g, g.rows, C::BM, tm, rt)) return false;
+    RowTile rt = row_tiles.find(tm);
     if (parts > 1 && block >= whole) {
       const int rows = C::BM / parts;
       rt.row0 += part * rows;
@@ -464,7 +464,7 @@ template <class C>
 __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::EU, C::EU)))
 group_tile_dma(const GroupArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[C::LDS];     // the only LDS object: see tile_step
-  zero_rest_rows(g, g.cols, blockIdx.x, gridDim.x, C::THREADS);
+  if (zero_rest_rows(g, C::THREADS)) return;
   TileOperands t;
   char* c_tile;
   int c_rows, c_cols;
@@ -737,7 +737,7 @@ __device__ __forceinline__ void pp_half_loop(char* lds, PingPongLoader<C>& ld, i
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) group_tile_pp(const GroupArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[PingPong<C>::LDS];     // the only LDS object: see tile_step
-  zero_rest_rows(g, g.cols, blockIdx.x, gridDim.x, C::THREADS);
+  if (zero_rest_rows(g, C::THREADS)) return;
   TileOperands t;
   char* c_tile;
   int c_rows, c_cols;
