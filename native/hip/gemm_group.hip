@@ -19,13 +19,17 @@ enum TileKernel { kTileDma, kTilePingPong };
 template <class C, TileKernel KERNEL>
 int launch_tile(const GroupArgs& g, hipStream_t s) {
   GroupArgs a = g;
-  // the last tiles are cut into parts: at most one more round of workgroups
-  a.slots = g.mode != kModeWgrad ? device_cu_count(s) * (160 * 1024 / C::LDS) : 0;
-  const long long grid = tile_grid<C>(g) + a.slots + (g.zero_rest ? kRestBlocks : 0);
-  if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
-  if (grid == 0) return 0;
-  if constexpr (KERNEL == kTilePingPong) hipLaunchKernelGGL((group_tile_pp<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
-  else hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
+  const int resident = device_cu_count(s) * (KERNEL == kTilePingPong ? 1 : C::RESIDENT);
+  a.slots = KERNEL == kTilePingPong || g.mode != kModeWgrad ? resident : 0;
+  if (tile_grid<C>(g) > 0x7fffffff - 2 * (long long)resident) return (int)hipErrorInvalidValue;
+  if (tile_grid<C>(g) == 0) return 0;
+  if constexpr (KERNEL == kTilePingPong) {
+    hipLaunchKernelGGL((group_tile_pp<C>), dim3((unsigned)resident), dim3(C::THREADS), 0, s, a);
+  } else {
+    // the last tiles are cut into parts: at most one more round of workgroups
+    const long long grid = tile_grid<C>(g) + a.slots + (g.zero_rest ? kRestBlocks : 0);
+    hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
+  }
   return (int)hipGetLastError();
 }
 
@@ -144,7 +148,8 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   }
   if (!ready) return kNeedsPacking;
   const int cus = device_cu_count(s);
-  const bool large_fills = 5 * tile_grid<Large>(g) >= 4 * cus;
+  // (a Large tile's stores are 32-bit offsets in it)
+  const bool large_fills = 5 * tile_grid<Large>(g) >= 4 * cus && g.ldc * 2 * 256 < 0x7fffffffll;
   if constexpr (ATR) {
     if (large_fills && g.red >= 128ll * g.experts) return launch_tile<Large, kTilePingPong>(g, s);
     return launch_tile<Small, kTileDma>(g, s);

@@ -87,7 +87,11 @@ struct RowTiles {
   }
   __device__ __forceinline__ int last() const { return __builtin_amdgcn_readlane(upto, 63); }
 
-  __device__ __forceinline__ RowTiles(const GroupArgs& g, int total_, int bm_) : off(g.offsets), experts(g.experts), total(total_), bm(bm_) {
+  __device__ __forceinline__ void init(const GroupArgs& g, int total_, int bm_) {
+    off = g.offsets;
+    experts = g.experts;
+    total = total_;
+    bm = bm_;
     if (off == nullptr) {
       tiles = (total + bm - 1) / bm;
       return;
@@ -101,21 +105,41 @@ struct RowTiles {
     }
   }
 
+  // The first step's lanes and the counts, to LDS and back (kWords words): a loop that needs its registers keeps the plan there.
+  static constexpr int kWords = 3 * 64;
+  __device__ __forceinline__ void save(int* at) const {
+    const int lane = threadIdx.x & 63;
+    at[lane] = begin;
+    at[64 + lane] = end;
+    at[128 + lane] = upto;
+  }
+  __device__ __forceinline__ void load(const GroupArgs& g, int total_, int bm_, const int* at) {
+    off = g.offsets;
+    experts = g.experts;
+    total = total_;
+    bm = bm_;
+    const int lane = threadIdx.x & 63;
+    begin = at[lane];
+    end = at[64 + lane];
+    upto = at[128 + lane];
+  }
+
   // tile t < tiles
-  __device__ __forceinline__ RowTile find(int t) {
+  __device__ __forceinline__ RowTile find(int t) const {
     if (off == nullptr) return RowTile{0, t * bm, total};
+    RowTiles at = *this;                               // (the first step's lanes stay, for the next tile)
     for (int e0 = 0;;) {
-      const unsigned long long past = __ballot(upto > t);
+      const unsigned long long past = __ballot(at.upto > t);
       if (past != 0) {
         const int lane = __builtin_ctzll(past);
-        const int b = __builtin_amdgcn_readlane(begin, lane), x = __builtin_amdgcn_readlane(end, lane);
-        const int first = __builtin_amdgcn_readlane(upto, lane) - (x - b + bm - 1) / bm;
+        const int b = __builtin_amdgcn_readlane(at.begin, lane), x = __builtin_amdgcn_readlane(at.end, lane);
+        const int first = __builtin_amdgcn_readlane(at.upto, lane) - (x - b + bm - 1) / bm;
         return RowTile{__builtin_amdgcn_readfirstlane(e0 + lane), b + (t - first) * bm, x};
       }
-      const int before = last();
+      const int before = at.last();
       e0 += 64;
       if (e0 >= experts) return RowTile{0, 0, 0};       // (not reached for t < tiles)
-      step(e0, before);
+      at.step(e0, before);
     }
   }
 };
@@ -152,18 +176,13 @@ __device__ __forceinline__ unsigned short to_out(float v) {
   else return __builtin_bit_cast(unsigned short, (__bf16)v);
 }
 
-// Rows that no expert owns, as zeros, by the launch's last kRestBlocks workgroups, which do nothing else (the others
-// would wait for the offsets once more). True: this is one of them.
-constexpr int kRestBlocks = 32;
-
-__device__ __forceinline__ bool zero_rest_rows(const GroupArgs& g, int threads) {
-  if (!g.zero_rest || g.offsets == nullptr) return false;
-  const int block = (int)blockIdx.x - ((int)gridDim.x - kRestBlocks);
-  if (block < 0) return false;
+// Rows that no expert owns, as zeros: workgroup `block` of `blocks`.
+__device__ __forceinline__ void zero_rest_rows(const GroupArgs& g, int block, int blocks, int threads) {
+  if (!g.zero_rest || g.offsets == nullptr) return;
   const int first = min(max(g.offsets[0], 0), g.rows), last = max(min(max(g.offsets[g.experts], 0), g.rows), first);
   unsigned short* c = (unsigned short*)g.c;
   const int rest = first + (g.rows - last);
-  for (int i = block; i < rest; i += kRestBlocks) {
+  for (int i = block; i < rest; i += blocks) {
     unsigned short* row = c + (size_t)(i < first ? i : last + (i - first)) * g.ldc;
     // 16 bytes a lane between the row's first and last whole ones
     const int head = min((int)((16 - ((uintptr_t)row & 15)) & 15) / 2, g.cols), body = (g.cols - head) / 8;
@@ -171,6 +190,16 @@ __device__ __forceinline__ bool zero_rest_rows(const GroupArgs& g, int threads) 
     if ((int)threadIdx.x < head) row[threadIdx.x] = 0;
     for (int j = head + 8 * body + threadIdx.x; j < g.cols; j += threads) row[j] = 0;
   }
+}
+
+// The same by a launch's last kRestBlocks workgroups, which do nothing else (the others would wait for the offsets once
+// more). True: this is one of them.
+constexpr int kRestBlocks = 32;
+
+__device__ __forceinline__ bool rest_block(const GroupArgs& g, int threads) {
+  const int block = (int)blockIdx.x - ((int)gridDim.x - kRestBlocks);
+  if (!g.zero_rest || g.offsets == nullptr || block < 0) return false;
+  zero_rest_rows(g, block, kRestBlocks, threads);
   return true;
 }
 

@@ -74,10 +74,11 @@ __device__ __forceinline__ void skinny_mul(const SkinnyPanel<C>& p, gf4 (&acc)[C
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) group_skinny(const GroupArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[C::LDS];
-  if (zero_rest_rows(g, C::THREADS)) return;
+  if (rest_block(g, C::THREADS)) return;
   const int tiles_n = (g.cols + C::COLS - 1) / C::COLS;
   const int tm = blockIdx.x / tiles_n, n0 = (blockIdx.x - tm * tiles_n) * C::COLS;
-  RowTiles row_tiles(g, g.rows, C::ROWS);
+  RowTiles row_tiles;
+  row_tiles.init(g, g.rows, C::ROWS);
   if (tm >= row_tiles.tiles) return;
   const RowTile rt = row_tiles.find(tm);
   const int lane = threadIdx.x & 63, l16 = lane & 15, q0 = lane >> 4;

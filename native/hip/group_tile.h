@@ -198,71 +198,123 @@ __device__ __forceinline__ void tile_compute(lds_in lds, int wm, int wn, gf4 (&a
   }
 }
 
-// The tile of this workgroup: what it reads and where it writes. False: nothing to do.
+// A tile: what it reads and where it writes.
+struct TileWork {
+  TileOperands t;
+  char* c;
+  int rows, cols;
+};
+
+// The launch's work items, one for each tile -- except that the tiles past the last whole round of the `slots`
+// workgroups that run at once, which would keep few of them busy for a whole tile's time, are cut into 2 or 4 parts by
+// rows, as many as still fit one round.
 template <class C>
-__device__ __forceinline__ bool tile_setup(const GroupArgs& g, int block, TileOperands& t, char*& c_tile, int& c_rows, int& c_cols) {
-  const int tiles_n = (g.cols + C::BN - 1) / C::BN;
-  if (g.mode == kModeWgrad) {
-    const int tiles_m = (g.rows + C::BM - 1) / C::BM, per = tiles_m * tiles_n;
-    // an expert's tiles over all XCDs: whole experts to an XCD would leave those with the short ones idle
-    const int place = block / per, e = group_by_size(g, g.red, place);
-    int tm, tn, begin = 0, end = g.red;
-    tile_coords(xcd_remap(block - place * per, per), tiles_m, tiles_n, tm, tn);
-    if (g.offsets) group_rows(g.offsets, e, g.red, begin, end);
-    t.a = (const char*)g.a + (size_t)begin * g.lda * C::ES;
-    t.b = (const char*)g.b + (size_t)begin * g.ldb * C::ES;
-    t.a_col0 = tm * C::BM;
-    t.b_col0 = tn * C::BN;
-    t.a_cols = g.rows;
-    t.b_cols = g.cols;
-    t.red = end - begin;
-    c_rows = min(C::BM, g.rows - tm * C::BM);
-    c_cols = min(C::BN, g.cols - tn * C::BN);
-    c_tile = (char*)g.c + 2 * ((size_t)e * g.c_expert + (size_t)tm * C::BM * g.ldc + (size_t)tn * C::BN);
-  } else {
-    RowTiles row_tiles(g, g.rows, C::BM);
-    const int tiles_m = row_tiles.tiles, tiles = tiles_m * tiles_n;
-    // The tiles past the last whole round of the `slots` workgroups that run at once would keep few of them busy for a
-    // whole tile's time: they are cut into 2 or 4 parts by rows, as many as still fit one round.
-    const int over = g.slots > 0 ? tiles % g.slots : 0, whole = tiles - over;
-    const int parts = over == 0 ? 1 : 4 * over <= g.slots ? 4 : 2 * over <= g.slots ? 2 : 1;
-    int tm, tn, tile, part = 0;
-    if (block < whole) {
-      tile = xcd_remap(block, whole);
+struct TilePlan {
+  RowTiles rows;
+  int tiles_m, tiles_n, whole, over, parts, items;
+
+  TilePlan() = default;
+  __device__ __forceinline__ explicit TilePlan(const GroupArgs& g) {
+    tiles_n = (g.cols + C::BN - 1) / C::BN;
+    if constexpr (C::ATR) {                                // weight gradients: whole tiles of every expert
+      tiles_m = (g.rows + C::BM - 1) / C::BM;
+      items = tiles_m * tiles_n * g.experts;
     } else {
-      if (block - whole >= over * parts) return false;
-      const int item = xcd_remap(block - whole, over * parts);
-      tile = whole + item / parts;
-      part = item % parts;
+      rows.init(g, g.rows, C::BM);
+      tiles_m = rows.tiles;
+      over = g.slots > 0 ? tiles_m * tiles_n % g.slots : 0;
+      whole = tiles_m * tiles_n - over;
+      parts = over == 0 ? 1 : 4 * over <= g.slots ? 4 : 2 * over <= g.slots ? 2 : 1;
+      items = whole + over * parts;
     }
-    tile_coords(tile, tiles_m, tiles_n, tm, tn);
-    RowTile rt = row_tiles.find(tm);
-    if (parts > 1 && block >= whole) {
-      const int rows = C::BM / parts;
-      rt.row0 += part * rows;
-      rt.row_end = min(rt.row_end, rt.row0 + rows);
-      if (rt.row0 >= rt.row_end) return false;
-    }
-    t.a = (const char*)g.a + (size_t)rt.row0 * g.lda * C::ES;
-    t.a_rows = min(C::BM, rt.row_end - rt.row0);
-    t.b_rows = min(C::BN, g.cols - tn * C::BN);
-    t.b_col0 = tn * C::BN;
-    t.b_cols = g.cols;
-    t.b = (const char*)g.b + ((size_t)rt.expert * g.b_expert + (C::BTR ? 0 : (size_t)tn * C::BN * g.ldb)) * C::ES;
-    t.red = g.red;
-    if constexpr (C::SC != kScaleNone) {
-      constexpr int S = C::SC == kScaleF32 ? 4 : 1;
-      t.as = (const char*)g.a_scale + (size_t)rt.row0 * g.as_row * S;
-      t.bs = (const char*)g.b_scale + ((size_t)rt.expert * g.bs_expert + (size_t)(tn * C::BN / kScaleBlock) * g.bs_row) * S;
-    }
-    c_rows = t.a_rows;
-    c_cols = t.b_rows;
-    c_tile = (char*)g.c + 2 * ((size_t)rt.row0 * g.ldc + (size_t)tn * C::BN);
   }
-  t.lda_b = g.lda * C::ES;
-  t.ldb_b = g.ldb * C::ES;
-  return true;
-}
+
+  static constexpr int kWords = RowTiles::kWords + 6;
+  __device__ __forceinline__ void save(int* at) const {
+    if constexpr (!C::ATR) {
+      if (rows.off != nullptr) rows.save(at);
+    }
+    at += RowTiles::kWords;
+    at[0] = tiles_m;
+    at[1] = tiles_n;
+    at[2] = items;
+    if constexpr (!C::ATR) {
+      at[3] = whole;
+      at[4] = over;
+      at[5] = parts;
+    }
+  }
+  __device__ __forceinline__ void load(const GroupArgs& g, const int* at) {
+    if constexpr (!C::ATR) rows.load(g, g.rows, C::BM, at);
+    at += RowTiles::kWords;
+    tiles_m = __builtin_amdgcn_readfirstlane(at[0]);
+    tiles_n = __builtin_amdgcn_readfirstlane(at[1]);
+    items = __builtin_amdgcn_readfirstlane(at[2]);
+    if constexpr (!C::ATR) {
+      whole = __builtin_amdgcn_readfirstlane(at[3]);
+      over = __builtin_amdgcn_readfirstlane(at[4]);
+      parts = __builtin_amdgcn_readfirstlane(at[5]);
+    }
+  }
+
+  // item < items; false: a part without rows
+  __device__ __forceinline__ bool work(const GroupArgs& g, int item, TileWork& w) {
+    TileOperands& t = w.t;
+    int tm, tn;
+    t.lda_b = g.lda * C::ES;
+    t.ldb_b = g.ldb * C::ES;
+    if constexpr (C::ATR) {
+      // an expert's tiles over all XCDs: whole experts to an XCD would leave those with the short ones idle
+      const int per = tiles_m * tiles_n, place = item / per, e = group_by_size(g, g.red, place);
+      int begin = 0, end = g.red;
+      tile_coords(xcd_remap(item - place * per, per), tiles_m, tiles_n, tm, tn);
+      if (g.offsets) group_rows(g.offsets, e, g.red, begin, end);
+      t.a = (const char*)g.a + (size_t)begin * g.lda * C::ES;
+      t.b = (const char*)g.b + (size_t)begin * g.ldb * C::ES;
+      t.a_col0 = tm * C::BM;
+      t.b_col0 = tn * C::BN;
+      t.a_cols = g.rows;
+      t.b_cols = g.cols;
+      t.red = end - begin;
+      w.rows = min(C::BM, g.rows - tm * C::BM);
+      w.cols = min(C::BN, g.cols - tn * C::BN);
+      w.c = (char*)g.c + 2 * ((size_t)e * g.c_expert + (size_t)tm * C::BM * g.ldc + (size_t)tn * C::BN);
+      return true;
+    } else {
+      int tile, part = 0;
+      if (item < whole) {
+        tile = xcd_remap(item, whole);
+      } else {
+        const int at = xcd_remap(item - whole, over * parts);
+        tile = whole + at / parts;
+        part = at % parts;
+      }
+      tile_coords(tile, tiles_m, tiles_n, tm, tn);
+      RowTile rt = rows.find(tm);
+      if (parts > 1 && item >= whole) {
+        rt.row0 += part * (C::BM / parts);
+        rt.row_end = min(rt.row_end, rt.row0 + C::BM / parts);
+        if (rt.row0 >= rt.row_end) return false;
+      }
+      t.a = (const char*)g.a + (size_t)rt.row0 * g.lda * C::ES;
+      t.a_rows = min(C::BM, rt.row_end - rt.row0);
+      t.b_rows = min(C::BN, g.cols - tn * C::BN);
+      t.b_col0 = tn * C::BN;
+      t.b_cols = g.cols;
+      t.b = (const char*)g.b + ((size_t)rt.expert * g.b_expert + (C::BTR ? 0 : (size_t)tn * C::BN * g.ldb)) * C::ES;
+      t.red = g.red;
+      if constexpr (C::SC != kScaleNone) {
+        constexpr int S = C::SC == kScaleF32 ? 4 : 1;
+        t.as = (const char*)g.a_scale + (size_t)rt.row0 * g.as_row * S;
+        t.bs = (const char*)g.b_scale + ((size_t)rt.expert * g.bs_expert + (size_t)(tn * C::BN / kScaleBlock) * g.bs_row) * S;
+      }
+      w.rows = t.a_rows;
+      w.cols = t.b_rows;
+      w.c = (char*)g.c + 2 * ((size_t)rt.row0 * g.ldc + (size_t)tn * C::BN);
+      return true;
+    }
+  }
+};
 
 // The result through LDS, which the loop has left: whole rows of the tile at a time, 16 bytes a lane (straight from
 // the accumulators a store would write 32 bytes of each of 16 rows). Accumulator [i][j] of a lane holds row
@@ -313,52 +365,45 @@ constexpr unsigned kNowhere = 0x80000000u;
 
 typedef __attribute__((address_space(3))) void* g_lds_ptr;
 
-// One operand's panels by LDS-DMA (buffer_load ... lds): a wave instruction fills 1 KiB of LDS in lane order,
-// so the permutation of the chunks goes on the addresses that the lanes read. Each lane keeps the offsets of its
-// pieces; the panel's place is the descriptor's base. Rows or columns that do not exist, and in the last panel
-// the reduction steps past the end, are offsets past the buffer: zeros, whatever lies there.
+// One operand's panels by LDS-DMA (buffer_load ... lds): a wave instruction (a piece) fills 1 KiB of LDS in lane
+// order, so the permutation of the chunks goes on the addresses that the lanes read. A wave's pieces are STEP panel rows
+// apart, a multiple of the permutations' period, so a lane's offset is that of its first piece and the rest is the same
+// for all lanes. Panel rows at or past `limit`, and lanes with nothing to read, ask for kNowhere: zeros, whatever lies
+// there. Panel rows are the operand's rows (K-major) or reduction steps (reduction-major).
 template <class C, bool TR, int ROWS>
 struct PanelDma {
   static constexpr int WAVES = C::THREADS / 64;
   static constexpr int PIECES = ROWS * C::PB / 1024 / WAVES;
+  static constexpr int LANES = TR ? ROWS / 8 : C::PB / 16;          // lanes, and chunks, of a panel row
+  static constexpr int STEP = WAVES * 64 / LANES, ALL = TR ? C::KT : ROWS;
   static_assert(PIECES * WAVES * 1024 == ROWS * C::PB, "whole pieces");
-  unsigned off[PIECES];
+  static_assert(STEP % 16 == 0, "the permutations' period");
+  unsigned off;
+  int row;                                                          // of the lane's first piece
 
-  __device__ __forceinline__ static int row_of(int piece, int wave, int lane) {
-    if constexpr (TR) return (piece * WAVES + wave) * (1024 / (2 * ROWS)) + lane / (ROWS / 8);
-    else return (piece * WAVES + wave) * (1024 / C::PB) + lane / (C::PB / 16);
-  }
   // the 16-byte chunk of its row that the lane reads
-  __device__ __forceinline__ static int chunk_of(int row, int lane) {
-    if constexpr (TR) {
-      const int q = lane % (ROWS / 8);
-      return (((q >> 1) ^ rm_swizzle(row)) << 1) | (q & 1);
-    } else {
-      return (lane % (C::PB / 16)) ^ km_swizzle<C::PB>(row);
-    }
+  __device__ __forceinline__ int chunk(int lane) const {
+    const int q = lane % LANES;
+    if constexpr (TR) return (((q >> 1) ^ rm_swizzle(row)) << 1) | (q & 1);
+    else return q ^ km_swizzle<C::PB>(row);
   }
-  __device__ __forceinline__ void init(int wave, int lane, unsigned ld, int rows, int col0, int cols) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int r = row_of(i, wave, lane), q = chunk_of(r, lane);
-      if constexpr (TR) off[i] = col0 + q * 8 < cols ? (unsigned)r * ld + (unsigned)(col0 + q * 8) * 2 : kNowhere;
-      else off[i] = r < rows ? (unsigned)r * ld + q * 16 : kNowhere;
-    }
+  __device__ __forceinline__ void init(int wave, int lane, unsigned ld, int col0, int cols) {
+    row = wave * (64 / LANES) + lane / LANES;
+    const int q = chunk(lane);
+    if constexpr (TR) off = col0 + q * 8 < cols ? (unsigned)row * ld + (unsigned)(col0 + q * 8) * 2 : kNowhere;
+    else off = (unsigned)row * ld + q * 16;
   }
-  // the last panel: `left` reduction steps of it exist
-  __device__ __forceinline__ void cut(int wave, int lane, int left) {
-#pragma unroll
-    for (int i = 0; i < PIECES; ++i) {
-      const int r = row_of(i, wave, lane);
-      if constexpr (TR) off[i] = r < left ? off[i] : kNowhere;
-      else off[i] = chunk_of(r, lane) * 16 < left * C::ES ? off[i] : kNowhere;
-    }
+  // K-major, the last panel: `left` reduction steps of it exist
+  __device__ __forceinline__ void cut(int lane, int left) {
+    if constexpr (!TR) off = chunk(lane) * 16 < left * C::ES ? off : kNowhere;
   }
-  __device__ __forceinline__ void load(char* lds, const char* panel, int wave) const {
+  __device__ __forceinline__ void load(char* lds, const char* panel, int wave, unsigned ld, int limit) const {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void*)panel, 0, 0x7fffffff, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < PIECES; ++i)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (g_lds_ptr)(lds + (i * WAVES + wave) * 1024), 16, off[i], 0, 0, 0);
+    for (int i = 0; i < PIECES; ++i) {
+      const unsigned o = limit >= ALL || row + i * STEP < limit ? off : kNowhere;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (g_lds_ptr)(lds + (i * WAVES + wave) * 1024), 16, o, i * STEP * ld, 0, 0);
+    }
   }
 };
 
@@ -368,16 +413,15 @@ template <class C>
 __device__ __forceinline__ void scale_lanes(const GroupArgs& g, const TileOperands& t, int wave, int lane, unsigned& soff,
                                             const char*& base, long long& step) {
   constexpr int SB = C::SC == kScaleF32 ? 4 : 1;
-  if (wave < C::BM / 64) {
-    const int r = wave * 64 + lane;
-    if (r < t.a_rows) soff = (unsigned)r * (unsigned)(g.as_row * SB);
-    base = t.as;
-    step = g.as_k * SB;
-  } else if (wave == C::BM / 64) {
-    if (lane < C::BN / kScaleBlock && lane * kScaleBlock < t.b_rows) soff = (unsigned)lane * (unsigned)(g.bs_row * SB);
-    base = t.bs;
-    step = g.bs_k * SB;
-  }
+  // (both operands' values first: a choice between the structs' members would put the structs into memory)
+  const bool of_a = wave < C::BM / 64, of_b = wave == C::BM / 64;
+  const int r = of_a ? wave * 64 + lane : lane, n = of_a ? t.a_rows : of_b ? min((t.b_rows + kScaleBlock - 1) / kScaleBlock, C::BN / kScaleBlock) : 0;
+  const unsigned ar = (unsigned)(g.as_row * SB), br = (unsigned)(g.bs_row * SB);
+  const long long ak = g.as_k * SB, bk = g.bs_k * SB;
+  const char *as = t.as, *bs = t.bs;
+  soff = r < n ? (unsigned)r * (of_a ? ar : br) : kNowhere;
+  base = of_a ? as : bs;
+  step = of_a ? ak : bk;
 }
 
 template <class C>
@@ -397,34 +441,34 @@ struct TileLoader {
   DmaA da;
   DmaB db;
   const char *pa, *pb, *ps;
-  size_t step_a, step_b;
   long long step_s;
-  unsigned soff;
-  int wave, lane, nk, left;
+  unsigned soff, lda, ldb;
+  int wave, lane, nk, left, a_rows, b_rows;
 
   __device__ __forceinline__ TileLoader(const GroupArgs& g, const TileOperands& t, int wave_, int lane_)
-      : pa(t.a), pb(t.b), ps(t.as), step_a(C::ATR ? (size_t)C::KT * t.lda_b : C::PB),
-        step_b(C::BTR ? (size_t)C::KT * t.ldb_b : C::PB), step_s(0), soff(kNowhere), wave(wave_), lane(lane_) {
+      : pa(t.a), pb(t.b), ps(t.as), step_s(0), soff(kNowhere), lda((unsigned)t.lda_b), ldb((unsigned)t.ldb_b), wave(wave_),
+        lane(lane_), a_rows(t.a_rows), b_rows(t.b_rows) {
     nk = (t.red + C::KT - 1) / C::KT;
     left = t.red - (nk - 1) * C::KT;
-    da.init(wave, lane, (unsigned)t.lda_b, t.a_rows, t.a_col0, t.a_cols);
-    db.init(wave, lane, (unsigned)t.ldb_b, t.b_rows, t.b_col0, t.b_cols);
+    da.init(wave, lane, lda, t.a_col0, t.a_cols);
+    db.init(wave, lane, ldb, t.b_col0, t.b_cols);
     if constexpr (C::SC != kScaleNone) scale_lanes<C>(g, t, wave, lane, soff, ps, step_s);
   }
   // panel kt (the next one) into `base`
   __device__ __forceinline__ void issue(int kt, char* base) {
-    if (kt == nk - 1 && left < C::KT) {
-      da.cut(wave, lane, left);
-      db.cut(wave, lane, left);
+    const int steps = kt == nk - 1 ? left : C::KT;
+    if (steps < C::KT) {
+      da.cut(lane, left);
+      db.cut(lane, left);
     }
-    da.load(base, pa, wave);
-    db.load(base + C::OPA, pb, wave);
+    da.load(base, pa, wave, lda, C::ATR ? steps : a_rows);
+    db.load(base + C::OPA, pb, wave, ldb, C::BTR ? steps : b_rows);
     if constexpr (C::SC != kScaleNone) {
       scale_load<C>(base + C::OPA + C::OPB, ps, wave, soff);
       ps += step_s;
     }
-    pa += step_a;
-    pb += step_b;
+    pa += C::ATR ? (size_t)C::KT * lda : C::PB;
+    pb += C::BTR ? (size_t)C::KT * ldb : C::PB;
   }
 };
 
@@ -464,14 +508,13 @@ template <class C>
 __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::EU, C::EU)))
 group_tile_dma(const GroupArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[C::LDS];     // the only LDS object: see tile_step
-  if (zero_rest_rows(g, C::THREADS)) return;
-  TileOperands t;
-  char* c_tile;
-  int c_rows, c_cols;
-  if (!tile_setup<C>(g, blockIdx.x, t, c_tile, c_rows, c_cols)) return;
-  const int lane = threadIdx.x & 63;
+  if (rest_block(g, C::THREADS)) return;
+  TilePlan<C> plan(g);
+  TileWork w;
+  if ((int)blockIdx.x >= plan.items || !plan.work(g, blockIdx.x, w)) return;
+  const int c_rows = w.rows, lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WN, wn = wave % C::WN;
-  TileLoader<C> ld(g, t, wave, lane);
+  TileLoader<C> ld(g, w.t, wave, lane);
   gf4 acc[C::NI][C::NJ];
 #pragma unroll
   for (int i = 0; i < C::NI; ++i)
@@ -484,7 +527,7 @@ group_tile_dma(const GroupArgs g) {
   if (C::NI < 4 || c_rows > C::BM / 2) tile_loop<C, C::NI>(lds, ld, wm, wn, acc);
   else if (c_rows > C::BM / 4) tile_loop<C, (C::NI + 1) / 2>(lds, ld, wm, wn, acc);
   else tile_loop<C, (C::NI + 3) / 4>(lds, ld, wm, wn, acc);
-  tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
+  tile_store_rows<C>(g, lds, w.c, c_rows, w.cols, wm, wn, acc);
 }
 
 // The ping-pong form of the 256 x 256 tile. Its 8 waves are two groups of 4 (a SIMD has one wave of each), one
@@ -503,55 +546,69 @@ template <class C>
 struct PingPong {
   static constexpr int HM = C::BM / 2, NH = C::NI / 2;                    // rows and a wave's blocks in a half
   static constexpr int HALF = HM * C::PB;
-  static constexpr int LO = 0, HI = HALF, B = 2 * HALF, STAGE = B + C::OPB;      // where they are in a stage
-  static constexpr int SCALES = 2 * STAGE, LDS = SCALES + 4 * C::SCB;             // the scales' ring
+  // where they are in a stage: every read is a lane's address and a 16-bit constant
+  static constexpr int B = 0, LO = C::OPB, HI = LO + HALF, STAGE = HI + HALF;
+  static constexpr int SCALES = 2 * STAGE, OUT = SCALES + 4 * C::SCB;             // the scales' ring; results
+  static constexpr int PLAN = OUT + 8 * 2048, LDS = PLAN + 1024, STORES = 2 * C::NI;
+  static_assert(LDS <= 160 * 1024 && (RowTiles::kWords + 6) * 4 <= 1024, "one CU's LDS");
   using DmaA = PanelDma<C, C::ATR, HM>;
   using DmaB = PanelDma<C, C::BTR, C::BN>;
   static constexpr int P1 = DmaA::PIECES + DmaB::PIECES + (C::SC != kScaleNone ? 1 : 0), P2 = DmaA::PIECES;
   static_assert(C::WM == 2 && C::WN == 4 && C::NBUF == 2 && C::PB == 128, "two groups of four waves, two panels");
 };
 
+// A value that is the same in all lanes, as the compiler should know: it stays in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ size_t uniform(size_t v) {
+  return (size_t)(unsigned)uniform((int)(v >> 32)) << 32 | (unsigned)uniform((int)v);
+}
+__device__ __forceinline__ const char* uniform(const char* p) { return (const char*)uniform((size_t)p); }
+
 template <class C>
 struct PingPongLoader {
   using P = PingPong<C>;
-  typename P::DmaA lo, hi;
+  typename P::DmaA lo, hi;                       // (K-major, they differ in the rows that exist alone)
   typename P::DmaB b;
   const char *pa, *pb, *ps;
-  size_t step_a, step_b;
   long long step_s;
-  unsigned soff;
-  int wave, lane, nk, left;
+  unsigned soff, lda, ldb;
+  int wave, lane, nk, left, a_rows, b_rows;
 
   __device__ __forceinline__ PingPongLoader(const GroupArgs& g, const TileOperands& t, int wave_, int lane_)
-      : pa(t.a), pb(t.b), ps(t.as), step_a(C::ATR ? (size_t)C::KT * t.lda_b : C::PB),
-        step_b(C::BTR ? (size_t)C::KT * t.ldb_b : C::PB), step_s(0), soff(kNowhere), wave(wave_), lane(lane_) {
-    nk = (t.red + C::KT - 1) / C::KT;
-    left = t.red - (nk - 1) * C::KT;
-    lo.init(wave, lane, (unsigned)t.lda_b, t.a_rows, t.a_col0, t.a_cols);
-    if constexpr (C::ATR) {
-      hi.init(wave, lane, (unsigned)t.lda_b, 0, t.a_col0 + P::HM, t.a_cols);
-    } else {
-      hi.init(wave, lane, (unsigned)t.lda_b, t.a_rows - P::HM, 0, 0);
-#pragma unroll
-      for (int i = 0; i < P::DmaA::PIECES; ++i)
-        if (hi.off[i] != kNowhere) hi.off[i] += (unsigned)P::HM * (unsigned)t.lda_b;
+      : pa(uniform(t.a)), pb(uniform(t.b)), ps(t.as), step_s(0), soff(kNowhere), lda((unsigned)uniform((int)t.lda_b)),
+        ldb((unsigned)uniform((int)t.ldb_b)), wave(wave_), lane(lane_), a_rows(uniform(t.a_rows)), b_rows(uniform(t.b_rows)) {
+    const int red = uniform(t.red);
+    nk = (red + C::KT - 1) / C::KT;
+    left = red - (nk - 1) * C::KT;
+    lo.init(wave, lane, lda, t.a_col0, t.a_cols);
+    if constexpr (C::ATR) hi.init(wave, lane, lda, t.a_col0 + P::HM, t.a_cols);
+    b.init(wave, lane, ldb, t.b_col0, t.b_cols);
+    if constexpr (C::SC != kScaleNone) {
+      scale_lanes<C>(g, t, wave, lane, soff, ps, step_s);
+      ps = uniform(ps);
+      step_s = (long long)uniform((size_t)step_s);
     }
-    b.init(wave, lane, (unsigned)t.ldb_b, t.b_rows, t.b_col0, t.b_cols);
-    if constexpr (C::SC != kScaleNone) scale_lanes<C>(g, t, wave, lane, soff, ps, step_s);
   }
+  __device__ __forceinline__ const char* a_panel(int kt) const { return pa + (size_t)kt * (C::ATR ? (size_t)C::KT * lda : C::PB); }
   // B, A's upper half and the scales of panel kt into the stage at `base`
   __device__ __forceinline__ void issue_lo(int kt, char* base, char* ring) {
-    if (kt == nk - 1 && left < C::KT) {
-      lo.cut(wave, lane, left);
-      b.cut(wave, lane, left);
+    const int steps = kt == nk - 1 ? left : C::KT;
+    typename P::DmaA a = lo;
+    if (steps < C::KT) {
+      a.cut(lane, left);
+      b.cut(lane, left);
     }
-    b.load(base + P::B, pb + (size_t)kt * step_b, wave);
-    lo.load(base + P::LO, pa + (size_t)kt * step_a, wave);
+    b.load(base + P::B, pb + (size_t)kt * (C::BTR ? (size_t)C::KT * ldb : C::PB), wave, ldb, C::BTR ? steps : b_rows);
+    a.load(base + P::LO, a_panel(kt), wave, lda, C::ATR ? steps : a_rows);
     if constexpr (C::SC != kScaleNone) scale_load<C>(ring + (kt & 3) * C::SCB, ps + kt * step_s, wave, soff);
   }
   __device__ __forceinline__ void issue_hi(int kt, char* base) {
-    if (kt == nk - 1 && left < C::KT) hi.cut(wave, lane, left);
-    hi.load(base + P::HI, pa + (size_t)kt * step_a, wave);
+    const int steps = kt == nk - 1 ? left : C::KT;
+    typename P::DmaA a = C::ATR ? hi : lo;
+    if (steps < C::KT) a.cut(lane, left);
+    const char* panel = a_panel(kt);
+    if constexpr (!C::ATR) panel += (size_t)P::HM * lda;
+    a.load(base + P::HI, panel, wave, lda, C::ATR ? steps : a_rows - P::HM);
   }
 };
 
@@ -668,28 +725,43 @@ __device__ __forceinline__ void pp_mul(const PingPongFrags<C>& f, gf4 (&acc)[C::
     for (int j = 0; j < C::NJ; ++j) asm volatile("" : "+v"(acc[I0 + i][j]));
 }
 
+// A tile's first panels, into stages that no wave reads any more.
 template <class C>
-__device__ __forceinline__ void pp_loop(char* lds, PingPongLoader<C>& ld, int wave, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+__device__ __forceinline__ void pp_prologue(char* lds, PingPongLoader<C>& ld, int rows) {
+  using P = PingPong<C>;
+  if (ld.nk == 0) return;
+  ld.issue_lo(0, lds, lds + P::SCALES);
+  if (rows <= C::BM / 2) return;
+  ld.issue_hi(0, lds);
+  if (ld.nk > 1) ld.issue_lo(1, lds + P::STAGE, lds + P::SCALES);
+}
+
+// wait_vm<N>, or with `stores` that many of this wave's stores (kStores) more
+template <class C, int N>
+__device__ __forceinline__ void pp_wait(bool stores) {
+  if (stores) wait_vm<N + PingPong<C>::STORES>();
+  else wait_vm<N>();
+}
+
+// After pp_prologue. `stores`: exactly PingPong::STORES of this wave's stores have been issued since, and may go on.
+template <class C>
+__device__ __forceinline__ void pp_loop(char* lds, PingPongLoader<C>& ld, int wave, int wm, int wn, bool stores,
+                                        gf4 (&acc)[C::NI][C::NJ]) {
   using P = PingPong<C>;
   const int nk = ld.nk;
   if (nk == 0) return;
   char* const ring = lds + P::SCALES;
-  ld.issue_lo(0, lds, ring);
-  ld.issue_hi(0, lds);
-  if (nk > 1) {
-    ld.issue_lo(1, lds + P::STAGE, ring);
-    wait_vm<P::P1 + P::P2>();
-  } else {
-    wait_vm<P::P2>();
-  }
+  if (nk > 1) pp_wait<C, P::P1 + P::P2>(stores);
+  else pp_wait<C, P::P2>(stores);
   bar();
   if (wave >= 4) bar();
   for (int kt = 0; kt < nk; ++kt) {
     char* const here = lds + (kt & 1) * P::STAGE;
     char* const there = lds + (~kt & 1) * P::STAGE;
+    const bool st = stores && kt == 0;
     PingPongFrags<C> f;
     pp_read_lo<C>(there, (lds_in)here, (lds_in)ring, ld, kt, wm, wn, f);
-    if (kt + 1 < nk) wait_vm<P::P1 + P::P2>();       // this wave's pieces of the lower half have landed
+    if (kt + 1 < nk) pp_wait<C, P::P1 + P::P2>(st);       // this wave's pieces of the lower half have landed
     else wait_vm<0>();
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     bar();
@@ -699,8 +771,8 @@ __device__ __forceinline__ void pp_loop(char* lds, PingPongLoader<C>& ld, int wa
     bar();
     // (the stage's upper half, B and scales have been read by both groups: panel kt + 2's go there)
     pp_read_hi<C>(here, (lds_in)here, ring, ld, kt, wm, wn, f);
-    if (kt + 2 < nk) wait_vm<P::P1 + P::P2>();       // and of the next panel's first part
-    else wait_vm<P::P2>();
+    if (kt + 2 < nk) pp_wait<C, P::P1 + P::P2>(st);       // and of the next panel's first part
+    else pp_wait<C, P::P2>(st);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     bar();
     __builtin_amdgcn_s_setprio(1);
@@ -725,33 +797,140 @@ __device__ __forceinline__ void pp_half_step(char* __restrict__ into, const __at
 template <class C, int NA>
 __device__ __forceinline__ void pp_half_loop(char* lds, PingPongLoader<C>& ld, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
   using P = PingPong<C>;
-  char* const ring = lds + P::SCALES;
-  if (ld.nk > 0) ld.issue_lo(0, lds, ring);
   for (int kt = 0; kt < ld.nk; ++kt) {
     wait_vm<0>();
     bar();
-    pp_half_step<C, NA>(lds + (~kt & 1) * P::STAGE, (lds_in)lds + (kt & 1) * P::STAGE, ring, ld, kt, wm, wn, acc);
+    pp_half_step<C, NA>(lds + (~kt & 1) * P::STAGE, (lds_in)lds + (kt & 1) * P::STAGE, lds + P::SCALES, ld, kt, wm, wn, acc);
+  }
+  bar();                                                 // every wave has left the stages
+}
+
+// The lane, as a value made here: what is computed from it stays inside the loop over the tiles (hoisted out of it, the
+// addresses of a tile's start and end fill the registers that the sums need).
+__device__ __forceinline__ int lane_here() {
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  return lane;
+}
+
+// The result while the next tile's first panels land: a wave's 16-row blocks one after the other through 2 KiB of its
+// own (no barrier), 8 rows of 128 bytes a store. True: exactly STORES stores (lanes without a row or column store past
+// the buffer's end, nowhere); else as many as it takes.
+template <class C>
+__device__ __forceinline__ bool pp_store(const GroupArgs& g, char* stage, const TileWork& w, int wm, int wn,
+                                         const gf4 (&acc)[C::NI][C::NJ]) {
+  constexpr int OUT = C::DT == kFp16 ? kFp16 : kBf16;
+  const int lane = lane_here(), l16 = lane & 15, q = lane >> 4;
+  const bool fast = ((((uintptr_t)g.c | (uintptr_t)(g.ldc * 2) | (uintptr_t)(g.c_expert * 2)) & 15) | (w.cols & 7)) == 0;
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(w.c, 0, 0x7fffffff, 0x00020000);
+  const int r8 = lane >> 3, c8 = lane & 7, col = wn * C::TN + c8 * 8;
+  static_assert(C::TN == 64, "a wave's rows are 128 bytes");
+#pragma unroll
+  for (int i = 0; i < C::NI; ++i) {
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+      unsigned short v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = to_out<OUT>(acc[i][j][e]);
+      const int c = 2 * j + (q >> 1);
+      *(uint2*)(stage + l16 * 128 + ((c ^ (l16 >> 1)) << 4) + (q & 1) * 8) = make_uint2(v[0] | (unsigned)v[1] << 16, v[2] | (unsigned)v[3] << 16);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int rl = r8 + 8 * h, r = (i * C::WM + wm) * 16 + rl;
+      const gi4 v = *(const gi4*)(stage + rl * 128 + ((c8 ^ (rl >> 1)) << 4));
+      if (fast) {
+        const unsigned at = r < w.rows && col < w.cols ? (unsigned)r * (unsigned)(g.ldc * 2) + (unsigned)col * 2 : kNowhere;
+        __builtin_amdgcn_raw_buffer_store_b128(v, rs, at, 0, 2);        // 2: streaming, as store_c16
+      } else if (r < w.rows) {
+        unsigned short* at = (unsigned short*)w.c + (size_t)r * g.ldc + col;
+        if (col + 8 <= w.cols) {
+          __builtin_memcpy(at, &v, 16);
+        } else {
+          const unsigned short* from = (const unsigned short*)(stage + rl * 128 + ((c8 ^ (rl >> 1)) << 4));
+#pragma unroll 1
+          for (int e = 0; col + e < w.cols; ++e) at[e] = from[e];
+        }
+      }
+    }
+  }
+  return fast;
+}
+
+// The launch's arguments, read here: kept in scalar registers from the start they would not leave the loops enough.
+__device__ __forceinline__ GroupArgs args_here() {
+  const __attribute__((address_space(4))) char* at = (const __attribute__((address_space(4))) char*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  GroupArgs g;
+  __builtin_memcpy(&g, (const char*)at, sizeof(g));
+  return g;
+}
+
+// The workgroup's next item with work: workgroup b of `slots` takes one of every round of `slots` items. Inside a
+// round it keeps its XCD (b & 7) and moves on by 5 places, or the same workgroups would get all of the short tiles that
+// come every 8 items.
+template <class C>
+__device__ __forceinline__ bool pp_next(const GroupArgs& g, TilePlan<C>& plan, int& round, TileWork& w) {
+  const int b = blockIdx.x;
+  for (;; ++round) {
+    const long long base = (long long)round * g.slots;
+    if (base >= plan.items) return false;
+    const int place = (g.slots & 7) == 0 ? ((b >> 3) + 5 * round) % (g.slots >> 3) * 8 + (b & 7) : b;
+    if (base + place < plan.items && plan.work(g, (int)base + place, w)) {
+      ++round;
+      return true;
+    }
   }
 }
 
+// One workgroup a CU, for all of the launch's tiles: the next tile's first panels are fetched before the result of the
+// last one is stored, so that the stores, and the wait for the first panels, run under each other and under the next
+// tile's loop (a workgroup a tile: 11 us a tile between the loops, 9.4 for fp8). What the tiles' starts and ends need
+// is kept in LDS and read there, not in registers across the loops.
 template <class C>
-__global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) group_tile_pp(const GroupArgs g) {
-  __shared__ __attribute__((aligned(16))) char lds[PingPong<C>::LDS];     // the only LDS object: see tile_step
-  if (zero_rest_rows(g, C::THREADS)) return;
-  TileOperands t;
-  char* c_tile;
-  int c_rows, c_cols;
-  if (!tile_setup<C>(g, blockIdx.x, t, c_tile, c_rows, c_cols)) return;
+__global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) group_tile_pp(const GroupArgs args) {
+  using P = PingPong<C>;
+  __shared__ __attribute__((aligned(16))) char lds[P::LDS];     // the only LDS object: see tile_step
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / C::WN, wn = wave % C::WN;
-  PingPongLoader<C> ld(g, t, wave, lane);
-  gf4 acc[C::NI][C::NJ];
+  int* const kept = (int*)(lds + P::PLAN);
+  TileWork w;
+  int round = 0;
+  bool more;
+  {
+    TilePlan<C> plan(args);
+    more = pp_next<C>(args, plan, round, w);
+    if (wave == 0) plan.save(kept);
+  }
+  __syncthreads();
+  if (more) {
+    PingPongLoader<C> ld(args, w.t, wave, lane);
+    pp_prologue<C>(lds, ld, w.rows);
+    int stores = 0;
+    while (more) {
+      gf4 acc[C::NI][C::NJ];
 #pragma unroll
-  for (int i = 0; i < C::NI; ++i)
+      for (int i = 0; i < C::NI; ++i)
 #pragma unroll
-    for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
-  if (c_rows > C::BM / 2) pp_loop<C>(lds, ld, wave, wm, wn, acc);
-  else if (c_rows > C::BM / 4) pp_half_loop<C, PingPong<C>::NH>(lds, ld, wm, wn, acc);
-  else pp_half_loop<C, PingPong<C>::NH / 2>(lds, ld, wm, wn, acc);
-  tile_store_rows<C>(g, lds, c_tile, c_rows, c_cols, wm, wn, acc);
+        for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
+      if (w.rows > C::BM / 2) pp_loop<C>(lds, ld, wave, wm, wn, stores, acc);
+      else if (w.rows > C::BM / 4) pp_half_loop<C, P::NH>(lds, ld, wm, wn, acc);
+      else pp_half_loop<C, P::NH / 2>(lds, ld, wm, wn, acc);
+      const GroupArgs g = args_here();
+      TileWork next;
+      TilePlan<C> plan;
+      plan.load(g, kept);
+      more = uniform((int)pp_next<C>(g, plan, round, next));
+      if (more) {
+        ld = PingPongLoader<C>(g, next.t, wave, lane_here());
+        pp_prologue<C>(lds, ld, next.rows);
+      }
+      stores = uniform((int)pp_store<C>(g, lds + P::OUT + wave * 2048, w, wm, wn, acc));
+      w.c = (char*)uniform((const char*)next.c);
+      w.rows = uniform(next.rows);
+      w.cols = uniform(next.cols);
+    }
+  }
+  const GroupArgs g = args_here();
+  zero_rest_rows(g, blockIdx.x, g.slots, C::THREADS);
 }

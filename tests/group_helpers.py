@@ -12,6 +12,10 @@ has under 2^(E - 13) is cut off (measured: of 448 * 448 - 448 * 448 + t, E = 16,
 and lost from 2^2 on; of 1 - 1 + t down to 2^-13; steps 8 apart do not touch each other). A product of two e4m3 values
 has 8 significant bits, so the largest is whole, and the 7 others lose less than 2^(E - 13) <= 2^-13 of the largest
 product's magnitude each: 7 * 2^-13 * (the sum over the groups of 8 of the largest product), `fp8_slack` below.
+A subnormal's exponent counts as the least one, -6, whatever its leading zeros (measured: of 2^-9 * 256 - 2^-9 * 256 +
+t, E = -6 + 8 = 2, t is kept down to 2^-11 and lost from 2^-12 on; a zero times 448 hides nothing). Its product's lowest
+bit is still 2^(E - 6) or more, so whole, but the product itself can be less than 2^E. "The largest product" is
+therefore that of the factors' magnitudes with a subnormal's raised to 2^-6: `raised64` gives such operands.
 """
 
 import torch
@@ -42,8 +46,15 @@ def tolerance(ref, mag, terms, dtype):
     return eps * (ref.abs() + sums) + sums + low
 
 
+def raised64(q, s, block_rows):
+    """The magnitudes of the block-scaled codes q, those of subnormal codes raised to the least normal one's."""
+    v = q.double().abs()
+    return dequantize64(torch.where(v > 0, v.clamp_min(2.0 ** -6), v), s, block_rows)
+
+
 def fp8_slack(x, w):
-    """7 * 2^-13 * sum over groups of 8 reduction steps of the largest |x w|, for each element of x @ w.T."""
+    """7 * 2^-13 * sum over groups of 8 reduction steps of the largest |x w|, for each element of x @ w.T; x and w as
+    `raised64` gives them."""
     x, w = (torch.nn.functional.pad(v.abs(), (0, -v.shape[1] % 8)) for v in (x, w))
     total = torch.zeros((x.shape[0], w.shape[0]), dtype=torch.float64, device=x.device)
     for k in range(0, x.shape[1], 8):

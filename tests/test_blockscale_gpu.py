@@ -122,7 +122,7 @@ def test_gemm(cuda_device, m, n, k, scale_dtype):
     a, sa, bt, sb = _operands(cuda_device, m, n, k, scale_dtype)
     x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
     H.check(B.gemm_fp8_block(a, sa, bt, sb), x @ w.t(), x.abs() @ w.abs().t(), k + 3 * -(-k // 128),
-            H.fp8_slack(x, w))
+            H.fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128)))
 
 
 @pytest.mark.parametrize("scale_dtype", SCALES)
@@ -138,7 +138,7 @@ def test_grouped_gemm(cuda_device, sizes, n, k, scale_dtype):
     x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
     ref, mag = H.forward64(x, w, off)
     got = B.gemm_grouped_fp8_block(a, sa, bt, sb, off)
-    H.check(got, ref, mag, k + 3 * -(-k // 128), H.grouped_fp8_slack(x, w, off))
+    H.check(got, ref, mag, k + 3 * -(-k // 128), H.grouped_fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128), off))
     out = torch.full_like(got, 5.0)
     B.gemm_grouped_fp8_block(a, sa, bt, sb, off, out)
     assert torch.equal(out[:-tail], got[:-tail]) and (out[-tail:] == 5.0).all()
@@ -188,7 +188,7 @@ def test_power_of_two_scales_are_float32_ones(cuda_device):
     a, sa, bt, sb = _operands(cuda_device, 130, 256, 512, torch.float8_e8m0fnu)
     x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
     for s, t in ((sa, sb), (sa.float(), sb.float())):
-        H.check(B.gemm_fp8_block(a, s, bt, t), x @ w.t(), x.abs() @ w.abs().t(), 512 + 12, H.fp8_slack(x, w))
+        H.check(B.gemm_fp8_block(a, s, bt, t), x @ w.t(), x.abs() @ w.abs().t(), 512 + 12, H.fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128)))
 
 
 @pytest.mark.parametrize("scale_dtype", SCALES)
@@ -229,9 +229,9 @@ def test_serving_path(cuda_device, scale_dtype):
         x64 = vx * sv.float().double().repeat_interleave(128, 1)[:, :h]
         w64 = H.dequantize64(q1, s1, 128)
         ref, mag = H.forward64(x64, w64, off)
-        H.check(up, ref, mag, h + 6, H.grouped_fp8_slack(x64, w64, off))
+        H.check(up, ref, mag, h + 6, H.grouped_fp8_slack(H.raised64(vx, sv, 1), H.raised64(q1, s1, 128), off))
         vy, sv = H.quantize64(y, 1, scale_dtype != torch.float32)
         y64 = vy * sv.float().double().repeat_interleave(128, 1)[:, :f]
         w64 = H.dequantize64(q2, s2, 128)
         ref, mag = H.forward64(y64, w64, off)
-        H.check(out, ref, mag, f + 9, H.grouped_fp8_slack(y64, w64, off))
+        H.check(out, ref, mag, f + 9, H.grouped_fp8_slack(H.raised64(vy, sv, 1), H.raised64(q2, s2, 128), off))

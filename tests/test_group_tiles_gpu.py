@@ -1,0 +1,250 @@
+"""The grouped and block-scaled products at the sizes that fill the card: every tile shape, each against 64 bits."""
+
+import pytest
+import torch
+
+import group_helpers as H
+
+pytestmark = pytest.mark.gpu
+
+SCALES = [torch.float32, torch.float8_e8m0fnu]
+
+
+def _rand(dev, seed, dtype, *shape, scale=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=dev) * scale).to(dtype)
+
+
+def _codes(dev, seed, *shape):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    c = torch.randint(0, 256, shape, generator=g, device=dev, dtype=torch.int16)
+    return torch.where((c & 0x7F) == 0x7F, c ^ 1, c).to(torch.uint8).view(torch.float8_e4m3fn)
+
+
+def _scales(dev, seed, dtype, *shape):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    s = torch.exp2(torch.randint(-12, 3, shape, generator=g, device=dev).float())
+    return s * (1 + torch.rand(shape, generator=g, device=dev)) if dtype == torch.float32 else s.to(dtype)
+
+
+# sizes, N, K, rows before the first expert, rows behind the last. Over 205 tiles of 256 x 256 and over 128 rows a
+# group, so the largest tiles: reductions of one, two, three and many panels, a last panel that is not whole, column
+# tails of 1 to 255, last row tiles of 1 to 256 rows, empty experts, more experts than a wave has lanes.
+BIG = [
+    ([3000, 0, 1, 257, 2500, 255, 1200, 64], 1536, 1024, 0, 0),
+    ([2048, 2048, 2100, 2040], 1800, 64, 0, 5),
+    ([4000, 129, 0, 0, 4200], 1601, 100, 3, 0),
+    ([1500, 1501, 1502, 1503, 1504], 1793, 130, 0, 70),
+    ([9000], 1544, 520, 0, 0),
+    ([150 + i for i in range(130)], 520, 200, 11, 300),
+    ([700, 900, 500], 8200, 72, 40, 1),
+    ([6000, 10], 2304, 8, 0, 0),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,n,k,first,tail", BIG)
+def test_forward(cuda_device, sizes, n, k, first, tail, dtype):
+    from gpu_operator_amd.ops import grouped as G
+
+    t, owned = first + sum(sizes) + tail, slice(first, first + sum(sizes))
+    a = _rand(cuda_device, 1, dtype, t, k)
+    bt = _rand(cuda_device, 2, dtype, len(sizes), n, k, scale=k ** -0.5)
+    off = H.offsets_of(sizes, first, cuda_device)
+    a[:first], a[t - tail:] = float("nan"), float("inf")
+    got = G.gemm_grouped(a, bt, off)
+    ref, mag = H.forward64(a, bt, off)
+    H.check(got, ref, mag, k)
+    out = torch.full((t, n + 8), 7.0, dtype=dtype, device=cuda_device)
+    G.gemm_grouped(a, bt, off, out[:, :n])
+    assert torch.equal(out[owned, :n], got[owned])
+    out[owned, :n] = 7.0
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,n,k,first,tail", BIG)
+def test_dgrad(cuda_device, sizes, n, k, first, tail, dtype):
+    """The same sizes with the reduction over K columns of the weights and N outputs."""
+    from gpu_operator_amd.ops import grouped as G
+
+    t = first + sum(sizes) + tail
+    dc = _rand(cuda_device, 3, dtype, t, k)
+    bt = _rand(cuda_device, 4, dtype, len(sizes), k, n, scale=k ** -0.5)
+    off = H.offsets_of(sizes, first, cuda_device)
+    dc[:first], dc[t - tail:] = float("nan"), float("inf")
+    ref, mag = H.dgrad64(dc, bt, off)
+    H.check(G.gemm_grouped_dgrad(dc, bt, off), ref, mag, k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes,n,k,first,tail", [
+    ([0, 1, 63, 64, 65, 128, 129, 600, 0, 500], 1500, 1000, 0, 0),
+    ([2000, 31, 0], 2304, 2056, 5, 70),
+    ([300] * 12, 1030, 1032, 0, 3),
+    ([1] + [250] * 8, 1281, 1281, 1, 0),
+])
+def test_wgrad(cuda_device, sizes, n, k, first, tail, dtype):
+    from gpu_operator_amd.ops import grouped as G
+
+    t = first + sum(sizes) + tail
+    a, dc = _rand(cuda_device, 5, dtype, t, k), _rand(cuda_device, 6, dtype, t, n)
+    off = H.offsets_of(sizes, first, cuda_device)
+    for x in (a, dc):
+        x[:first], x[t - tail:] = float("nan"), float("inf")
+    ref, mag = H.wgrad64(dc, a, off)
+    H.check(G.gemm_grouped_wgrad(dc, a, off), ref, mag, max(sizes))
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("sizes,n,k,first,tail", BIG)
+def test_grouped_fp8(cuda_device, sizes, n, k, first, tail, scale_dtype):
+    from gpu_operator_amd.ops import blockscale as B
+
+    t, e, kb, nb = first + sum(sizes) + tail, len(sizes), -(-k // 128), -(-n // 128)
+    a, bt = _codes(cuda_device, 7, t, k), _codes(cuda_device, 8, e, n, k)
+    sa, sb = _scales(cuda_device, 9, scale_dtype, t, kb), _scales(cuda_device, 10, scale_dtype, e, nb, kb)
+    off = H.offsets_of(sizes, first, cuda_device)
+    for r in (slice(0, first), slice(t - tail, t)):
+        a.view(torch.uint8)[r] = 0x7F
+    x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
+    ref, mag = H.forward64(x, w, off)
+    slack = H.grouped_fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128), off)
+    H.check(B.gemm_grouped_fp8_block(a, sa, bt, sb, off), ref, mag, k + 3 * kb, slack)
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("m,n,k", [(4096, 4096, 128), (4097, 3840, 300), (3500, 4104, 1152), (8000, 1793, 96), (6000, 2304, 272)])
+def test_fp8(cuda_device, m, n, k, scale_dtype):
+    from gpu_operator_amd.ops import blockscale as B
+
+    kb, nb = -(-k // 128), -(-n // 128)
+    a, bt = _codes(cuda_device, 11, m, k), _codes(cuda_device, 12, n, k)
+    sa, sb = _scales(cuda_device, 13, scale_dtype, m, kb), _scales(cuda_device, 14, scale_dtype, nb, kb)
+    x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
+    got = B.gemm_fp8_block(a, sa, bt, sb)
+    H.check(got, x @ w.t(), x.abs() @ w.abs().t(), k + 3 * kb, H.fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128)))
+    # scales stored column by column
+    cols = [s.view(torch.uint8 if scale_dtype != torch.float32 else scale_dtype).t().contiguous().t().view(scale_dtype) for s in (sa, sb)]
+    assert torch.equal(B.gemm_fp8_block(a, cols[0], bt, cols[1]), got)
+
+
+# one case for each smaller tile shape: (sizes, N, K)
+MIDDLE = [([40, 30, 0, 50] * 8, 2048, 256), ([100] * 16, 2000, 320), ([300, 200, 10, 0], 1000, 1000), ([2000], 264, 520),
+          ([20] * 60, 1288, 200), ([500, 490], 1792, 136)]
+
+
+@pytest.mark.parametrize("sizes,n,k", MIDDLE)
+def test_middle_sizes(cuda_device, sizes, n, k):
+    from gpu_operator_amd.ops import blockscale as B
+    from gpu_operator_amd.ops import grouped as G
+
+    t, e = sum(sizes), len(sizes)
+    off = H.offsets_of(sizes, 0, cuda_device)
+    a, dc = _rand(cuda_device, 15, torch.bfloat16, t, k), _rand(cuda_device, 16, torch.bfloat16, t, n)
+    bt = _rand(cuda_device, 17, torch.bfloat16, e, n, k, scale=k ** -0.5)
+    for got, (ref, mag), terms in ((G.gemm_grouped(a, bt, off), H.forward64(a, bt, off), k),
+                                   (G.gemm_grouped_dgrad(dc, bt, off), H.dgrad64(dc, bt, off), n),
+                                   (G.gemm_grouped_wgrad(dc, a, off), H.wgrad64(dc, a, off), max(sizes))):
+        H.check(got, ref, mag, terms)
+    for scale_dtype in SCALES:
+        qa, sa = B.quantize_fp8_block(a, scale_dtype=scale_dtype)
+        qb, sb = B.quantize_fp8_block(bt, 128, scale_dtype=scale_dtype)
+        x, w = H.dequantize64(qa, sa, 1), H.dequantize64(qb, sb, 128)
+        ref, mag = H.forward64(x, w, off)
+        slack = H.grouped_fp8_slack(H.raised64(qa, sa, 1), H.raised64(qb, sb, 128), off)
+        H.check(B.gemm_grouped_fp8_block(qa, sa, qb, sb, off), ref, mag, k + 3 * -(-k // 128), slack)
+
+
+def _shifted(x):
+    """x at an address and with rows that are not on 16 bytes."""
+    flat = torch.empty(1 + x[..., 0].numel() * (x.shape[-1] + 1), dtype=x.dtype, device=x.device)
+    v = flat[1:].view(*x.shape[:-1], x.shape[-1] + 1)[..., : x.shape[-1]]
+    v.copy_(x)
+    return v
+
+
+def test_unaligned_operands_at_every_size(cuda_device):
+    """Operands that have to be laid out first: the aligned ones' bits, for the largest tiles and small ones, in every
+    direction; an fp8 product whose N and K are not multiples of 16."""
+    from gpu_operator_amd.ops import blockscale as B
+    from gpu_operator_amd.ops import grouped as G
+
+    for sizes, n, k in (([3000, 0, 4000, 1], 1801, 515), ([70, 0, 33], 135, 77)):
+        t, e = sum(sizes), len(sizes)
+        off = H.offsets_of(sizes, 0, cuda_device)
+        a, dc = _rand(cuda_device, 18, torch.bfloat16, t, k), _rand(cuda_device, 19, torch.bfloat16, t, n)
+        bt = _rand(cuda_device, 20, torch.bfloat16, e, n, k, scale=k ** -0.5)
+        for fn, x, y, (ref, mag), terms in ((G.gemm_grouped, a, bt, H.forward64(a, bt, off), k),
+                                            (G.gemm_grouped_dgrad, dc, bt, H.dgrad64(dc, bt, off), n),
+                                            (G.gemm_grouped_wgrad, dc, a, H.wgrad64(dc, a, off), max(sizes))):
+            got = fn(x, y, off)
+            H.check(got, ref, mag, terms)
+            assert torch.equal(fn(_shifted(x), _shifted(y), off), got)
+    a, bt = _codes(cuda_device, 21, 5000, 301), _codes(cuda_device, 22, 3001, 301)
+    sa, sb = _scales(cuda_device, 23, torch.float32, 5000, 3), _scales(cuda_device, 24, torch.float32, 24, 3)
+    x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
+    H.check(B.gemm_fp8_block(a, sa, bt, sb), x @ w.t(), x.abs() @ w.abs().t(), 301 + 9, H.fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128)))
+
+
+@pytest.mark.parametrize("sizes,n,k", [([3000, 0, 4000, 1], 1801, 515), ([70, 0, 33], 135, 77), ([2, 0, 1], 135, 77)])
+def test_unaligned_operands_in_a_graph(cuda_device, sizes, n, k):
+    """The workspace that unaligned operands are laid out in belongs to the graph: replays over new inputs, with eager
+    calls of the same operators between them, give the eager results."""
+    from gpu_operator_amd.ops import grouped as G
+
+    t, e = sum(sizes), len(sizes)
+    off = H.offsets_of(sizes, 0, cuda_device)
+    a, dc = _rand(cuda_device, 25, torch.bfloat16, t, k), _rand(cuda_device, 26, torch.bfloat16, t, n)
+    bt = _rand(cuda_device, 27, torch.bfloat16, e, n, k)
+
+    def step():
+        return G.gemm_grouped(a, bt, off), G.gemm_grouped_dgrad(dc, bt, off), G.gemm_grouped_wgrad(dc, a, off)
+
+    step()
+    graphs, outs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(step())
+    for seed in range(3):
+        for x in (a, dc, bt):
+            x.copy_(_rand(cuda_device, 28 + seed, torch.bfloat16, *x.shape))
+        for graph in graphs:
+            graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for out in outs:
+            assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_two_streams_at_once(cuda_device):
+    """Products of either kind queued on two streams without a wait between them: each stream's own results."""
+    from gpu_operator_amd.ops import blockscale as B
+    from gpu_operator_amd.ops import grouped as G
+
+    work = []
+    for seed in range(2):
+        sizes = H.random_sizes(8000, 6, seed=seed + 1)
+        off = H.offsets_of(sizes, 0, cuda_device)
+        a = _rand(cuda_device, 40 + seed, torch.bfloat16, 8000, 515)          # unaligned: laid out on its own stream
+        bt = _rand(cuda_device, 50 + seed, torch.bfloat16, 6, 1544, 515)
+        dc = _rand(cuda_device, 60 + seed, torch.bfloat16, 8000, 1544)
+
+        def step(a=a, bt=bt, dc=dc, off=off):
+            q, s = B.quantize_fp8_block(a)
+            qw, sw = B.quantize_fp8_block(bt, 128)
+            return (G.gemm_grouped(a, bt, off), G.gemm_grouped_dgrad(dc, bt, off), G.gemm_grouped_wgrad(dc, a, off),
+                    B.gemm_grouped_fp8_block(q, s, qw, sw, off))
+
+        work.append((step, torch.cuda.Stream()))
+    want = [step() for step, _ in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for i, (step, stream) in enumerate(work):
+            with torch.cuda.stream(stream):
+                got[i].append(step())
+    torch.cuda.synchronize()
+    for w, rounds in zip(want, got):
+        for r in rounds:
+            assert all(torch.equal(p, q) for p, q in zip(r, w))
