@@ -125,7 +125,10 @@ int skinny_rows(const GroupArgs& g) {
 // The tile, by how many there are (`cus` workgroups run at once, or twice that) and how many rows a group has:
 //
 //   Large    256 x 256, ping-pong, one a CU: groups that fill it and a grid that nearly fills the CUs (16 groups of
-//            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1)
+//            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1); from 5/16 of the CUs on where the groups are
+//            long, since a part of a tile is most of its width still (1280 x 4096 x 4096 fp8, 80 tiles as 240 parts:
+//            35.2 us, Deep 40.9; 2560 rows, 160 tiles: 52.1, 60.9; 64 tiles: 31.1, Low 26.9; 8 groups of 160 rows, 4096 x
+//            2048: 39.3, Deep 32.0)
 //   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: grids of nearly two
 //            rounds or more (32 fp8 groups of 64 rows, 4096 x 2048: 64.8 us, Low 71.6, Large 74.6)
 //   Deep     128 x 128, 8 waves, a ring of four: smaller grids, where a workgroup's own latency is the time (fp8 256 x
@@ -143,13 +146,15 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   if constexpr (!ATR && !BTR) {
     switch (skinny_rows(g)) {
       case 1: return ready ? skinny_columns<DT, SC, 1>(g, s) : skinny_unaligned<DT, SC, 1>(g, s);
-      case 2: return ready ? skinny_columns<DT, SC, 2>(g, s) : skinny_unaligned<DT, SC, 2>(g, s);
+      case 2:                                        // (a product without groups is an fp8 one)
+        if constexpr (DT == kFp8) return ready ? skinny_columns<DT, SC, 2>(g, s) : skinny_unaligned<DT, SC, 2>(g, s);
     }
   }
   if (!ready) return kNeedsPacking;
   const int cus = device_cu_count(s);
   // (a Large tile's stores are 32-bit offsets in it)
-  const bool large_fills = 5 * tile_grid<Large>(g) >= 4 * cus && g.ldc * 2 * 256 < 0x7fffffffll;
+  const long long large = g.ldc * 2 * 256 < 0x7fffffffll ? tile_grid<Large>(g) : 0;
+  const bool large_fills = 5 * large >= 4 * cus;
   if constexpr (ATR) {
     if (large_fills && g.red >= 128ll * g.experts) return launch_tile<Large, kTilePingPong>(g, s);
     return launch_tile<Small, kTileDma>(g, s);
@@ -157,7 +162,7 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
     using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 128, 4>;
     using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 128, 3>;
     const long long per_group = g.rows / g.experts, small = tile_grid<Small>(g);
-    if (large_fills && per_group > 128) return launch_tile<Large, kTilePingPong>(g, s);
+    if ((large_fills && per_group > 128) || (16 * large >= 5 * cus && per_group >= 512)) return launch_tile<Large, kTilePingPong>(g, s);
     const bool near_two_rounds = 4 * small > 7 * cus;
     if (4 * small <= cus || per_group <= (near_two_rounds ? 48 : 32)) return launch_tile<Low, kTileDma>(g, s);
     if (near_two_rounds) return launch_tile<Small, kTileDma>(g, s);

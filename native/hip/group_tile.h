@@ -548,8 +548,10 @@ struct PingPong {
   static constexpr int HALF = HM * C::PB;
   // where they are in a stage: every read is a lane's address and a 16-bit constant
   static constexpr int B = 0, LO = C::OPB, HI = LO + HALF, STAGE = HI + HALF;
-  static constexpr int SCALES = 2 * STAGE, OUT = SCALES + 4 * C::SCB;             // the scales' ring; results
-  static constexpr int PLAN = OUT + 8 * 2048, LDS = PLAN + 1024, STORES = 2 * C::NI;
+  // a half tile's panels: a ring of three, the last of them over the results
+  static constexpr int HSTAGE = HI;
+  static constexpr int OUT = 2 * STAGE, OUT_END = 3 * HSTAGE > OUT + 8 * 2048 ? 3 * HSTAGE : OUT + 8 * 2048;
+  static constexpr int SCALES = OUT_END, PLAN = SCALES + 4 * C::SCB, LDS = PLAN + 1024, STORES = 2 * C::NI;
   static_assert(LDS <= 160 * 1024 && (RowTiles::kWords + 6) * 4 <= 1024, "one CU's LDS");
   using DmaA = PanelDma<C, C::ATR, HM>;
   using DmaB = PanelDma<C, C::BTR, C::BN>;
@@ -730,10 +732,10 @@ template <class C>
 __device__ __forceinline__ void pp_prologue(char* lds, PingPongLoader<C>& ld, int rows) {
   using P = PingPong<C>;
   if (ld.nk == 0) return;
+  const bool half = rows <= C::BM / 2;
   ld.issue_lo(0, lds, lds + P::SCALES);
-  if (rows <= C::BM / 2) return;
-  ld.issue_hi(0, lds);
-  if (ld.nk > 1) ld.issue_lo(1, lds + P::STAGE, lds + P::SCALES);
+  if (!half) ld.issue_hi(0, lds);
+  if (ld.nk > 1) ld.issue_lo(1, lds + (half ? P::HSTAGE : P::STAGE), lds + P::SCALES);
 }
 
 // wait_vm<N>, or with `stores` that many of this wave's stores (kStores) more
@@ -783,26 +785,42 @@ __device__ __forceinline__ void pp_loop(char* lds, PingPongLoader<C>& ld, int wa
   if (wave < 4) bar();
 }
 
-// A tile of at most half the rows: its upper half alone, NA of a wave's blocks, all waves in step.
+// A tile of at most half the rows: its upper half alone, NA of a wave's blocks. The two groups take turns here too, with
+// two intervals a panel and a ring of three: panel t + 2 goes where panel t - 1 was, which both groups have read.
 template <class C, int NA>
-__device__ __forceinline__ void pp_half_step(char* __restrict__ into, const __attribute__((address_space(3))) char* __restrict__ from,
-                                             char* ring, PingPongLoader<C>& ld, int kt, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
-  if (kt + 1 < ld.nk) ld.issue_lo(kt + 1, into, ring);
-  PingPongFrags<C> f;
+__device__ __forceinline__ void pp_half_read(char* __restrict__ into, const __attribute__((address_space(3))) char* __restrict__ from,
+                                             char* ring, PingPongLoader<C>& ld, int kt, int wm, int wn, PingPongFrags<C>& f) {
   pp_frags_lo<C, NA>(from, wm, wn, f);
   pp_scales<C, NA, 0>((lds_in)ring, kt, wm, wn, f);
-  pp_mul<C, 0, NA>(f, acc);
+  if (kt + 2 < ld.nk) ld.issue_lo(kt + 2, into, ring);
 }
 
 template <class C, int NA>
-__device__ __forceinline__ void pp_half_loop(char* lds, PingPongLoader<C>& ld, int wm, int wn, gf4 (&acc)[C::NI][C::NJ]) {
+__device__ __forceinline__ void pp_half_loop(char* lds, PingPongLoader<C>& ld, int wave, int wm, int wn, bool stores,
+                                             gf4 (&acc)[C::NI][C::NJ]) {
   using P = PingPong<C>;
-  for (int kt = 0; kt < ld.nk; ++kt) {
-    wait_vm<0>();
+  const int nk = ld.nk;
+  if (nk == 0) return;
+  if (nk > 1) pp_wait<C, P::P1>(stores);
+  else pp_wait<C, 0>(stores);
+  bar();
+  if (wave >= 4) bar();
+  int buf = 0;
+  for (int kt = 0; kt < nk; ++kt) {
+    const bool st = stores && kt == 0;
+    PingPongFrags<C> f;
+    pp_half_read<C, NA>(lds + (buf == 0 ? 2 : buf - 1) * P::HSTAGE, (lds_in)lds + buf * P::HSTAGE, lds + P::SCALES, ld, kt, wm, wn, f);
+    if (kt + 2 < nk) pp_wait<C, P::P1>(st);                // this wave's pieces of the next panel have landed
+    else pp_wait<C, 0>(st);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     bar();
-    pp_half_step<C, NA>(lds + (~kt & 1) * P::STAGE, (lds_in)lds + (kt & 1) * P::STAGE, lds + P::SCALES, ld, kt, wm, wn, acc);
+    __builtin_amdgcn_s_setprio(1);
+    pp_mul<C, 0, NA>(f, acc);
+    __builtin_amdgcn_s_setprio(0);
+    bar();
+    buf = buf == 2 ? 0 : buf + 1;
   }
-  bar();                                                 // every wave has left the stages
+  if (wave < 4) bar();
 }
 
 // The lane, as a value made here: what is computed from it stays inside the loop over the tiles (hoisted out of it, the
@@ -914,8 +932,8 @@ __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int j = 0; j < C::NJ; ++j) acc[i][j] = gf4{0.f, 0.f, 0.f, 0.f};
       if (w.rows > C::BM / 2) pp_loop<C>(lds, ld, wave, wm, wn, stores, acc);
-      else if (w.rows > C::BM / 4) pp_half_loop<C, P::NH>(lds, ld, wm, wn, acc);
-      else pp_half_loop<C, P::NH / 2>(lds, ld, wm, wn, acc);
+      else if (w.rows > C::BM / 4) pp_half_loop<C, P::NH>(lds, ld, wave, wm, wn, stores, acc);
+      else pp_half_loop<C, P::NH / 2>(lds, ld, wave, wm, wn, stores, acc);
       const GroupArgs g = args_here();
       TileWork next;
       TilePlan<C> plan;

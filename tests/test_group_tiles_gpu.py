@@ -129,20 +129,24 @@ def test_fp8(cuda_device, m, n, k, scale_dtype):
     assert torch.equal(B.gemm_fp8_block(a, cols[0], bt, cols[1]), got)
 
 
-# one case for each smaller tile shape: (sizes, N, K)
-MIDDLE = [([40, 30, 0, 50] * 8, 2048, 256), ([100] * 16, 2000, 320), ([300, 200, 10, 0], 1000, 1000), ([2000], 264, 520),
+# cases for each smaller tile shape in each direction, for parts of the largest tiles on an idle card, and for many groups
+# of a few rows: (sizes, N, K)
+MIDDLE = [([64, 70, 0, 130] * 8, 1992, 256), ([64, 70, 0, 130] * 8, 256, 1992), ([8, 12, 0, 9] * 16, 640, 320),
+          ([1290], 4096, 200), ([700, 600], 200, 4100), ([1500, 1536], 1400, 264),
+          ([40, 30, 0, 50] * 8, 2048, 256), ([100] * 16, 2000, 320), ([300, 200, 10, 0], 1000, 1000), ([2000], 264, 520),
           ([20] * 60, 1288, 200), ([500, 490], 1792, 136)]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("sizes,n,k", MIDDLE)
-def test_middle_sizes(cuda_device, sizes, n, k):
+def test_middle_sizes(cuda_device, sizes, n, k, dtype):
     from gpu_operator_amd.ops import blockscale as B
     from gpu_operator_amd.ops import grouped as G
 
     t, e = sum(sizes), len(sizes)
     off = H.offsets_of(sizes, 0, cuda_device)
-    a, dc = _rand(cuda_device, 15, torch.bfloat16, t, k), _rand(cuda_device, 16, torch.bfloat16, t, n)
-    bt = _rand(cuda_device, 17, torch.bfloat16, e, n, k, scale=k ** -0.5)
+    a, dc = _rand(cuda_device, 15, dtype, t, k), _rand(cuda_device, 16, dtype, t, n)
+    bt = _rand(cuda_device, 17, dtype, e, n, k, scale=k ** -0.5)
     for got, (ref, mag), terms in ((G.gemm_grouped(a, bt, off), H.forward64(a, bt, off), k),
                                    (G.gemm_grouped_dgrad(dc, bt, off), H.dgrad64(dc, bt, off), n),
                                    (G.gemm_grouped_wgrad(dc, a, off), H.wgrad64(dc, a, off), max(sizes))):
