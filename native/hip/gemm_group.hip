@@ -19,14 +19,15 @@ enum TileKernel { kTileDma, kTilePingPong };
 template <class C, TileKernel KERNEL>
 int launch_tile(const GroupArgs& g, hipStream_t s) {
   GroupArgs a = g;
-  const int resident = device_cu_count(s) * (KERNEL == kTilePingPong ? 1 : C::RESIDENT);
-  a.slots = KERNEL == kTilePingPong || g.mode != kModeWgrad ? resident : 0;
-  if (tile_grid<C>(g) > 0x7fffffff - 2 * (long long)resident) return (int)hipErrorInvalidValue;
+  const int cus = device_cu_count(s);
+  a.slots = KERNEL == kTilePingPong || g.mode != kModeWgrad ? cus : 0;
+  if (tile_grid<C>(g) > 0x7fffffff - 2 * (long long)cus) return (int)hipErrorInvalidValue;
   if (tile_grid<C>(g) == 0) return 0;
   if constexpr (KERNEL == kTilePingPong) {
-    hipLaunchKernelGGL((group_tile_pp<C>), dim3((unsigned)resident), dim3(C::THREADS), 0, s, a);
+    hipLaunchKernelGGL((group_tile_pp<C>), dim3((unsigned)cus), dim3(C::THREADS), 0, s, a);
   } else {
-    // the last tiles are cut into parts: at most one more round of workgroups
+    // The last tiles are cut into parts, at most one more round of workgroups of one a CU (of as many as fit a CU, 80 x 8192 x
+    // 8192 fp8 took 42 us for 30: the parts read their columns of B once each).
     const long long grid = tile_grid<C>(g) + a.slots + (g.zero_rest ? kRestBlocks : 0);
     hipLaunchKernelGGL((group_tile_dma<C>), dim3((unsigned)grid), dim3(C::THREADS), 0, s, a);
   }
@@ -122,22 +123,26 @@ int skinny_rows(const GroupArgs& g) {
   return g.rows <= 12 * busy ? 1 : 0;
 }
 
-// The tile, by how many there are (`cus` workgroups run at once, or twice that) and how many rows a group has:
+// The tile, by how many there are and how many rows a group has:
 //
 //   Large    256 x 256, ping-pong, one a CU: groups that fill it and a grid that nearly fills the CUs (16 groups of
 //            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1); from 5/16 of the CUs on where the groups are
 //            long, since a part of a tile is most of its width still (1280 x 4096 x 4096 fp8, 80 tiles as 240 parts:
-//            35.2 us, Deep 40.9; 2560 rows, 160 tiles: 52.1, 60.9; 64 tiles: 31.1, Low 26.9; 8 groups of 160 rows, 4096 x
+//            35.2 us, Deep 40.9; 2560 rows, 160 tiles: 52.1, 60.9; 64 tiles: 31.1, Low 27.2; 8 groups of 160 rows, 4096 x
 //            2048: 39.3, Deep 32.0)
-//   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: grids of nearly two
-//            rounds or more (32 fp8 groups of 64 rows, 4096 x 2048: 64.8 us, Low 71.6, Large 74.6)
-//   Deep     128 x 128, 8 waves, a ring of four: smaller grids, where a workgroup's own latency is the time (fp8 256 x
-//            8192 x 8192: 44.3 us, Low 54.9, Small 63.8; 32 groups of 64 rows, 1024 x 2048: 37.2, 42.2, 45.9)
-//   Low      64 x 128, a ring of three: few rows, or few tiles (fp8 128 x 4096 x 4096: 16.3 us, Deep 20.2, Small 23.1;
-//            20 groups of 30 rows, 1024 x 1024: 12.7, 13.7, 15.2; 32 fp8 groups of 32, 2048 x 2048: 32.1, 41.8, 34.6)
+//   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: one round to about
+//            two of groups that fill most of it (16 groups of 128 rows, 2048 x 2048: 41.3 us, Low 47.5, Deep 44.9;
+//            700 x 8192 x 2048 fp8: 17.8, 23.3, 25.5; 32 groups of 94 rows, 880 tiles: 83.7, 70.6, 73.7)
+//   Deep     128 x 128, 8 waves, a ring of four: most of one round, where a workgroup's own latency is the time (fp8
+//            512 x 8192 x 8192: 52.9 us, Low 59.7, Small 60.2; 16 groups of 125 rows, 1024 x 2048: 23.4, 26.2, 32.6)
+//   Low      64 x 128, a ring of three: few rows a group, or fewer tiles than that (fp8 128 x 4096 x 4096: 13.5 us,
+//            Deep 16.7, Small 21.9; 4 groups of 250 rows, 2048 x 2048: 18.8, 22.7, 24.7; 20 groups of 30 rows, 1024 x
+//            1024: 10.6, 13.1, 14.3; 32 fp8 groups of 32, 2048 x 2048: 26.1, 33.5, 28.7)
 //
-// A weight gradient has whole tiles whatever the groups are; with short reductions the stores are the time, and two
-// workgroups a CU overlap them (20 groups of 30 rows, 1024 x 1024: Small 15.5 us, Large 19.8).
+// A weight gradient has whole tiles whatever the groups are, as long as their groups: from two rounds on Large, where
+// the next tile starts under the stores and the rounds even out (32 groups of 65 rows, 1024 x 2048: 38.3 us, Small 45.5;
+// 64 of 16 rows: 70.8, 101.8), below Small, whose tiles find a free CU (16 groups of 40 to 3000 rows, 1024 x 1024: 50.7, Large
+// 64.2).
 template <int DT, int SC, bool ATR, bool BTR>
 int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
@@ -154,18 +159,17 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   const int cus = device_cu_count(s);
   // (a Large tile's stores are 32-bit offsets in it)
   const long long large = g.ldc * 2 * 256 < 0x7fffffffll ? tile_grid<Large>(g) : 0;
-  const bool large_fills = 5 * large >= 4 * cus;
   if constexpr (ATR) {
-    if (large_fills && g.red >= 128ll * g.experts) return launch_tile<Large, kTilePingPong>(g, s);
+    if (large >= 2 * cus) return launch_tile<Large, kTilePingPong>(g, s);
     return launch_tile<Small, kTileDma>(g, s);
   } else {
     using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 128, 4>;
     using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 128, 3>;
     const long long per_group = g.rows / g.experts, small = tile_grid<Small>(g);
-    if ((large_fills && per_group > 128) || (16 * large >= 5 * cus && per_group >= 512)) return launch_tile<Large, kTilePingPong>(g, s);
-    const bool near_two_rounds = 4 * small > 7 * cus;
-    if (4 * small <= cus || per_group <= (near_two_rounds ? 48 : 32)) return launch_tile<Low, kTileDma>(g, s);
-    if (near_two_rounds) return launch_tile<Small, kTileDma>(g, s);
+    if ((5 * large >= 4 * cus && per_group > 128) || (16 * large >= 5 * cus && per_group >= 512))
+      return launch_tile<Large, kTilePingPong>(g, s);
+    if (small > cus && per_group > 40 && (small <= 3 * cus || per_group > 128)) return launch_tile<Small, kTileDma>(g, s);
+    if (small > cus || 4 * small <= 3 * cus || per_group <= 64) return launch_tile<Low, kTileDma>(g, s);
     return launch_tile<Deep, kTileDma>(g, s);
   }
 }

@@ -320,13 +320,15 @@ struct TilePlan {
 // the accumulators a store would write 32 bytes of each of 16 rows). Accumulator [i][j] of a lane holds row
 // 16 (i WM + wm) + (lane & 15), columns 16 j + 4 (lane >> 4) + 0..3 of the wave's part: B is the matrix instruction's
 // first operand, so a lane's four values lie along a row. 16-byte chunk c of row r lies at c ^ (r & 15): neither side
-// conflicts. Rows that do not start on 16 bytes are stored by the same unaligned vector stores.
+// conflicts. Rows that start with a line of 128 bytes are streamed past the caches. Others share their lines with another
+// workgroup's: those go the ordinary way, so that the L2 writes whole lines (32 experts' 1032 x 2056 weight gradients, 65
+// rows each: 49 us, streamed 91).
 template <class C>
 __device__ __forceinline__ void tile_store_rows(const GroupArgs& g, char* lds, char* c_tile, int c_rows, int c_cols, int wm, int wn,
                                                 const gf4 (&acc)[C::NI][C::NJ]) {
   static_assert(C::BM * C::BN * 2 <= C::LDS, "the tile fits the ring");
   constexpr int OUT = C::DT == kFp16 ? kFp16 : kBf16;
-  const bool wide = (((uintptr_t)g.c | (uintptr_t)(g.ldc * 2) | (uintptr_t)(g.c_expert * 2)) & 15) == 0;
+  const bool lines = (((uintptr_t)g.c | (uintptr_t)(g.ldc * 2) | (uintptr_t)(g.c_expert * 2)) & 127) == 0;
   const int lane = threadIdx.x & 63, l16 = lane & 15, q = lane >> 4;
   bar();                                                 // every wave has read its last fragments
 #pragma unroll
@@ -349,7 +351,7 @@ __device__ __forceinline__ void tile_store_rows(const GroupArgs& g, char* lds, c
     const uint4 v = *(const uint4*)(lds + r * (C::BN * 2) + ((c ^ (r & 15)) << 4));
     unsigned short* at = (unsigned short*)c_tile + (size_t)r * g.ldc + c * 8;
     if (c * 8 + 8 <= c_cols) {
-      if (wide) store_c16(at, v);
+      if (lines) store_c16(at, v);
       else __builtin_memcpy(at, &v, 16);
     } else {
       const unsigned w[4] = {v.x, v.y, v.z, v.w};
@@ -839,7 +841,8 @@ __device__ __forceinline__ bool pp_store(const GroupArgs& g, char* stage, const 
                                          const gf4 (&acc)[C::NI][C::NJ]) {
   constexpr int OUT = C::DT == kFp16 ? kFp16 : kBf16;
   const int lane = lane_here(), l16 = lane & 15, q = lane >> 4;
-  const bool fast = ((((uintptr_t)g.c | (uintptr_t)(g.ldc * 2) | (uintptr_t)(g.c_expert * 2)) & 15) | (w.cols & 7)) == 0;
+  const size_t apart = (uintptr_t)g.c | (uintptr_t)(g.ldc * 2) | (uintptr_t)(g.c_expert * 2);
+  const bool fast = ((apart & 15) | (w.cols & 7)) == 0, lines = (apart & 127) == 0;
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(w.c, 0, 0x7fffffff, 0x00020000);
   const int r8 = lane >> 3, c8 = lane & 7, col = wn * C::TN + c8 * 8;
   static_assert(C::TN == 64, "a wave's rows are 128 bytes");
@@ -859,7 +862,8 @@ __device__ __forceinline__ bool pp_store(const GroupArgs& g, char* stage, const 
       const gi4 v = *(const gi4*)(stage + rl * 128 + ((c8 ^ (rl >> 1)) << 4));
       if (fast) {
         const unsigned at = r < w.rows && col < w.cols ? (unsigned)r * (unsigned)(g.ldc * 2) + (unsigned)col * 2 : kNowhere;
-        __builtin_amdgcn_raw_buffer_store_b128(v, rs, at, 0, 2);        // 2: streaming, as store_c16
+        if (lines) __builtin_amdgcn_raw_buffer_store_b128(v, rs, at, 0, 2);        // 2: streaming, as store_c16
+        else __builtin_amdgcn_raw_buffer_store_b128(v, rs, at, 0, 0);
       } else if (r < w.rows) {
         unsigned short* at = (unsigned short*)w.c + (size_t)r * g.ldc + col;
         if (col + 8 <= w.cols) {
@@ -893,7 +897,9 @@ __device__ __forceinline__ bool pp_next(const GroupArgs& g, TilePlan<C>& plan, i
   for (;; ++round) {
     const long long base = (long long)round * g.slots;
     if (base >= plan.items) return false;
-    const int place = (g.slots & 7) == 0 ? ((b >> 3) + 5 * round) % (g.slots >> 3) * 8 + (b & 7) : b;
+    int place = b;
+    if constexpr (C::ATR) place = (round & 1) != 0 ? g.slots - 1 - b : b;
+    else if ((g.slots & 7) == 0) place = ((b >> 3) + 5 * round) % (g.slots >> 3) * 8 + (b & 7);
     if (base + place < plan.items && plan.work(g, (int)base + place, w)) {
       ++round;
       return true;
