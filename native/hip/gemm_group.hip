@@ -129,7 +129,8 @@ int skinny_rows(const GroupArgs& g) {
 //            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1); from 5/16 of the CUs on where the groups are
 //            long, since a part of a tile is most of its width still (1280 x 4096 x 4096 fp8, 80 tiles as 240 parts:
 //            35.2 us, Deep 40.9; 2560 rows, 160 tiles: 52.1, 60.9; 64 tiles: 31.1, Low 27.2; 8 groups of 160 rows, 4096 x
-//            2048: 39.3, Deep 32.0)
+//            2048: 39.3, Deep 32.0). Not where a fifth or more of its columns would be empty (64 groups of 256 rows, 384
+//            x 384: 16.1, Small 11.3; 4 of 8192 rows, 128 x 4096 fp8: 64.5, 50.6)
 //   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: one round to about
 //            two of groups that fill most of it (16 groups of 128 rows, 2048 x 2048: 41.3 us, Low 47.5, Deep 44.9;
 //            700 x 8192 x 2048 fp8: 17.8, 23.3, 25.5; 32 groups of 94 rows, 880 tiles: 83.7, 70.6, 73.7)
@@ -141,12 +142,14 @@ int skinny_rows(const GroupArgs& g) {
 //
 // A weight gradient has whole tiles whatever the groups are, as long as their groups: from two rounds on Large, where
 // the next tile starts under the stores and the rounds even out (32 groups of 65 rows, 1024 x 2048: 38.3 us, Small 45.5;
-// 64 of 16 rows: 70.8, 101.8), below Small, whose tiles find a free CU (16 groups of 40 to 3000 rows, 1024 x 1024: 50.7, Large
-// 64.2).
+// 64 of 16 rows: 70.8, 101.8), unless a fifth of it would be empty (64 of 640 x 640: 53.6, 38.9); below Small, whose tiles
+// find a free CU (16 groups of 40 to 3000 rows, 1024 x 1024: 50.7, Large 64.2); below one round Deep (4 groups of 8192
+// rows, 1024 x 1024: 118, Small 169).
 template <int DT, int SC, bool ATR, bool BTR>
 int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
   using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
+  using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 128, 4>;
   const bool ready = dma_ready(g);
   if constexpr (!ATR && !BTR) {
     switch (skinny_rows(g)) {
@@ -159,14 +162,16 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   const int cus = device_cu_count(s);
   // (a Large tile's stores are 32-bit offsets in it)
   const long long large = g.ldc * 2 * 256 < 0x7fffffffll ? tile_grid<Large>(g) : 0;
+  const long long small = tile_grid<Small>(g);
   if constexpr (ATR) {
-    if (large >= 2 * cus) return launch_tile<Large, kTilePingPong>(g, s);
-    return launch_tile<Small, kTileDma>(g, s);
+    if (large >= 2 * cus && 16 * large < 5 * small) return launch_tile<Large, kTilePingPong>(g, s);
+    if (small > cus) return launch_tile<Small, kTileDma>(g, s);
+    return launch_tile<Deep, kTileDma>(g, s);
   } else {
-    using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 128, 4>;
     using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 128, 3>;
-    const long long per_group = g.rows / g.experts, small = tile_grid<Small>(g);
-    if ((5 * large >= 4 * cus && per_group > 128) || (16 * large >= 5 * cus && per_group >= 512))
+    const long long per_group = g.rows / g.experts;
+    const bool fills_columns = 10 * ((g.cols + 255ll) / 256) < 6 * ((g.cols + 127ll) / 128);
+    if (fills_columns && ((5 * large >= 4 * cus && per_group > 128) || (16 * large >= 5 * cus && per_group >= 512)))
       return launch_tile<Large, kTilePingPong>(g, s);
     if (small > cus && per_group > 40 && (small <= 3 * cus || per_group > 128)) return launch_tile<Small, kTileDma>(g, s);
     if (small > cus || 4 * small <= 3 * cus || per_group <= 64) return launch_tile<Low, kTileDma>(g, s);
