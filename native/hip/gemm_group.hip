@@ -126,11 +126,11 @@ int skinny_rows(const GroupArgs& g) {
 // The tile, by how many there are and how many rows a group has:
 //
 //   Large    256 x 256, ping-pong, one a CU: groups that fill it and a grid that nearly fills the CUs (16 groups of
-//            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1); from 5/16 of the CUs on where the groups are
-//            long, since a part of a tile is most of its width still (1280 x 4096 x 4096 fp8, 80 tiles as 240 parts:
-//            35.2 us, Deep 40.9; 2560 rows, 160 tiles: 52.1, 60.9; 64 tiles: 31.1, Low 27.2; 8 groups of 160 rows, 4096 x
-//            2048: 39.3, Deep 32.0). Not where a fifth or more of its columns would be empty (64 groups of 256 rows, 384
-//            x 384: 16.1, Small 11.3; 4 of 8192 rows, 128 x 4096 fp8: 64.5, 50.6)
+//            250 rows, 2048 x 1024: 248 tiles 27.0 us, 128 x 128 36.1); from 7/16 of the CUs on where the groups are
+//            long, since a part of a tile is most of its width still (1792 x 4096 x 4096 fp8, 112 tiles as 224 parts:
+//            37.3 us, Small 39.4; 2304 rows, 144 tiles: 51.3, 57.3; 1536 rows, 96 tiles: 36.0, 33.5). Not where a fifth or
+//            more of its columns would be empty (64 groups of 256 rows, 384 x 384: 16.1, Small 11.3; 4 of 8192 rows, 128
+//            x 4096 fp8: 64.5, 50.6)
 //   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: one round to about
 //            two of groups that fill most of it (16 groups of 128 rows, 2048 x 2048: 41.3 us, Low 47.5, Deep 44.9;
 //            700 x 8192 x 2048 fp8: 17.8, 23.3, 25.5; 32 groups of 94 rows, 880 tiles: 83.7, 70.6, 73.7)
@@ -171,7 +171,7 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
     using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 128, 3>;
     const long long per_group = g.rows / g.experts;
     const bool fills_columns = 10 * ((g.cols + 255ll) / 256) < 6 * ((g.cols + 127ll) / 128);
-    if (fills_columns && ((5 * large >= 4 * cus && per_group > 128) || (16 * large >= 5 * cus && per_group >= 512)))
+    if (fills_columns && ((5 * large >= 4 * cus && per_group > 128) || (16 * large >= 7 * cus && per_group >= 512)))
       return launch_tile<Large, kTilePingPong>(g, s);
     if (small > cus && per_group > 40 && (small <= 3 * cus || per_group > 128)) return launch_tile<Small, kTileDma>(g, s);
     if (small > cus || 4 * small <= 3 * cus || per_group <= 64) return launch_tile<Low, kTileDma>(g, s);

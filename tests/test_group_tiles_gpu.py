@@ -132,7 +132,7 @@ def test_fp8(cuda_device, m, n, k, scale_dtype):
 # cases for each smaller tile shape in each direction, for parts of the largest tiles on an idle card, and for many groups
 # of a few rows: (sizes, N, K)
 MIDDLE = [([64, 70, 0, 130] * 8, 1992, 256), ([64, 70, 0, 130] * 8, 256, 1992), ([8, 12, 0, 9] * 16, 640, 320),
-          ([1290], 4096, 200), ([700, 600], 200, 4100), ([1500, 1536], 1400, 264),
+          ([1800], 4096, 200), ([900, 850], 200, 4100), ([1500, 1536], 1400, 264),
           ([40, 30, 0, 50] * 8, 2048, 256), ([100] * 16, 2000, 320), ([300, 200, 10, 0], 1000, 1000), ([2000], 264, 520),
           ([20] * 60, 1288, 200), ([500, 490], 1792, 136)]
 
@@ -252,3 +252,17 @@ def test_two_streams_at_once(cuda_device):
     for w, rounds in zip(want, got):
         for r in rounds:
             assert all(torch.equal(p, q) for p, q in zip(r, w))
+
+
+def test_a_gradient_of_the_gradients_is_refused(cuda_device):
+    from gpu_operator_amd.ops import grouped as G
+
+    a = _rand(cuda_device, 70, torch.bfloat16, 20, 64).requires_grad_(True)
+    bt = _rand(cuda_device, 71, torch.bfloat16, 2, 32, 64).requires_grad_(True)
+    dc = _rand(cuda_device, 72, torch.bfloat16, 20, 32).requires_grad_(True)
+    off = H.offsets_of([7, 13], 0, cuda_device)
+    da, dbt = torch.autograd.grad(G.grouped_linear(a, bt, off), (a, bt), dc, create_graph=True)
+    assert torch.equal(da, G.gemm_grouped_dgrad(dc.detach(), bt.detach(), off))
+    assert torch.equal(dbt, G.gemm_grouped_wgrad(dc.detach(), a.detach(), off))
+    with pytest.raises(RuntimeError, match="twice"):
+        da.float().sum().backward()
