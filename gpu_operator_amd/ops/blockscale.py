@@ -63,7 +63,8 @@ def _result(out, name, shape, dtype, like):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=like.device)
     _matrix(out, name, len(shape), (dtype,), like.device)
-    _shape(tuple(out.shape) == shape and out.is_contiguous(), f"{name} must be contiguous {shape}, got {tuple(out.shape)}")
+    if out.shape != shape or not out.is_contiguous():
+        raise ValueError(f"{name} must be contiguous {shape}, got {tuple(out.shape)}")
     return out
 
 
@@ -73,8 +74,10 @@ def _scale(t, name, shape, dtypes, device) -> None:
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, "
                         f"got {getattr(t, 'dtype', type(t).__name__)}")
-    _shape(tuple(t.shape) == shape, f"{name} must be {shape}, got {tuple(t.shape)}")
-    _shape(t.device == device, f"{name} is on {t.device}, the operands on {device}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the operands on {device}")
 
 
 def _product(a, a_scale, bt, bt_scale, offsets, out):
@@ -87,7 +90,8 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
     sb = _matrix(bt, "bt", dims, f8, device)
     (m, k), shape_b = a.shape, tuple(bt.shape)
     n, e = shape_b[-2], shape_b[0] if dims == 3 else 1
-    _shape(shape_b[-1] == k, f"a is [{m},{k}], bt is {shape_b}: their last dimensions differ")
+    if shape_b[-1] != k:
+        raise ValueError(f"a is [{m},{k}], bt is {shape_b}: their last dimensions differ")
     _shape(e >= 1, "bt has no experts")
     _scale(a_scale, "a_scale", (m, _blocks(k)), (torch.float32, torch.float8_e8m0fnu), device)
     _scale(bt_scale, "bt_scale", (*shape_b[:-2], _blocks(n), _blocks(k)), (a_scale.dtype,), device)
