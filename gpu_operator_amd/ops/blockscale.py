@@ -16,7 +16,7 @@ two scales (a float32: scales whose product leaves float32's range are not suppo
 from __future__ import annotations
 
 from . import _lib
-from .grouped import MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, launch
+from .grouped import MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, _stride, launch
 
 BLOCK = 128
 
@@ -100,12 +100,12 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
     out, ldc, rest = _out(out, (m, n), torch.bfloat16, device)
     rest = 0 if offsets is None else rest
     if m and n:
-        ssa, ssb = a_scale.stride(), bt_scale.stride()
+        ssa, ssb, ha, hb = a_scale.stride(), bt_scale.stride(), a_scale.shape, bt_scale.shape
         launch(device, "amdgo_gemm_group(fp8)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
                a.data_ptr(), bt.data_ptr(), out.data_ptr(), a_scale.data_ptr(), bt_scale.data_ptr(),
                0 if offsets is None else offsets.data_ptr(),
-               _row_stride((m, k), sa), _row_stride((n, k), sb), ldc, sb[0] if dims == 3 else 0, 0,
-               ssa[0], ssa[1], ssb[0] if dims == 3 else 0, ssb[-2], ssb[-1],
+               _row_stride((m, k), sa), _row_stride((n, k), sb), ldc, sb[0] if e > 1 else 0, 0,
+               _stride(ha, ssa, 0), _stride(ha, ssa, 1), ssb[0] if e > 1 else 0, _stride(hb, ssb, -2), _stride(hb, ssb, -1),
                m, n, k, e, MODE_FORWARD, 2, 1 if a_scale.dtype == torch.float32 else 2, rest, 0)
     return out
 

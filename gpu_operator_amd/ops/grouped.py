@@ -49,6 +49,11 @@ def _row_stride(shape, strides) -> int:
     return strides[-2] if shape[-2] > 1 else shape[-1]
 
 
+def _stride(shape, strides, dim: int) -> int:
+    """The same of any dimension: 0 where there is no second one."""
+    return strides[dim] if shape[dim] > 1 else 0
+
+
 def _out(out, shape, dtype, device):
     """(tensor to write, its row stride, whether rows that no expert owns have to be cleared). The rows (and matrices)
     of an output may be apart, but not overlap."""
@@ -174,7 +179,7 @@ def gemm_grouped(a, bt, offsets, out=None):
     if t and n:
         launch(device, "amdgo_gemm_group", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
                a.data_ptr(), bt.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
-               _row_stride((t, k), sa), _row_stride((n, k), sb), ldc, sb[0], 0, 0, 0, 0, 0, 0,
+               _row_stride((t, k), sa), _row_stride((n, k), sb), ldc, _stride((e,), sb, 0), 0, 0, 0, 0, 0, 0,
                t, n, k, e, MODE_FORWARD, _dtype_code(dtype), 0, rest, 0)
     return out
 
@@ -193,7 +198,7 @@ def gemm_grouped_dgrad(dc, bt, offsets, out=None):
     if t and k:
         launch(device, "amdgo_gemm_group(dgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
                dc.data_ptr(), bt.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
-               _row_stride((t, n), sd), _row_stride((n, k), sb), ldc, sb[0], 0, 0, 0, 0, 0, 0,
+               _row_stride((t, n), sd), _row_stride((n, k), sb), ldc, _stride((e,), sb, 0), 0, 0, 0, 0, 0, 0,
                t, k, n, e, MODE_DGRAD, _dtype_code(dtype), 0, rest, 0)
     return out
 
@@ -216,7 +221,7 @@ def gemm_grouped_wgrad(dc, a, offsets, out=None):
     if n and k:
         launch(device, "amdgo_gemm_group(wgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
                dc.data_ptr(), a.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
-               _row_stride((t, n), sd), _row_stride((t, k), sa), ldc, 0, out.stride(0), 0, 0, 0, 0, 0,
+               _row_stride((t, n), sd), _row_stride((t, k), sa), ldc, 0, out.stride(0) if e > 1 else 0, 0, 0, 0, 0, 0,
                n, k, t, e, MODE_WGRAD, _dtype_code(dtype), 0, 0, 0)
     return out
 

@@ -266,3 +266,54 @@ def test_a_gradient_of_the_gradients_is_refused(cuda_device):
     assert torch.equal(dbt, G.gemm_grouped_wgrad(dc.detach(), a.detach(), off))
     with pytest.raises(RuntimeError, match="twice"):
         da.float().sum().backward()
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+def test_strides_of_single_rows_say_nothing(cuda_device, scale_dtype):
+    """A dimension of one may have any stride: the results are those of contiguous operands."""
+    from gpu_operator_amd.ops import blockscale as B
+    from gpu_operator_amd.ops import grouped as G
+
+    def odd(t, far):
+        return t.as_strided(t.shape, [far if n == 1 else st for n, st in zip(t.shape, t.stride())])
+
+    a, bt = _codes(cuda_device, 80, 1, 96), _codes(cuda_device, 81, 1, 48, 96)
+    sa, sb = _scales(cuda_device, 82, scale_dtype, 1, 1), _scales(cuda_device, 83, scale_dtype, 1, 1, 1)
+    off = torch.tensor([0, 1], dtype=torch.int32, device=cuda_device)
+    want = B.gemm_grouped_fp8_block(a, sa, bt, sb, off)
+    got = B.gemm_grouped_fp8_block(odd(a, 3), odd(sa, 1 << 40), odd(bt, 7), odd(sb, 1 << 40), off, odd(torch.empty_like(want), 5))
+    assert torch.equal(got, want)
+    assert torch.equal(B.gemm_fp8_block(odd(a, 3), odd(sa, 1 << 40), bt[0], odd(sb[0], 1 << 40)), want)
+    x, w = _rand(cuda_device, 84, torch.bfloat16, 1, 96), _rand(cuda_device, 85, torch.bfloat16, 1, 48, 96)
+    dc = _rand(cuda_device, 86, torch.bfloat16, 1, 48)
+    assert torch.equal(G.gemm_grouped(odd(x, 3), odd(w, 7), off), G.gemm_grouped(x, w, off))
+    assert torch.equal(G.gemm_grouped_dgrad(odd(dc, 1 << 40), odd(w, 7), off), G.gemm_grouped_dgrad(dc, w, off))
+    dw = G.gemm_grouped_wgrad(dc, x, off)
+    assert torch.equal(G.gemm_grouped_wgrad(odd(dc, 3), odd(x, 1 << 40), off, odd(torch.empty_like(dw), 1 << 40)), dw)
+
+
+@pytest.mark.parametrize("m", [5, 40, 200, 4000])
+def test_power_of_two_scales_at_their_ends(cuda_device, m):
+    """The least and the largest scale together, and NaN (code 255), in every kernel: NaN stays in its row or columns."""
+    from gpu_operator_amd.ops import blockscale as B
+
+    n, k = 4000 if m == 4000 else 272, 384
+    a, bt = _codes(cuda_device, 87, m, k), _codes(cuda_device, 88, n, k)
+    sa = torch.full((m, 3), 254, dtype=torch.uint8, device=cuda_device)          # 2^127
+    sb = torch.zeros((-(-n // 128), 3), dtype=torch.uint8, device=cuda_device)   # 2^-127
+    sa[1], sb[1] = 127 - 60, 127 + 60
+    sa[2] = 0                                                                    # rows times 2^-254, and of 2^-67
+    e8 = torch.float8_e8m0fnu
+    x64 = lambda q, s, rows: H.dequantize64(q, torch.exp2(s.double() - 127), rows)  # noqa: E731
+    x, w = x64(a, sa, 1), x64(bt, sb, 128)
+    keep = [r for r in range(m) if r != 3]
+    sa[3, 2] = 255
+    got = B.gemm_fp8_block(a, sa.view(e8), bt, sb.view(e8))
+    assert torch.isnan(got[3]).all()
+    ref, mag = x @ w.t(), x.abs() @ w.abs().t()
+    cols = slice(0, 128)                  # (the others' products of 2^127 and 2^60 leave the type's range)
+    slack = H.fp8_slack(H.raised64(a, torch.exp2(sa.double() - 127), 1), H.raised64(bt, torch.exp2(sb.double() - 127), 128))
+    H.check(got[keep][:, cols], ref[keep][:, cols], mag[keep][:, cols], k + 9, slack[keep][:, cols])
+    sb[0, 0] = 255
+    got = B.gemm_fp8_block(a, sa.view(e8), bt, sb.view(e8))
+    assert torch.isnan(got[:, :128]).all() and not torch.isnan(got[2, 128:]).any()
