@@ -141,15 +141,15 @@ int skinny_rows(const GroupArgs& g) {
 //            1024: 10.6, 13.1, 14.3; 32 fp8 groups of 32, 2048 x 2048: 26.1, 33.5, 28.7)
 //
 // A weight gradient has whole tiles whatever the groups are, as long as their groups: from two rounds on Large, where
-// the next tile starts under the stores and the rounds even out (32 groups of 65 rows, 1024 x 2048: 38.3 us, Small 45.5;
-// 64 of 16 rows: 70.8, 101.8), unless a fifth of it would be empty (64 of 640 x 640: 53.6, 38.9); below Small, whose tiles
+// the next tile starts under the stores and the rounds even out (32 groups of 65 rows, 1024 x 2048: 35.9 us, Small 44.3;
+// 64 of 16 rows: 57.1, 99.3), unless a fifth of it would be empty (64 of 640 x 640: 53.6, 38.9); below Small, whose tiles
 // find a free CU (16 groups of 40 to 3000 rows, 1024 x 1024: 50.7, Large 64.2); below one round Deep (4 groups of 8192
 // rows, 1024 x 1024: 118, Small 169).
 template <int DT, int SC, bool ATR, bool BTR>
 int dispatch_tile(const GroupArgs& g, hipStream_t s) {
-  using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 128, 2>;
-  using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 128, 2>;
-  using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 128, 4>;
+  using Large = TileCfg<DT, SC, ATR, BTR, 256, 256, 2, 4, 2>;
+  using Small = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 2, 2>;
+  using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 4>;
   const bool ready = dma_ready(g);
   if constexpr (!ATR && !BTR) {
     switch (skinny_rows(g)) {
@@ -168,7 +168,7 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
     if (small > cus) return launch_tile<Small, kTileDma>(g, s);
     return launch_tile<Deep, kTileDma>(g, s);
   } else {
-    using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 128, 3>;
+    using Low = TileCfg<DT, SC, ATR, BTR, 64, 128, 1, 4, 3>;
     const long long per_group = g.rows / g.experts;
     const bool fills_columns = 10 * ((g.cols + 255ll) / 256) < 6 * ((g.cols + 127ll) / 128);
     if (fills_columns && ((5 * large >= 4 * cus && per_group > 128) || (16 * large >= 7 * cus && per_group >= 512)))

@@ -144,22 +144,36 @@ struct RowTiles {
   }
 };
 
-// The expert with the `want`-th most rows (ties in order), up to 64 experts; above that the experts in order. A
-// weight gradient's tiles take as long as their expert has rows: started with the longest, the last ones to end are
-// short.
-__device__ __forceinline__ int group_by_size(const GroupArgs& g, int total, int want) {
-  if (g.offsets == nullptr || g.experts > 64) return want;
-  const int lane = threadIdx.x & 63;
-  int b = 0, x = -1;
-  if (lane < g.experts) group_rows(g.offsets, lane, total, b, x);
-  const int n = x - b;                               // -1 in lanes without an expert
-  int rank = 0;
-  for (int e = 0; e < g.experts; ++e) {
-    const int other = __builtin_amdgcn_readlane(n, e);
-    rank += other > n || (other == n && e < lane) ? 1 : 0;
+// The experts by their rows, most first (ties in order), up to 64 experts; above that in order. A weight gradient's tiles
+// take as long as their expert has rows: started with the longest, the last ones to end are short. A wave's lane has
+// expert (lane)'s rows and rank.
+struct GroupsBySize {
+  int begin, end, rank;
+
+  __device__ __forceinline__ GroupsBySize(const GroupArgs& g, int total) {
+    const int lane = threadIdx.x & 63;
+    begin = 0;
+    end = -1;
+    if (lane < g.experts) group_rows(g.offsets, lane, total, begin, end);
+    const int n = end - begin;                       // -1 in lanes without an expert
+    rank = 0;
+    for (int e = 0; e < g.experts; ++e) {
+      const int other = __builtin_amdgcn_readlane(n, e);
+      rank += other > n || (other == n && e < lane) ? 1 : 0;
+    }
   }
-  return __builtin_ctzll(__ballot(lane < g.experts && rank == want));
-}
+  static __device__ __forceinline__ bool sorted(const GroupArgs& g) { return g.offsets != nullptr && g.experts <= 64; }
+
+  // to LDS by rank (kWords words), and from there
+  static constexpr int kWords = 3 * 64;
+  __device__ __forceinline__ void save(const GroupArgs& g, int* at) const {
+    const int lane = threadIdx.x & 63;
+    if (lane >= g.experts) return;
+    at[rank] = lane;
+    at[64 + rank] = begin;
+    at[128 + rank] = end;
+  }
+};
 
 // Most row tiles that `experts` groups of `total` rows together can have: every busy expert adds at most one
 // that is not full. The host sizes the grid with it, since the offsets live on the device.

@@ -1,16 +1,15 @@
 // The tiled kernels of the grouped products: a BM x BN output tile per workgroup, WM x WN waves, operand panels
-// of PB bytes along the reduction (128: 64 elements of 16 bits, or 128 of fp8, one scale block) staged through
-// LDS.
+// of 128 bytes along the reduction (64 elements of 16 bits, or 128 of fp8, one scale block) staged through LDS.
 #pragma once
 
 #include "group_common.h"
 
-template <int DT_, int SC_, bool ATR_, bool BTR_, int BM_, int BN_, int WM_, int WN_, int PB_ = 128, int NBUF_ = 1>
+template <int DT_, int SC_, bool ATR_, bool BTR_, int BM_, int BN_, int WM_, int WN_, int NBUF_>
 struct TileCfg {
   static constexpr int DT = DT_, SC = SC_, BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr bool ATR = ATR_, BTR = BTR_;
   static constexpr int ES = DT == kFp8 ? 1 : 2;          // bytes an element
-  static constexpr int PB = PB_, NBUF = NBUF_;            // bytes a panel is wide; panels in the ring
+  static constexpr int PB = 128, NBUF = NBUF_;            // bytes a panel is wide; panels in the ring
   static constexpr int KT = PB / ES;                      // reduction steps a panel
   static constexpr int THREADS = 64 * WM * WN;
   // a wave's part: TN columns, and of the 16-row blocks every WM-th, so that all waves share what rows there are
@@ -27,15 +26,12 @@ struct TileCfg {
   static_assert((DT == kFp8) == (SC != kScaleNone), "fp8 has scales");
   static_assert(NBUF <= 4, "the ring's counted waits");
   static_assert(BN >= 128 && (!ATR || BM >= 128), "the chunk permutations reach over 256 bytes of a row");
-  static_assert(PB == 128 || (PB == 64 && DT != kFp8), "an fp8 panel is one scale block");
 };
 
-// Byte of 16-byte chunk q of row r in a K-major panel: rows of PB bytes, chunks permuted by the row so that
+// Byte of 16-byte chunk q of row r in a K-major panel: rows of 128 bytes, chunks permuted by the row so that
 // the fragment reads (16 rows, one chunk) spread over the banks.
-template <int PB>
-__device__ __forceinline__ int km_swizzle(int r) { return PB == 128 ? r & 7 : (r >> 1) & 3; }
-template <int PB>
-__device__ __forceinline__ int km_at(int r, int q) { return r * PB + ((q ^ km_swizzle<PB>(r)) << 4); }
+__device__ __forceinline__ int km_swizzle(int r) { return r & 7; }
+__device__ __forceinline__ int km_at(int r, int q) { return r * 128 + ((q ^ km_swizzle(r)) << 4); }
 
 // Byte of 16-byte chunk q of row r in a reduction-major panel of W columns (2 W bytes a row): 32-byte slots
 // permuted by the row. A transposing read takes 16 columns (one slot) of rows 8 g + 4 h + 0..3, so the rows
@@ -102,7 +98,7 @@ __device__ __forceinline__ gi4 tile_frag(lds_in base, int blk0, int blk, int s) 
     const gi2 l2 = __builtin_bit_cast(gi2, lo), h2 = __builtin_bit_cast(gi2, hi);
     return gi4{l2[0], l2[1], h2[0], h2[1]};
   } else {
-    return lds_chunk(base + blk0 * 16 * C::PB + km_at<C::PB>(j16, s * 4 + g) + blk * 16 * C::PB);
+    return lds_chunk(base + blk0 * 16 * C::PB + km_at(j16, s * 4 + g) + blk * 16 * C::PB);
   }
 }
 
@@ -135,8 +131,8 @@ __device__ __forceinline__ void tile_mul(const TileFrags<C>& f, gf4 (&acc)[C::NI
 template <class C>
 __device__ __forceinline__ gi8 tile_frag8(lds_in base, int blk0, int blk) {
   const int lane = threadIdx.x & 63, j16 = lane & 15, g = lane >> 4;
-  const gi4 x = lds_chunk(base + blk0 * 2048 + km_at<128>(j16, g) + blk * 2048);
-  const gi4 y = lds_chunk(base + blk0 * 2048 + km_at<128>(j16, g + 4) + blk * 2048);
+  const gi4 x = lds_chunk(base + blk0 * 2048 + km_at(j16, g) + blk * 2048);
+  const gi4 y = lds_chunk(base + blk0 * 2048 + km_at(j16, g + 4) + blk * 2048);
   return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -211,6 +207,7 @@ struct TileWork {
 template <class C>
 struct TilePlan {
   RowTiles rows;
+  const int* by_size = nullptr;                            // weight gradients: GroupsBySize in LDS, where they have been saved
   int tiles_m, tiles_n, whole, over, parts, items;
 
   TilePlan() = default;
@@ -229,9 +226,13 @@ struct TilePlan {
     }
   }
 
+  // Of one wave.
   static constexpr int kWords = RowTiles::kWords + 6;
-  __device__ __forceinline__ void save(int* at) const {
-    if constexpr (!C::ATR) {
+  static_assert(RowTiles::kWords >= GroupsBySize::kWords, "either in the same place");
+  __device__ __forceinline__ void save(const GroupArgs& g, int* at) const {
+    if constexpr (C::ATR) {
+      if (GroupsBySize::sorted(g)) GroupsBySize(g, g.red).save(g, at);
+    } else {
       if (rows.off != nullptr) rows.save(at);
     }
     at += RowTiles::kWords;
@@ -245,7 +246,8 @@ struct TilePlan {
     }
   }
   __device__ __forceinline__ void load(const GroupArgs& g, const int* at) {
-    if constexpr (!C::ATR) rows.load(g, g.rows, C::BM, at);
+    if constexpr (C::ATR) by_size = at;
+    else rows.load(g, g.rows, C::BM, at);
     at += RowTiles::kWords;
     tiles_m = __builtin_amdgcn_readfirstlane(at[0]);
     tiles_n = __builtin_amdgcn_readfirstlane(at[1]);
@@ -265,10 +267,21 @@ struct TilePlan {
     t.ldb_b = g.ldb * C::ES;
     if constexpr (C::ATR) {
       // an expert's tiles over all XCDs: whole experts to an XCD would leave those with the short ones idle
-      const int per = tiles_m * tiles_n, place = item / per, e = group_by_size(g, g.red, place);
-      int begin = 0, end = g.red;
+      const int per = tiles_m * tiles_n, place = item / per;
+      int e = place, begin = 0, end = g.red;
       tile_coords(xcd_remap(item - place * per, per), tiles_m, tiles_n, tm, tn);
-      if (g.offsets) group_rows(g.offsets, e, g.red, begin, end);
+      if (!GroupsBySize::sorted(g)) {
+        if (g.offsets) group_rows(g.offsets, e, g.red, begin, end);
+      } else if (by_size != nullptr) {
+        e = __builtin_amdgcn_readfirstlane(by_size[place]);
+        begin = __builtin_amdgcn_readfirstlane(by_size[64 + place]);
+        end = __builtin_amdgcn_readfirstlane(by_size[128 + place]);
+      } else {
+        const GroupsBySize groups(g, g.red);
+        e = __builtin_ctzll(__ballot((int)(threadIdx.x & 63) < g.experts && groups.rank == place));
+        begin = __builtin_amdgcn_readlane(groups.begin, e);
+        end = __builtin_amdgcn_readlane(groups.end, e);
+      }
       t.a = (const char*)g.a + (size_t)begin * g.lda * C::ES;
       t.b = (const char*)g.b + (size_t)begin * g.ldb * C::ES;
       t.a_col0 = tm * C::BM;
@@ -321,8 +334,8 @@ struct TilePlan {
 // 16 (i WM + wm) + (lane & 15), columns 16 j + 4 (lane >> 4) + 0..3 of the wave's part: B is the matrix instruction's
 // first operand, so a lane's four values lie along a row. 16-byte chunk c of row r lies at c ^ (r & 15): neither side
 // conflicts. Rows that start with a line of 128 bytes are streamed past the caches. Others share their lines with another
-// workgroup's: those go the ordinary way, so that the L2 writes whole lines (32 experts' 1032 x 2056 weight gradients, 65
-// rows each: 49 us, streamed 91).
+// workgroup's: those go the ordinary way, so that the L2 writes whole lines (32 experts' 1032 x 2056 weight gradients of 65
+// rows each take 1.8 times as long streamed).
 template <class C>
 __device__ __forceinline__ void tile_store_rows(const GroupArgs& g, char* lds, char* c_tile, int c_rows, int c_cols, int wm, int wn,
                                                 const gf4 (&acc)[C::NI][C::NJ]) {
@@ -387,7 +400,7 @@ struct PanelDma {
   __device__ __forceinline__ int chunk(int lane) const {
     const int q = lane % LANES;
     if constexpr (TR) return (((q >> 1) ^ rm_swizzle(row)) << 1) | (q & 1);
-    else return q ^ km_swizzle<C::PB>(row);
+    else return q ^ km_swizzle(row);
   }
   __device__ __forceinline__ void init(int wave, int lane, unsigned ld, int col0, int cols) {
     row = wave * (64 / LANES) + lane / LANES;
@@ -503,9 +516,13 @@ __device__ __forceinline__ void tile_loop(char* lds, TileLoader<C>& ld, int wm, 
   }
 }
 
-// The same tile with its panels in a ring of NBUF, NBUF - 1 of them in flight. At panel t a counted wait
+// A workgroup a tile, its panels in a ring of NBUF, NBUF - 1 of them in flight. At panel t a counted wait
 // retires t's pieces only, a bare s_barrier publishes them, and panel t + NBUF - 1 goes into the buffer that
 // every wave left at t - 1.
+//
+// Bound by what a CU's panels bring in from the L2, 40 to 50 KB a microsecond (a 128 x 128 tile reads 32 KB for 2 * 128^3
+// fp8 operations), or for few rows a group by the weights: fp8 128 x 4096 x 4096 13.5 us, 512 x 8192 x 8192 52.9 (1300
+// TFLOP/s); bf16 16 groups of 32 rows, 2048 x 4096, 56 us (4.8 TB/s of weights), of 128 rows, 2048 x 2048, 41.
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(C::EU, C::EU)))
 group_tile_dma(const GroupArgs g) {
@@ -558,7 +575,7 @@ struct PingPong {
   using DmaA = PanelDma<C, C::ATR, HM>;
   using DmaB = PanelDma<C, C::BTR, C::BN>;
   static constexpr int P1 = DmaA::PIECES + DmaB::PIECES + (C::SC != kScaleNone ? 1 : 0), P2 = DmaA::PIECES;
-  static_assert(C::WM == 2 && C::WN == 4 && C::NBUF == 2 && C::PB == 128, "two groups of four waves, two panels");
+  static_assert(C::WM == 2 && C::WN == 4 && C::NBUF == 2, "two groups of four waves, two panels");
 };
 
 // A value that is the same in all lanes, as the compiler should know: it stays in scalar registers.
@@ -890,7 +907,8 @@ __device__ __forceinline__ GroupArgs args_here() {
 
 // The workgroup's next item with work: workgroup b of `slots` takes one of every round of `slots` items. Inside a
 // round it keeps its XCD (b & 7) and moves on by 5 places, or the same workgroups would get all of the short tiles that
-// come every 8 items.
+// come every 8 items. A weight gradient's items come in order of their length: there every other round runs backwards (16
+// experts of 40 to 1500 rows, 2056 x 1032: 68.9 -> 65.0 us).
 template <class C>
 __device__ __forceinline__ bool pp_next(const GroupArgs& g, TilePlan<C>& plan, int& round, TileWork& w) {
   const int b = blockIdx.x;
@@ -909,8 +927,12 @@ __device__ __forceinline__ bool pp_next(const GroupArgs& g, TilePlan<C>& plan, i
 
 // One workgroup a CU, for all of the launch's tiles: the next tile's first panels are fetched before the result of the
 // last one is stored, so that the stores, and the wait for the first panels, run under each other and under the next
-// tile's loop (a workgroup a tile: 11 us a tile between the loops, 9.4 for fp8). What the tiles' starts and ends need
-// is kept in LDS and read there, not in registers across the loops.
+// tile's loop (a workgroup a tile: 11 us a tile between the loops, 9.4 for fp8; like this 6 and 8). What the tiles'
+// starts and ends need is kept in LDS and read there, not in registers across the loops.
+//
+// Bound by the matrix unit, which the card clocks down under it: 8192^3 fp8 444 to 500 us (2200 to 2480 TFLOP/s; each
+// further 4096 of K at 2620, e8m0 2970), bf16 of 8192 x 8192 x 4096 361 us (1520; 1630). With groups, by their last tiles: 8 of
+// 2048 rows on average, 8192 x 4096 bf16, 815 to 860 us (1350 to 1280), 26 fp8 ones of 590, 4096 x 4096, 315 to 330 (1640).
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) group_tile_pp(const GroupArgs args) {
   using P = PingPong<C>;
@@ -924,7 +946,7 @@ __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu
   {
     TilePlan<C> plan(args);
     more = pp_next<C>(args, plan, round, w);
-    if (wave == 0) plan.save(kept);
+    if (wave == 0) plan.save(args, kept);
   }
   __syncthreads();
   if (more) {

@@ -13,7 +13,8 @@
 // within that error of a border between two of them, and every border has 5 significant bits: those rare
 // values (the test below) are compared with the border exactly, in float64.
 //
-// Bound by the memory: 2 (4) bytes read and 1 written for each element.
+// Bound by the memory: 2 (4) bytes read and 1 written for each element. 16384 x 8192 bf16, a scale a row's block: 92 us (4.4
+// TB/s; a large copy 5.1); 12200 x 8256 fp32, 128 x 128 blocks: 95 us (5.3 TB/s).
 #include "gemm_tile_common.h"
 
 enum : int { kInBf16 = 0, kInFp16 = 1, kInFp32 = 2 };
