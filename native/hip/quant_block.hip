@@ -8,12 +8,15 @@
 // e4m3() rounds the exact quotient to the nearest value, ties to even; 448 is e4m3's largest, so nothing
 // saturates. An infinity or NaN becomes NaN (e4m3 has no infinity) and leaves its block's scale alone.
 //
-// The quotient with a float32 scale is formed from x and amax brought to amax's binade, by a reciprocal
-// with an error of a few units in the last place. That can only change the e4m3 value where the quotient is
-// within that error of a border between two of them, and every border has 5 significant bits: those rare
-// values (the test below) are compared with the border exactly, in float64.
+// The quotient with a float32 scale is x times 448 / amax nearly, within 4 units in the last place. That can only change
+// the e4m3 value where the exact quotient is a border between two of them, or that close to one. A border has 5
+// significant bits, B. Of 16-bit inputs x = X 2^i and amax = A 2^j have at most 11: 448 x / amax is the border B 2^k where 7 X
+// and B A agree but for a power of two, both integers under 2^16; so it is a border, or at least 2^-16 of it away. There the
+// quotient rounded to 20 bits decides right: it moves by 2^-20 at most, and onto the border where that is
+// exact (many are: half of all blocks hold an x of 3/4 or 3/8 amax). Of float32 inputs the rare values within 8 units of
+// a border are compared with it exactly, in float64.
 //
-// Bound by the memory: 2 (4) bytes read and 1 written for each element. 16384 x 8192 bf16, a scale a row's block: 92 us (4.4
+// Bound by the memory: 2 (4) bytes read and 1 written for each element. 16384 x 8192 bf16, a scale a row's block: 70 us (5.7
 // TB/s; a large copy 5.1); 12200 x 8256 fp32, 128 x 128 blocks: 95 us (5.3 TB/s).
 #include "gemm_tile_common.h"
 
@@ -31,6 +34,7 @@ struct QuantArgs {
 namespace {
 
 typedef unsigned int qu2 __attribute__((ext_vector_type(2)));
+typedef unsigned short qs2 __attribute__((ext_vector_type(2)));
 
 constexpr int QT = 256;                // threads
 
@@ -80,7 +84,8 @@ constexpr unsigned int kLeastAmax = ((unsigned)(127 - 118) << 23) | 0x600000u;  
 struct Scale {
   float f;            // float32: the scale; e8m0: 2^e
   int e;              // float32: amax's exponent; e8m0: e
-  float d, r;         // float32: amax * 2^-e in [1, 2) and 448 / d nearly
+  float d;            // float32: amax * 2^-e in [1, 2)
+  float m;            // float32: 448 / amax nearly; e8m0: 2^-e (a power of two more or less rounds nothing: -118 <= e <= 127)
 };
 
 template <bool E8>
@@ -90,28 +95,34 @@ __device__ __forceinline__ Scale make_scale(unsigned int amax) {
   if constexpr (E8) {
     s.e = (int)(amax >> 23) - 127 - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
     s.f = __builtin_bit_cast(float, (unsigned)(s.e + 127) << 23);
-    s.d = s.r = 0.f;
+    s.d = 0.f;
+    s.m = __builtin_bit_cast(float, (unsigned)(127 - s.e) << 23);
   } else {
-    s.f = __builtin_bit_cast(float, amax) / 448.0f;
+    // amax / 448, rounded once: a quotient by 7 with an error under one unit, one correction by its exact remainder
+    // (amax / 64 and the results are normal numbers)
+    const float a7 = __builtin_bit_cast(float, amax) * 0x1p-6f, q7 = a7 * (1.0f / 7.0f);
+    s.f = fmaf(fmaf(-7.0f, q7, a7), 1.0f / 7.0f, q7);
     s.e = (int)(amax >> 23) - 127;
     s.d = __builtin_bit_cast(float, (amax & 0x7fffffu) | 0x3f800000u);
-    s.r = 448.0f * __builtin_amdgcn_rcpf(s.d);
+    s.m = ldexpf(448.0f * __builtin_amdgcn_rcpf(s.d), -s.e);
   }
   return s;
 }
 
-template <bool E8>
+// Less than kNearBorder where a quotient's last 19 bits are within 8 of zeros, as a border's are.
+constexpr unsigned int kNearBorder = 16u << 13;
+__device__ __forceinline__ unsigned int border_bits(float y) { return (__builtin_bit_cast(unsigned int, y) + 8) << 13; }
+
+// Any value's quotient: what quantize8 leaves to it.
+template <int DT, bool E8>
 __device__ __forceinline__ float quotient(float x, const Scale& s) {
-  const float xs = ldexpf(x, -s.e);           // exact wherever the result does not round to zero
-  float y;
-  if constexpr (E8) {
-    y = xs;
-  } else {
-    y = xs * s.r;                              // within 4 units in the last place of 448 x / amax
-    const unsigned int b = __builtin_bit_cast(unsigned int, y);
-    if (((b + 8) & 0x7ffffu) < 16) {           // maybe a border: compare with it exactly
-      const unsigned int tb = (b + 8) & ~0x7ffffu;
-      const double t = (double)__builtin_bit_cast(float, tb) * (double)s.d, n = 448.0 * (double)xs;
+  float y = x * s.m;                             // float32 scales: within 4 units in the last place of 448 x / amax
+  if constexpr (!E8 && DT != kInFp32) {
+    y = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned int, y) + 8) & ~15u);
+  } else if constexpr (!E8) {
+    if (border_bits(y) < kNearBorder && fabsf(y) >= 0x1p-11f) {   // (under that all are 0) compare with it exactly
+      const unsigned int tb = (__builtin_bit_cast(unsigned int, y) + 8) & ~0x7ffffu;
+      const double t = (double)__builtin_bit_cast(float, tb) * (double)s.d, n = 448.0 * (double)ldexpf(x, -s.e);
       const double at = fabs(t), an = fabs(n);
       y = __builtin_bit_cast(float, tb + (an > at ? 1u : an < at ? 0xffffffffu : 0u));
     }
@@ -119,11 +130,22 @@ __device__ __forceinline__ float quotient(float x, const Scale& s) {
   return finite_bits(x) == 0 && x != 0.f ? __builtin_nanf("") : y;
 }
 
+// The vector unit is close to the memory's pace here, so a value takes one multiplication, what its type needs at a border,
+// and its share of a test for all 8: whether one is not finite (or, of float32, may be a border).
 template <int DT, bool E8>
-__device__ __forceinline__ qu2 quantize8(const Raw8<DT>& r, const Scale& s) {
+__device__ __forceinline__ qu2 quantize8(const Raw8<DT>& r, bool finite, const Scale& s) {
   float y[8];
+  unsigned int near = 0xffffffffu;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = quotient<E8>(raw_get<DT>(r, i), s);
+  for (int i = 0; i < 8; ++i) {
+    y[i] = raw_get<DT>(r, i) * s.m;
+    if constexpr (!E8 && DT == kInFp32) near = min(near, border_bits(y[i]));
+    else if constexpr (!E8) y[i] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned int, y[i]) + 8) & ~15u);
+  }
+  if (near < kNearBorder || !finite) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = quotient<DT, E8>(raw_get<DT>(r, i), s);
+  }
   qu2 o;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -150,34 +172,57 @@ __device__ __forceinline__ void store_scale(void* s, size_t at, const Scale& v) 
   else ((float*)s)[at] = v.f;
 }
 
+// The largest finite magnitude of 8, as a float's bits; whether all are finite. (16-bit magnitudes are ordered as their
+// bits are: two to an instruction.)
 template <int DT>
-__device__ __forceinline__ unsigned int amax8(const Raw8<DT>& r) {
+__device__ __forceinline__ unsigned int amax8(const Raw8<DT>& r, bool& finite) {
   unsigned int m = 0;
+  if constexpr (DT == kInFp32) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, finite_bits(raw_get<DT>(r, i)));
+    for (int i = 0; i < 8; ++i) m = max(m, r.w[i] & 0x7fffffffu);
+    finite = m < 0x7f800000u;
+  } else {
+    qs2 h = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h = __builtin_elementwise_max(h, __builtin_bit_cast(qs2, r.w[i] & 0x7fff7fffu));
+    const unsigned int top = max(h[0], h[1]);
+    finite = top < (DT == kInBf16 ? 0x7f80u : 0x7c00u);
+    m = DT == kInBf16 ? top << 16 : __builtin_bit_cast(unsigned int, (float)__builtin_bit_cast(_Float16, (unsigned short)top));
+  }
+  if (!finite) {
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, finite_bits(raw_get<DT>(r, i)));
+  }
   return m;
 }
 
-// One row's block a quarter wave: 16 lanes of 8 elements; a wave takes 4 blocks of one row.
-template <int DT, bool E8>
+// One row's block a quarter wave: 16 lanes of 8 elements; a wave takes 4 U blocks of one row, all loads first.
+template <int DT, bool E8, int U>
 __global__ void __launch_bounds__(QT) quantize_row_blocks(const QuantArgs a) {
   constexpr int ES = DT == kInFp32 ? 4 : 2;
-  const int lane = threadIdx.x & 63, kb_count = (a.cols + 127) / 128, per_row = (kb_count + 3) / 4;
-  const long long id = (long long)blockIdx.x * (QT / 64) + (threadIdx.x >> 6);
-  const long long row = id / per_row;
-  if (row >= (long long)a.batches * a.rows) return;
-  const int kb = (int)(id - row * per_row) * 4 + (lane >> 4);
-  const int batch = (int)(row / a.rows), r = (int)(row - (long long)batch * a.rows);
+  const int lane = threadIdx.x & 63, kb_count = (a.cols + 127) / 128, per_row = (kb_count + 4 * U - 1) / (4 * U);
+  const unsigned id = blockIdx.x * (QT / 64) + (unsigned)__builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned row = id / (unsigned)per_row;
+  if (row >= (unsigned)a.batches * (unsigned)a.rows) return;
+  const int kb0 = (int)(id - row * per_row) * 4 * U + (lane >> 4);
+  const unsigned batch = a.batches == 1 ? 0 : row / (unsigned)a.rows, r = row - batch * (unsigned)a.rows;
   const char* x = (const char*)a.x + ((size_t)batch * a.batch_stride + (size_t)r * a.ld) * ES;
-  const int c = kb * 128 + (lane & 15) * 8;
-  const Raw8<DT> v = raw_load<DT>(x, c, a.cols);
-  unsigned int m = amax8<DT>(v);
+  Raw8<DT> v[U];
 #pragma unroll
-  for (int d = 1; d < 16; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
-  if (kb >= kb_count) return;
-  const Scale s = make_scale<E8>(m);
-  store8(a.q + (size_t)row * a.cols, c, a.cols, quantize8<DT, E8>(v, s));
-  if ((lane & 15) == 0) store_scale<E8>(a.s, (size_t)row * kb_count + kb, s);
+  for (int u = 0; u < U; ++u) v[u] = raw_load<DT>(x, (kb0 + 4 * u) * 128 + (lane & 15) * 8, a.cols);
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int kb = kb0 + 4 * u;
+    bool finite;
+    unsigned int m = amax8<DT>(v[u], finite);
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
+    if (kb >= kb_count) continue;
+    const Scale s = make_scale<E8>(m);
+    store8(a.q + (size_t)row * a.cols, kb * 128 + (lane & 15) * 8, a.cols, quantize8<DT, E8>(v[u], finite, s));
+    if ((lane & 15) == 0) store_scale<E8>(a.s, (size_t)row * kb_count + kb, s);
+  }
 }
 
 // A block of 128 rows a workgroup: thread t holds chunk t & 15 of rows t / 16 + 16 i.
@@ -191,6 +236,7 @@ __global__ void __launch_bounds__(QT) quantize_square_blocks(const QuantArgs a) 
   const char* x = (const char*)a.x + (size_t)batch * a.batch_stride * ES;
   const int c = kb * 128 + (threadIdx.x & 15) * 8, r0 = rb * 128 + (threadIdx.x >> 4);
   Raw8<DT> v[8];
+  bool finite[8];
   unsigned int m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -198,7 +244,7 @@ __global__ void __launch_bounds__(QT) quantize_square_blocks(const QuantArgs a) 
     v[i] = raw_load<DT>(x + (size_t)(r < a.rows ? r : 0) * a.ld * ES, c, r < a.rows ? a.cols : 0);
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, amax8<DT>(v[i]));
+  for (int i = 0; i < 8; ++i) m = max(m, amax8<DT>(v[i], finite[i]));
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) m = max(m, (unsigned)__shfl_xor((int)m, d));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
@@ -208,19 +254,31 @@ __global__ void __launch_bounds__(QT) quantize_square_blocks(const QuantArgs a) 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int r = r0 + 16 * i;
-    if (r < a.rows) store8(a.q + ((size_t)batch * a.rows + r) * a.cols, c, a.cols, quantize8<DT, E8>(v[i], s));
+    if (r < a.rows) store8(a.q + ((size_t)batch * a.rows + r) * a.cols, c, a.cols, quantize8<DT, E8>(v[i], finite[i], s));
   }
   if (threadIdx.x == 0) store_scale<E8>(a.s, blockIdx.x, s);
 }
 
+template <int DT, bool E8, int U>
+int launch_rows(const QuantArgs& a, hipStream_t s) {
+  const long long kb = ((long long)a.cols + 127) / 128, waves = (long long)a.batches * a.rows * ((kb + 4 * U - 1) / (4 * U));
+  if (waves > 0xffffffffll - QT / 64) return (int)hipErrorInvalidValue;      // (their numbers are 32 bits)
+  hipLaunchKernelGGL((quantize_row_blocks<DT, E8, U>), dim3((unsigned)((waves + QT / 64 - 1) / (QT / 64))), dim3(QT), 0, s, a);
+  return (int)hipGetLastError();
+}
+
+// Two chunks a lane of 16-bit rows that fill the card with waves twice over, one else (16384 x 8192 bf16: 69.9 us, one chunk
+// 86.5; 300 rows: 5.1, 4.6; 16384 x 2048 fp32: 32.5, 31.4).
 template <int DT, bool E8>
 int launch_quant(const QuantArgs& a, hipStream_t s) {
   const long long kb = ((long long)a.cols + 127) / 128;
-  const long long grid = a.block_rows == 1 ? ((long long)a.batches * a.rows * ((kb + 3) / 4) + QT / 64 - 1) / (QT / 64)
-                                           : a.batches * (((long long)a.rows + 127) / 128) * kb;
+  if (a.block_rows == 1) {
+    if (DT != kInFp32 && (long long)a.batches * a.rows * ((kb + 3) / 4) > 16384) return launch_rows<DT, E8, DT == kInFp32 ? 1 : 2>(a, s);
+    return launch_rows<DT, E8, 1>(a, s);
+  }
+  const long long grid = a.batches * (((long long)a.rows + 127) / 128) * kb;
   if (grid > 0x7fffffff) return (int)hipErrorInvalidValue;
-  if (a.block_rows == 1) hipLaunchKernelGGL((quantize_row_blocks<DT, E8>), dim3((unsigned)grid), dim3(QT), 0, s, a);
-  else hipLaunchKernelGGL((quantize_square_blocks<DT, E8>), dim3((unsigned)grid), dim3(QT), 0, s, a);
+  hipLaunchKernelGGL((quantize_square_blocks<DT, E8>), dim3((unsigned)grid), dim3(QT), 0, s, a);
   return (int)hipGetLastError();
 }
 

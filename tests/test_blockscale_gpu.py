@@ -235,3 +235,38 @@ def test_serving_path(cuda_device, scale_dtype):
         w64 = H.dequantize64(q2, s2, 128)
         ref, mag = H.forward64(y64, w64, off)
         H.check(out, ref, mag, f + 9, H.grouped_fp8_slack(H.raised64(vy, sv, 1), H.raised64(q2, s2, 128), off))
+
+
+@pytest.mark.parametrize("scale_dtype", SCALES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(6000, 1544), (20000, 513), (5000, 2056)])
+def test_quantize_many_rows(cuda_device, rows, cols, dtype, scale_dtype):
+    """Enough rows for two chunks a lane; zeros among them, and a row with an infinity and a NaN."""
+    g = torch.Generator(device=cuda_device).manual_seed(cols)
+    x = torch.randn((rows, cols), generator=g, device=cuda_device)
+    x = torch.where(torch.rand((rows, cols), generator=g, device=cuda_device) < 0.1, torch.zeros_like(x), x)
+    x[7, 3], x[7, 500] = float("inf"), float("nan")
+    _check_quantized(x.to(dtype), 1, scale_dtype)
+
+
+def test_scales_are_rounded_quotients_of_any_amax(cuda_device):
+    """amax over all of float32's range, and every e4m3 value of a block: the scale is amax / 448 rounded once."""
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    bits = torch.randint(0, 0x7F800000, (40000, 1), generator=g, device=cuda_device, dtype=torch.int32)
+    amax = bits.view(torch.float32)
+    x = amax * (torch.randint(-448, 449, (40000, 128), generator=g, device=cuda_device) / 448)
+    x[:, :1] = amax
+    _check_quantized(x, 1, torch.float32)
+    _check_quantized(x, 1, torch.float8_e8m0fnu)
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 7), (torch.float16, 10)])
+def test_every_ratio_of_16_bit_values(cuda_device, dtype, bits):
+    """Every pair of significands x, amax, 17 binades apart at most: all of their ties and neighbours of ties."""
+    n = 1 << bits
+    m = (torch.arange(n, 2 * n, device=cuda_device, dtype=torch.float64) / n)
+    for shift in range(17):
+        x = torch.minimum((m * 2.0 ** -shift).view(1, -1, 64), m.view(-1, 1, 1)).reshape(-1, 64)
+        top = m.view(-1, 1).expand(-1, n // 64).reshape(-1, 1)
+        block = torch.cat([x, top, -x[:, :63]], dim=1)
+        _check_quantized(block.to(dtype), 1, torch.float32)
