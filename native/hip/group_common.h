@@ -49,6 +49,23 @@ typedef _Float16 gh8 __attribute__((ext_vector_type(8)));
 typedef short gs4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) gs4* gs4_lds;
 
+// 16 bytes from any address. Vector loads that do not start on 4 bytes take several times as long, so whole words are loaded,
+// the last of which holds the 16th byte (none without a byte that is wanted), and moved down.
+struct Any16 {
+  gi4 w;
+  int last;
+};
+
+__device__ __forceinline__ void any16_load(Any16& x, const char* p) {
+  __builtin_memcpy(&x.w, __builtin_assume_aligned((const void*)((uintptr_t)p & ~(uintptr_t)3), 4), 16);
+  x.last = *(const int*)((uintptr_t)(p + 15) & ~(uintptr_t)3);
+}
+
+__device__ __forceinline__ gi4 any16_get(const Any16& x, unsigned shift) {            // shift: the address' last two bits
+  return gi4{(int)__builtin_amdgcn_alignbyte(x.w[1], x.w[0], shift), (int)__builtin_amdgcn_alignbyte(x.w[2], x.w[1], shift),
+             (int)__builtin_amdgcn_alignbyte(x.w[3], x.w[2], shift), (int)__builtin_amdgcn_alignbyte(x.last, x.w[3], shift)};
+}
+
 // The rows [begin, end) of expert e. The offsets live on the device and are not checked by the host, so
 // they are clamped here: whatever they hold, no row outside the operands is touched.
 __device__ __forceinline__ void group_rows(const int* __restrict__ off, int e, int total, int& begin, int& end) {

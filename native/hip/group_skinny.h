@@ -13,9 +13,9 @@
 
 #include "group_tile.h"
 
-template <int DT_, int SC_, int MT_, int NJ_, int KW_, int U_, bool ALIGNED_ = true>
+template <int DT_, int SC_, int MT_, int NJ_, int KW_, int U_, int ALIGN_ = 16>
 struct SkinnyCfg {
-  static constexpr bool ALIGNED = ALIGNED_;      // whole, aligned 16-byte chunks (else they are loaded piece by piece)
+  static constexpr int ALIGN = ALIGN_;           // 16: rows of whole, aligned 16-byte chunks; 4, 1: rows that start on so many bytes
   static constexpr int DT = DT_, SC = SC_, MT = MT_, NJ = NJ_, KW = KW_, U = U_;
   static constexpr int ES = DT == kFp8 ? 1 : 2;
   static constexpr int ROWS = 16 * MT, COLS = 16 * NJ, THREADS = 64 * KW;
@@ -29,6 +29,74 @@ struct SkinnyPanel {
   gi4 a[C::MT][2], b[C::NJ][2];
   int sa[C::MT], sb;
 };
+
+// The same of rows that start anywhere: the words that hold the chunks (`moved`: not yet moved down).
+template <class C>
+struct SkinnyWords {
+  Any16 a[C::MT][2], b[C::NJ][2];
+  int sa[C::MT], sb;
+  bool moved;
+};
+
+template <class C>
+__device__ __forceinline__ void skinny_panel(const SkinnyWords<C>& w, const unsigned (&shift_a)[C::MT], const unsigned (&shift_b)[C::NJ],
+                                             SkinnyPanel<C>& p) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int m = 0; m < C::MT; ++m) p.a[m][h] = any16_get(w.a[m][h], w.moved ? shift_a[m] : 0);
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) p.b[j][h] = any16_get(w.b[j][h], w.moved ? shift_b[j] : 0);
+  }
+#pragma unroll
+  for (int m = 0; m < C::MT; ++m) p.sa[m] = w.sa[m];
+  p.sb = w.sb;
+}
+
+// Panel k of rows without whole aligned chunks.
+template <class C>
+__device__ __forceinline__ void skinny_load(SkinnyPanel<C>& p, const char* const (&pa)[C::MT], const char* const (&pb)[C::NJ], int k,
+                                            int q0, int red) {
+  const unsigned at = (unsigned)k * 128u;
+  const bool whole = at + 128u <= (unsigned)red * C::ES;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const unsigned from = at + (unsigned)(q0 + 4 * h) * 16u;
+    if (whole) {
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) __builtin_memcpy(&p.a[m][h], pa[m] + from, 16);
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) __builtin_memcpy(&p.b[j][h], pb[j] + from, 16);
+    } else {                                           // the last panel, or none
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) p.a[m][h] = load_chunk<C::ES>(pa[m], (int)(from / C::ES), red);
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) p.b[j][h] = load_chunk<C::ES>(pb[j], (int)(from / C::ES), red);
+    }
+  }
+}
+
+template <class C>
+__device__ __forceinline__ void skinny_load(SkinnyWords<C>& p, const char* const (&pa)[C::MT], const char* const (&pb)[C::NJ], int k,
+                                            int q0, int red) {
+  const unsigned at = (unsigned)k * 128u;
+  p.moved = at + 128u <= (unsigned)red * C::ES;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const unsigned from = at + (unsigned)(q0 + 4 * h) * 16u;
+    if (p.moved) {
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) any16_load(p.a[m][h], pa[m] + from);
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) any16_load(p.b[j][h], pb[j] + from);
+    } else {                                           // the last panel, or none
+#pragma unroll
+      for (int m = 0; m < C::MT; ++m) p.a[m][h] = Any16{load_chunk<C::ES>(pa[m], (int)(from / C::ES), red), 0};
+#pragma unroll
+      for (int j = 0; j < C::NJ; ++j) p.b[j][h] = Any16{load_chunk<C::ES>(pb[j], (int)(from / C::ES), red), 0};
+    }
+  }
+}
 
 __device__ __forceinline__ gi4 buffer_chunk(__amdgpu_buffer_rsrc_t rs, unsigned off) {
   return __builtin_bit_cast(gi4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
@@ -74,6 +142,11 @@ __device__ __forceinline__ void skinny_mul(const SkinnyPanel<C>& p, gf4 (&acc)[C
   }
 }
 
+template <class C, int ALIGN>
+struct SkinnyLoaded { using T = SkinnyPanel<C>; };
+template <class C>
+struct SkinnyLoaded<C, 1> { using T = SkinnyWords<C>; };
+
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) group_skinny(const GroupArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[C::LDS];
@@ -111,28 +184,37 @@ __global__ void __launch_bounds__(C::THREADS) group_skinny(const GroupArgs g) {
   const unsigned bytes = (unsigned)g.red * C::ES;
   const unsigned as_k = (unsigned)(g.as_k * S), bs_k = (unsigned)(g.bs_k * S);
   const int nk = (g.red + 128 / C::ES - 1) / (128 / C::ES);
+  // Operands without whole aligned chunks: a lane's rows and columns by their address, the last existing one in place of one
+  // that does not exist (it multiplies into results that are not stored).
+  const char *pa[C::MT], *pb[C::NJ];
+  unsigned shift_a[C::MT], shift_b[C::NJ];
+  if constexpr (C::ALIGN < 16) {
+#pragma unroll
+    for (int m = 0; m < C::MT; ++m) {
+      pa[m] = (const char*)g.a + (size_t)(rt.row0 + min(m * 16 + l16, rows - 1)) * g.lda * C::ES;
+      shift_a[m] = (unsigned)(uintptr_t)pa[m] & 3;
+    }
+#pragma unroll
+    for (int j = 0; j < C::NJ; ++j) {
+      pb[j] = (const char*)g.b + ((size_t)rt.expert * g.b_expert + (size_t)(n0 + min(j * 16 + l16, cols - 1)) * g.ldb) * C::ES;
+      shift_b[j] = (unsigned)(uintptr_t)pb[j] & 3;
+    }
+  }
   // panel k: `at` is added to offsets that may already be past the end; they stay there (both under 2^31)
-  const char* const pa = (const char*)g.a + (size_t)rt.row0 * g.lda * C::ES;
-  const char* const pb = (const char*)g.b + ((size_t)rt.expert * g.b_expert + (size_t)n0 * g.ldb) * C::ES;
-  const auto load = [&](SkinnyPanel<C>& p, int k) {
+  using Loaded = typename SkinnyLoaded<C, C::ALIGN>::T;
+  const auto load = [&](Loaded& p, int k) {
     const unsigned at = (unsigned)k * 128u;
+    if constexpr (C::ALIGN < 16) {
+      skinny_load<C>(p, pa, pb, k, q0, g.red);
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const bool in = at + (unsigned)(q0 + 4 * h) * 16u < bytes;
-      if constexpr (!C::ALIGNED) {
-        const int from = (int)(at / C::ES) + (q0 + 4 * h) * (16 / C::ES);
+      for (int h = 0; h < 2; ++h) {
+        const bool in = at + (unsigned)(q0 + 4 * h) * 16u < bytes;
 #pragma unroll
-        for (int m = 0; m < C::MT; ++m)
-          p.a[m][h] = load_chunk<C::ES>(pa + (size_t)(m * 16 + l16) * g.lda * C::ES, from, m * 16 + l16 < rows ? g.red : 0);
+        for (int m = 0; m < C::MT; ++m) p.a[m][h] = buffer_chunk(ra, in ? oa[m] + at + h * 64u : kNowhere);
 #pragma unroll
-        for (int j = 0; j < C::NJ; ++j)
-          p.b[j][h] = load_chunk<C::ES>(pb + (size_t)(j * 16 + l16) * g.ldb * C::ES, from, j * 16 + l16 < cols ? g.red : 0);
-        continue;
+        for (int j = 0; j < C::NJ; ++j) p.b[j][h] = buffer_chunk(rb, in ? ob[j] + at + h * 64u : kNowhere);
       }
-#pragma unroll
-      for (int m = 0; m < C::MT; ++m) p.a[m][h] = buffer_chunk(ra, in ? oa[m] + at + h * 64u : kNowhere);
-#pragma unroll
-      for (int j = 0; j < C::NJ; ++j) p.b[j][h] = buffer_chunk(rb, in ? ob[j] + at + h * 64u : kNowhere);
     }
     if constexpr (C::SC != kScaleNone) {
 #pragma unroll
@@ -145,14 +227,22 @@ __global__ void __launch_bounds__(C::THREADS) group_skinny(const GroupArgs g) {
   for (int m = 0; m < C::MT; ++m)
 #pragma unroll
     for (int j = 0; j < C::NJ; ++j) acc[m][j] = gf4{0.f, 0.f, 0.f, 0.f};
-  SkinnyPanel<C> cur[C::U], nxt[C::U];
+  Loaded cur[C::U], nxt[C::U];
 #pragma unroll
   for (int u = 0; u < C::U; ++u) load(cur[u], wave + u * C::KW);
   for (int k = wave; k < nk; k += C::U * C::KW) {
 #pragma unroll
     for (int u = 0; u < C::U; ++u) load(nxt[u], k + (C::U + u) * C::KW);
 #pragma unroll
-    for (int u = 0; u < C::U; ++u) skinny_mul<C>(cur[u], acc);
+    for (int u = 0; u < C::U; ++u) {
+      if constexpr (C::ALIGN > 1) {
+        skinny_mul<C>(cur[u], acc);
+      } else {
+        SkinnyPanel<C> p;
+        skinny_panel<C>(cur[u], shift_a, shift_b, p);
+        skinny_mul<C>(p, acc);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < C::U; ++u) cur[u] = nxt[u];
   }

@@ -49,7 +49,11 @@ __device__ __forceinline__ gi4 load_chunk(const char* row, int from, int upto) {
   gi4 v = {0, 0, 0, 0};
   if (from + N <= upto) {
     __builtin_memcpy(&v, row + (size_t)from * ES, 16);
-  } else {
+  } else if (from < upto && upto >= N) {                  // the row's last 16 bytes, moved down: one load
+    unsigned __int128 last;
+    __builtin_memcpy(&last, row + (size_t)(upto - N) * ES, 16);
+    v = __builtin_bit_cast(gi4, last >> ((from + N - upto) * (8 * ES)));
+  } else if (from < upto) {
     union { unsigned char b[16]; unsigned short h[8]; gi4 v; } u;
     u.v = v;
 #pragma unroll

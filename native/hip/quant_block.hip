@@ -63,12 +63,19 @@ __device__ __forceinline__ Raw8<DT> raw_load(const char* row, int c, int cols) {
   } else {
 #pragma unroll
     for (int i = 0; i < Raw8<DT>::W; ++i) r.w[i] = 0;
+    if (ES == 2 && c < cols && cols >= 8) {             // the row's last 16 bytes, moved down: one load
+      unsigned __int128 last;
+      __builtin_memcpy(&last, row + (size_t)(cols - 8) * ES, 16);
+      last >>= (c + 8 - cols) * 16;
+      __builtin_memcpy(r.w, &last, 16);
+    } else if (c < cols) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < cols) {
-        if constexpr (ES == 4) r.w[i] = ((const unsigned int*)row)[c + i];
-        else r.w[i >> 1] |= (unsigned int)((const unsigned short*)row)[c + i] << ((i & 1) * 16);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (c + i < cols) {
+          if constexpr (ES == 4) r.w[i] = ((const unsigned int*)row)[c + i];
+          else r.w[i >> 1] |= (unsigned int)((const unsigned short*)row)[c + i] << ((i & 1) * 16);
+        }
+    }
   }
   return r;
 }
