@@ -118,12 +118,14 @@ int skinny_unaligned(const GroupArgs& g, hipStream_t s) {
 
 // Few rows: the skinny kernel with tiles of 16 rows, or of 32 for a single group of 17 to 64 (8192 x 8192 fp8, 32 rows:
 // 16-row tiles 30 us, 32-row ones 22.5; 64 rows of 4096 x 4096: 15.6, 12.2). Groups of more than 12 rows on average
-// are for the tiled kernel (16 of 16 rows, 4096 x 2048: 65.5 us, Low 60.4; 64 of 8 rows: 93.8, Small 110.5). 0: not here.
-int skinny_rows(const GroupArgs& g) {
+// are for the tiled kernel (16 of 16 rows, 4096 x 2048: 65.5 us, Low 60.4; 64 of 8 rows: 93.8, Small 110.5); of more than
+// 20 where the operands are not `ready`, since that one needs a copy of the weights then (16 of 15 rows, 2048 x 1537 bf16:
+// 42.9, 59.1; of 25: 58.4, 59.5; fp8 29.8, 33.6 and 40.0, 34.4). 0: not here.
+int skinny_rows(const GroupArgs& g, bool ready) {
   if (g.mode != kModeForward) return 0;
   if (g.offsets == nullptr) return g.rows <= 16 ? 1 : g.rows <= 64 ? 2 : 0;
   const long long busy = g.experts < g.rows ? g.experts : g.rows;
-  return g.rows <= 12 * busy ? 1 : 0;
+  return g.rows <= (ready ? 12 : 20) * busy ? 1 : 0;
 }
 
 // The tile, by how many there are and how many rows a group has:
@@ -155,7 +157,7 @@ int dispatch_tile(const GroupArgs& g, hipStream_t s) {
   using Deep = TileCfg<DT, SC, ATR, BTR, 128, 128, 2, 4, 4>;
   const bool ready = dma_ready(g);
   if constexpr (!ATR && !BTR) {
-    switch (skinny_rows(g)) {
+    switch (skinny_rows(g, ready)) {
       case 1: return ready ? skinny_columns<DT, SC, 1>(g, s) : skinny_unaligned<DT, SC, 1>(g, s);
       case 2:                                        // (a product without groups is an fp8 one)
         if constexpr (DT == kFp8) return ready ? skinny_columns<DT, SC, 2>(g, s) : skinny_unaligned<DT, SC, 2>(g, s);

@@ -191,7 +191,7 @@ def test_unaligned_operands_at_every_size(cuda_device):
     H.check(B.gemm_fp8_block(a, sa, bt, sb), x @ w.t(), x.abs() @ w.abs().t(), 301 + 9, H.fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128)))
 
 
-@pytest.mark.parametrize("sizes,n,k", [([3000, 0, 4000, 1], 1801, 515), ([70, 0, 33], 135, 77), ([2, 0, 1], 135, 77)])
+@pytest.mark.parametrize("sizes,n,k", [([3000, 0, 4000, 1], 1801, 515), ([70, 0, 33], 135, 77), ([2, 0, 1], 135, 77), ([17, 0, 30], 70, 6)])
 def test_unaligned_operands_in_a_graph(cuda_device, sizes, n, k):
     """The workspace that unaligned operands are laid out in belongs to the graph: replays over new inputs, with eager
     calls of the same operators between them, give the eager results."""
@@ -317,3 +317,39 @@ def test_power_of_two_scales_at_their_ends(cuda_device, m):
     sb[0, 0] = 255
     got = B.gemm_fp8_block(a, sa.view(e8), bt, sb.view(e8))
     assert torch.isnan(got[:, :128]).all() and not torch.isnan(got[2, 128:]).any()
+
+
+@pytest.mark.parametrize("sizes,n,k", [([17, 0, 33, 5], 300, 259), ([16] * 5, 77, 1030), ([3, 40], 33, 7), ([1, 1, 0, 9], 130, 641),
+                                       ([20, 20], 64, 15), ([2], 100, 64)])
+def test_few_rows_from_any_address(cuda_device, sizes, n, k):
+    """Rows that start on each byte of a word (fp8), on 2 and 4 bytes (16 bits), with widths that end inside a piece: the bits
+    of aligned copies; nothing behind the operands is read into the results."""
+    from gpu_operator_amd.ops import blockscale as B
+    from gpu_operator_amd.ops import grouped as G
+
+    t, e, kb = sum(sizes), len(sizes), -(-k // 128)
+    off = H.offsets_of(sizes, 0, cuda_device)
+
+    def at(x, lead, pad):
+        flat = torch.full((lead + x[..., 0].numel() * (x.shape[-1] + pad) + 64,), 0x7F, dtype=torch.uint8, device=x.device)
+        if x.dtype != torch.float8_e4m3fn:
+            flat = torch.full((flat.numel(),), float("nan"), dtype=x.dtype, device=x.device)
+        v = flat[lead : lead + x[..., 0].numel() * (x.shape[-1] + pad)].view(*x.shape[:-1], -1)[..., : x.shape[-1]]
+        v.copy_(x.view(torch.uint8) if x.dtype == torch.float8_e4m3fn else x)
+        return v.view(x.dtype)
+
+    a, bt = _codes(cuda_device, 90, t, k), _codes(cuda_device, 91, e, n, k)
+    sa, sb = _scales(cuda_device, 92, torch.float32, t, kb), _scales(cuda_device, 93, torch.float32, e, -(-n // 128), kb)
+    x, w = H.dequantize64(a, sa, 1), H.dequantize64(bt, sb, 128)
+    ref, mag = H.forward64(x, w, off)
+    slack = H.grouped_fp8_slack(H.raised64(a, sa, 1), H.raised64(bt, sb, 128), off)
+    for lead, pad in ((0, 0), (1, 0), (2, 1), (3, 2), (0, 3), (5, 7)):
+        got = B.gemm_grouped_fp8_block(at(a, lead, pad), sa, at(bt, lead + 1, pad), sb, off)
+        H.check(got, ref, mag, k + 3 * kb, slack)
+        if len(sizes) == 1:
+            assert torch.equal(B.gemm_fp8_block(at(a, lead, pad), sa, at(bt, lead, pad)[0], sb[0]), got)
+    for dtype in (torch.bfloat16, torch.float16):
+        x, w = _rand(cuda_device, 94, dtype, t, k), _rand(cuda_device, 95, dtype, e, n, k, scale=k ** -0.5)
+        ref, mag = H.forward64(x, w, off)
+        for lead, pad in ((0, 0), (1, 0), (2, 2), (0, 1), (3, 5)):
+            H.check(G.gemm_grouped(at(x, lead, pad), at(w, lead + 1, pad), off), ref, mag, k)
