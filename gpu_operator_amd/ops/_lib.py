@@ -103,12 +103,11 @@ def load() -> ctypes.CDLL:
 
 # The argument structs of native/hip/group_common.h (GroupArgs) and quant_block.hip (QuantArgs), packed in one call:
 # building a ctypes.Structure field by field costs more than the launch.
-GROUP_FIELDS = ("a", "b", "c", "a_scale", "b_scale", "offsets",
-                "lda", "ldb", "ldc", "b_expert", "c_expert", "as_row", "as_k", "bs_expert", "bs_row", "bs_k",
-                "rows", "cols", "red", "experts", "mode", "dtype", "scale", "zero_rest", "padded")
+# GroupArgs: a, b, c, a_scale, b_scale, offsets; lda, ldb, ldc, b_expert, c_expert, as_row, as_k, bs_expert, bs_row, bs_k;
+# rows, cols, red, experts, mode, dtype, scale, zero_rest, padded
 pack_group = struct.Struct("=6Q10q9i").pack
 NEEDS_PACKING = -1           # amdgo_gemm_group's answer where it cannot read the operands in place
-QUANT_FIELDS = ("x", "q", "s", "ld", "batch_stride", "batches", "rows", "cols", "dtype", "block_rows", "e8")
+# QuantArgs: x, q, s; ld, batch_stride; batches, rows, cols, dtype, block_rows, e8
 pack_quant = struct.Struct("=3Q2q6i").pack
 
 
@@ -132,9 +131,10 @@ def load_group() -> ctypes.CDLL:
             lib = ctypes.CDLL(str(p))
             lib.amdgo_gemm_group.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
             lib.amdgo_gemm_group.restype = ctypes.c_int
-            vp, i, ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-            lib.amdgo_group_pack.argtypes = [vp, vp, ll, ll, i, i, ll, i, ll, vp]
-            lib.amdgo_group_pack.restype = i
+            lib.amdgo_group_workspace.argtypes = [ctypes.c_char_p]
+            lib.amdgo_group_workspace.restype = ctypes.c_longlong
+            lib.amdgo_gemm_group_packed.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p]
+            lib.amdgo_gemm_group_packed.restype = ctypes.c_int
             lib.amdgo_quantize_fp8_block.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
             lib.amdgo_quantize_fp8_block.restype = ctypes.c_int
             _GROUP_LIB = lib

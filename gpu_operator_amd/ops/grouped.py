@@ -107,47 +107,21 @@ def launch(device, what: str, entry, pack, *fields) -> None:
             err = entry(args, stream)
     if err:
         if err == _lib.NEEDS_PACKING:
-            return _launch_packed(device, what, fields)
+            return _launch_packed(device, what, args, stream)
         _lib.check(err, what)
 
 
-def _launch_packed(device, what: str, fields) -> None:
-    """The product on copies of what the kernels cannot read in place: rows on 16 bytes, the reduction filled up with
-    zeros to whole 16-byte pieces (in both operands, so that they add nothing)."""
+def _launch_packed(device, what: str, args: bytes, stream: int) -> None:
+    """The product on copies, in a workspace of the call, of what the kernels cannot read in place."""
     import torch
 
-    f = dict(zip(_lib.GROUP_FIELDS, fields))
-    lib, size = _lib.load_group(), 1 if f["dtype"] == 2 else 2
-    unit = 16 // size
-    rows, cols, red, experts = f["rows"], f["cols"], f["red"], f["experts"]
-    full = -(-red // unit) * unit
-    # an operand's rows and row length, now and as wanted, for each mode
-    a_now, b_now = {MODE_FORWARD: ((rows, red), (cols, red)), MODE_DGRAD: ((rows, red), (red, cols)),
-                    MODE_WGRAD: ((red, rows), (red, cols))}[f["mode"]]
-    b_rows = full if f["mode"] == MODE_DGRAD else b_now[0]
-    kept = []
-
-    def pack(at, ld, batch, batches, now, to_rows):
-        length = -(-now[1] // unit) * unit
-        fits = not (f[at] | f[ld] * size | batch * size | now[1] * size) & 15 and to_rows == now[0] \
-            and f[ld] * size * 256 + (max(rows, cols) + red) * size < 2 ** 31 - 1
-        if fits:
-            return batch
-        space = torch.empty(max(1, batches * to_rows * length * size), dtype=torch.uint8, device=device)
-        kept.append(space)
-        _lib.check(lib.amdgo_group_pack(f[at], space.data_ptr(), f[ld] * size, batch * size, batches, now[0],
-                                        now[1] * size, to_rows, length * size,
-                                        torch.cuda.current_stream(device).cuda_stream), what)
-        f[at], f[ld] = space.data_ptr(), length
-        return to_rows * length
-
+    lib = _lib.load_group()
+    need = lib.amdgo_group_workspace(args)
+    if need < 0:
+        raise ValueError(f"{what}: operands too large to be laid out anew")
     with torch.cuda.device(device):
-        pack("a", "lda", 0, 1, a_now, a_now[0])
-        f["b_expert"] = pack("b", "ldb", f["b_expert"], experts if f["mode"] != MODE_WGRAD else 1, b_now, b_rows)
-        if f["mode"] != MODE_WGRAD:
-            f["red"] = full
-        f["padded"] = 1
-        err = lib.amdgo_gemm_group(_lib.pack_group(*f.values()), torch.cuda.current_stream(device).cuda_stream)
+        space = torch.empty(need, dtype=torch.uint8, device=device)
+        err = lib.amdgo_gemm_group_packed(args, space.data_ptr(), stream)
     if err == _lib.NEEDS_PACKING:
         raise ValueError(f"{what}: the scales' strides reach over 2 GiB")
     _lib.check(err, what)

@@ -35,7 +35,7 @@ int launch_tile(const GroupArgs& g, hipStream_t s) {
 }
 
 // What amdgo_gemm_group answers, having launched nothing, where the operands have to be laid out first
-// (amdgo_group_pack): see dma_ready.
+// (amdgo_gemm_group_packed): see dma_ready.
 constexpr int kNeedsPacking = -1;
 
 // Whether a tile's lane offsets fit a buffer's 2 GiB.
@@ -59,30 +59,72 @@ bool dma_ready(const GroupArgs& g) {
   return whole(g.a, g.lda, 0, a_tr, g.rows) && whole(g.b, g.ldb, g.b_expert, b_tr, g.cols) && offsets_fit(g);
 }
 
-// A matrix [batches, rows, row_bytes] of any strides to [batches, to_rows, to_bytes] (to_bytes a multiple of 16), zeros
-// where the source has nothing. A workgroup takes whole rows, 16 bytes a lane.
-__global__ void __launch_bounds__(256) pack_rows(const char* __restrict__ from, char* __restrict__ to, long long ld_b,
-                                                 long long batch_b, int rows, long long row_bytes, int to_rows, long long to_bytes) {
-  const int batch = blockIdx.x / to_rows, r = blockIdx.x - batch * to_rows;
-  const char* src = from + (size_t)batch * batch_b + (size_t)r * ld_b;
-  char* dst = to + (size_t)blockIdx.x * to_bytes;
-  for (long long at = threadIdx.x * 16ll; at < to_bytes; at += 256 * 16) {
+// A matrix [batches, rows, row_bytes] of any strides to [batches, to_rows, to_bytes] (to_bytes a multiple of 16, rows to_ld
+// apart), zeros where the source has nothing.
+struct PackMatrix {
+  const char* from;
+  char* to;
+  long long ld, batch, to_ld, row_bytes, to_bytes;
+  int batches, rows, to_rows;
+
+  __host__ __device__ long long blocks() const { return (long long)batches * to_rows; }
+};
+
+// Both operands in one launch: a workgroup takes whole rows, 16 bytes a lane.
+__global__ void __launch_bounds__(256) pack_rows(const PackMatrix a, const PackMatrix b) {
+  const unsigned in_a = (unsigned)a.blocks(), block = blockIdx.x < in_a ? blockIdx.x : blockIdx.x - in_a;
+  const PackMatrix m = blockIdx.x < in_a ? a : b;
+  const int batch = block / (unsigned)m.to_rows, r = block - batch * (unsigned)m.to_rows;
+  const char* src = m.from + (size_t)batch * m.batch + (size_t)r * m.ld;
+  char* dst = m.to + (size_t)block * m.to_ld;
+  for (long long at = threadIdx.x * 16ll; at < m.to_bytes; at += 256 * 16) {
     uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < rows) {
-      if (at + 16 <= row_bytes) {
-        __builtin_memcpy(&v, src + at, 16);
-      } else {
-        union { unsigned char b[16]; uint4 v; } u;
-        u.v = v;
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          if (at + i < row_bytes) u.b[i] = (unsigned char)src[at + i];
-        v = u.v;
-      }
-    }
+    if (r < m.rows) v = __builtin_bit_cast(uint4, load_chunk<1>(src, (int)at, (int)m.row_bytes));
     *(uint4*)(dst + at) = v;
   }
 }
+
+// What has to be laid out for a product whose operands are not dma_ready, and the product on it. A reduction along the rows is
+// filled up with zeros to whole 16-byte pieces, in both operands, so that they add nothing; the rows start on lines.
+struct PackPlan {
+  PackMatrix a, b;
+  GroupArgs g;
+  long long bytes;
+
+  explicit PackPlan(const GroupArgs& from) : a{}, b{}, g(from), bytes(0) {
+    const long long es = g.dtype == kFp8 ? 1 : 2, unit = 16 / es, full = (g.red + unit - 1) / unit * unit;
+    const bool a_tr = g.mode == kModeWgrad, b_tr = g.mode != kModeForward;
+    const auto lay = [&](PackMatrix& m, const void*& p, long long& ld, long long* batch, int batches, long long rows, long long width,
+                         long long to_rows) {
+      const long long to = (width + unit - 1) / unit * unit, pitch = (to * es + 127) / 128 * 128;
+      const long long strides = (long long)(uintptr_t)p | ld * es | (batch ? *batch * es : 0) | width * es;
+      const long long across = ((long long)(g.rows > g.cols ? g.rows : g.cols) + g.red) * es;
+      if ((strides & 15) == 0 && to_rows == rows && ld * es * 256 + across < 0x7fffffffll) return;
+      m = PackMatrix{(const char*)p, nullptr, ld * es, batch ? *batch * es : 0, pitch, width * es, to * es, batches, (int)rows, (int)to_rows};
+      m.to = (char*)(uintptr_t)bytes;                     // its place in the workspace
+      bytes += batches * to_rows * pitch;
+      ld = pitch / es;
+      if (batch) *batch = to_rows * ld;
+    };
+    lay(a, g.a, g.lda, nullptr, 1, a_tr ? g.red : g.rows, a_tr ? g.rows : g.red, a_tr ? g.red : g.rows);
+    const long long b_rows = b_tr ? g.red : g.cols;
+    lay(b, g.b, g.ldb, g.mode == kModeWgrad ? nullptr : &g.b_expert, g.mode == kModeWgrad ? 1 : g.experts, b_rows, b_tr ? g.cols : g.red,
+        g.mode == kModeDgrad ? full : b_rows);
+    if (g.mode != kModeWgrad) g.red = (int)full;
+    g.padded = 1;
+  }
+  bool fits() const {
+    return g.red >= 0 && a.blocks() + b.blocks() <= 0x7fffffffll && a.to_ld * 256 < 0x7fffffffll && b.to_ld * 256 < 0x7fffffffll;
+  }
+  int launch(char* space, hipStream_t s) {
+    for (PackMatrix* m : {&a, &b}) m->to = space + (uintptr_t)m->to;
+    if (a.blocks()) g.a = a.to;
+    if (b.blocks()) g.b = b.to;
+    if (bytes == 0) return 0;
+    hipLaunchKernelGGL(pack_rows, dim3((unsigned)(a.blocks() + b.blocks())), dim3(256), 0, s, a, b);
+    return (int)hipGetLastError();
+  }
+};
 
 template <class C>
 int launch_skinny(const GroupArgs& g, long long tiles_m, hipStream_t s) {
@@ -196,37 +238,53 @@ int dispatch16(const GroupArgs& g, hipStream_t s) {
 
 }  // namespace
 
+namespace {
+
+// The arguments as the caller packs them, up to `slots`.
+GroupArgs group_args(const void* args) {
+  GroupArgs g = {};
+  __builtin_memcpy(&g, args, offsetof(GroupArgs, slots));
+  if (g.offsets == nullptr || g.mode == kModeWgrad) g.zero_rest = 0;
+  return g;
+}
+
+bool valid(const GroupArgs& g) {
+  if (g.rows < 0 || g.cols < 0 || g.red < 0 || g.experts < 1) return false;
+  if (g.dtype == kFp8) return g.mode == kModeForward && (g.scale == kScaleF32 || g.scale == kScaleE8);
+  return (g.dtype == kBf16 || g.dtype == kFp16) && g.scale == kScaleNone && g.mode >= kModeForward && g.mode <= kModeWgrad;
+}
+
+int dispatch(const GroupArgs& g, hipStream_t s) {
+  if (g.rows == 0 || g.cols == 0) return 0;
+  if (g.dtype == kFp8) return g.scale == kScaleF32 ? dispatch_tile<kFp8, kScaleF32, false, false>(g, s)
+                                                   : dispatch_tile<kFp8, kScaleE8, false, false>(g, s);
+  return g.dtype == kBf16 ? dispatch16<kBf16>(g, s) : dispatch16<kFp16>(g, s);
+}
+
+}  // namespace
+
 extern "C" {
 
 int amdgo_gemm_group(const void* args, hipStream_t s) {
   if (!args) return (int)hipErrorInvalidValue;
-  GroupArgs g = {};
-  __builtin_memcpy(&g, args, offsetof(GroupArgs, slots));       // packed by the caller up to there
-  if (g.rows < 0 || g.cols < 0 || g.red < 0 || g.experts < 1) return (int)hipErrorInvalidValue;
-  if (g.rows == 0 || g.cols == 0) return 0;
-  if (g.offsets == nullptr || g.mode == kModeWgrad) g.zero_rest = 0;
-  if (g.dtype == kFp8) {
-    if (g.mode != kModeForward) return (int)hipErrorInvalidValue;
-    if (g.scale == kScaleF32) return dispatch_tile<kFp8, kScaleF32, false, false>(g, s);
-    if (g.scale == kScaleE8) return dispatch_tile<kFp8, kScaleE8, false, false>(g, s);
-    return (int)hipErrorInvalidValue;
-  }
-  if (g.scale != kScaleNone) return (int)hipErrorInvalidValue;
-  if (g.dtype == kBf16) return dispatch16<kBf16>(g, s);
-  if (g.dtype == kFp16) return dispatch16<kFp16>(g, s);
-  return (int)hipErrorInvalidValue;
+  const GroupArgs g = group_args(args);
+  return valid(g) ? dispatch(g, s) : (int)hipErrorInvalidValue;
 }
 
-// `to`: batches * to_rows rows of to_bytes, 16-byte aligned.
-int amdgo_group_pack(const void* from, void* to, long long ld_b, long long batch_b, int batches, int rows, long long row_bytes,
-                     int to_rows, long long to_bytes, hipStream_t s) {
-  const long long grid = (long long)batches * to_rows;
-  if (grid < 0 || grid > 0x7fffffff || to_rows < rows || to_bytes < row_bytes || (to_bytes & 15) || ((uintptr_t)to & 15))
-    return (int)hipErrorInvalidValue;
-  if (grid == 0 || to_bytes == 0) return 0;
-  hipLaunchKernelGGL(pack_rows, dim3((unsigned)grid), dim3(256), 0, s, (const char*)from, (char*)to, ld_b, batch_b, rows, row_bytes,
-                     to_rows, to_bytes);
-  return (int)hipGetLastError();
+// Bytes of the workspace that amdgo_gemm_group_packed needs; negative: an argument is invalid.
+long long amdgo_group_workspace(const void* args) {
+  if (!args || !valid(group_args(args))) return -1;
+  const PackPlan plan(group_args(args));
+  return plan.fits() ? plan.bytes : -1;
+}
+
+// `space`: 16-byte aligned, of that many bytes.
+int amdgo_gemm_group_packed(const void* args, void* space, hipStream_t s) {
+  if (!args || !valid(group_args(args)) || ((uintptr_t)space & 15)) return (int)hipErrorInvalidValue;
+  PackPlan plan(group_args(args));
+  if (!plan.fits() || (plan.bytes && !space)) return (int)hipErrorInvalidValue;
+  const int err = plan.launch((char*)space, s);
+  return err ? err : dispatch(plan.g, s);
 }
 
 }  // extern "C"

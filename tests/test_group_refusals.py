@@ -114,3 +114,29 @@ def test_block_product_refusals(fake):
     ]:
         with pytest.raises(exc):
             B.gemm_grouped_fp8_block(*args)
+
+
+def test_workspace_of_unaligned_operands():
+    """Bytes of the copies: rows of whole lines, of what does not lie on 16 bytes alone; refusals of sizes and kinds."""
+    from gpu_operator_amd.ops import _lib
+
+    if not _lib.group_lib_path().exists():
+        pytest.skip("the library is not built")
+    lib = _lib.load_group()
+
+    def need(mode, rows, cols, red, experts, lda, ldb, b_expert, dtype=0, scale=0, a=1 << 20, b=1 << 21):
+        return lib.amdgo_group_workspace(_lib.pack_group(a, b, 1 << 22, 0, 0, 1 << 23, lda, ldb, cols, b_expert, 0, 0, 0, 0, 0, 0,
+                                                         rows, cols, red, experts, mode, dtype, scale, 0, 0))
+
+    assert need(0, 10, 20, 64, 3, 64, 64, 20 * 64) == 0
+    assert need(0, 10, 20, 64, 3, 65, 64, 20 * 64) == 10 * 128                      # a's rows alone
+    assert need(0, 10, 20, 64, 3, 64, 64, 20 * 64, b=(1 << 21) + 2) == 3 * 20 * 128
+    assert need(0, 10, 20, 65, 3, 72, 72, 20 * 72) == (10 + 3 * 20) * 256           # the reduction's end: both
+    assert need(1, 10, 64, 20, 3, 24, 64, 20 * 64) == 10 * 128 + 3 * 24 * 128       # zero rows behind each of bt's
+    assert need(2, 33, 64, 500, 3, 33, 64, 0) == 500 * 128
+    assert need(0, 10, 20, 130, 3, 130, 130, 20 * 130, dtype=2, scale=1) == (10 + 3 * 20) * 256
+    assert need(0, 10, 20, 64, 0, 64, 64, 0) < 0 and need(3, 10, 20, 64, 3, 64, 64, 0) < 0
+    assert need(0, 10, 20, 64, 3, 64, 64, 0, dtype=2) < 0 and need(0, 10, 20, 64, 3, 64, 64, 0, scale=1) < 0
+    assert need(0, -1, 20, 64, 3, 64, 64, 0) < 0
+    assert need(0, 10, 20, 2 ** 31 - 1, 3, 2 ** 31 - 1, 2 ** 31 - 1, 0) < 0         # rows too long for a copy
+    assert need(0, 2 ** 31 - 1, 2 ** 31 - 1, 63, 2 ** 20, 63, 63, 63) < 0           # too many of them
