@@ -137,13 +137,18 @@ int launch_skinny(const GroupArgs& g, long long tiles_m, hipStream_t s) {
 // MT 16-row tiles a workgroup. 64 columns and 4 waves where that leaves more than two workgroups a CU, else
 // narrower columns and the reduction over more waves (8192 x 8192 fp8, 16 rows: 128 workgroups of 64 columns
 // 23.0 us, 256 of 32 with 8 waves 17.5; 1024 x 2048 bf16 over 4 experts: 32 columns 7.5, 16 columns 6.5; 64 experts of
-// 4096 x 2048 fp8: 64 columns and 4 waves 54.3, 32 and 8 58.0; the weights at a copy's rate: 13.3, 2.2, 58.0).
+// 4096 x 2048 fp8: 64 columns and 4 waves 54.3, 32 and 8 58.0; the weights at a copy's rate: 13.3, 2.2, 58.0). 16-bit
+// weights of a few rows each are narrower still, down to 16 columns from 4096 of K on (16 rows over 16 experts, 4096 x 4096
+// bf16: 64 columns 65.1, 32 62.1, 16 54.1; 64 over 64, 4096 x 2048: 108.9, 100.3, 110.3; but 64 rows over 8: 48.8, 52.3, 51.4).
 template <int DT, int SC, int MT>
 int skinny_columns(const GroupArgs& g, hipStream_t s) {
   const long long tiles_m = group_tile_bound(g.rows, g.experts, g.offsets != nullptr, 16 * MT);
-  if (tiles_m * ((g.cols + 63) / 64) > 512) return launch_skinny<SkinnyCfg<DT, SC, MT, 4, 4, 1>>(g, tiles_m, s);
+  const long long busy = g.experts < g.rows ? g.experts : g.rows;
+  const bool narrow = DT != kFp8 && g.rows <= 4 * busy;
+  if (!narrow && tiles_m * ((g.cols + 63) / 64) > 512) return launch_skinny<SkinnyCfg<DT, SC, MT, 4, 4, 1>>(g, tiles_m, s);
   if constexpr (MT == 1)
-    if (tiles_m * ((g.cols + 31) / 32) < 256) return launch_skinny<SkinnyCfg<DT, SC, 1, 1, 8, 1>>(g, tiles_m, s);
+    if ((narrow && g.red >= 4096) || tiles_m * ((g.cols + 31) / 32) < 256)
+      return launch_skinny<SkinnyCfg<DT, SC, 1, 1, 8, 1>>(g, tiles_m, s);
   return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1>>(g, tiles_m, s);
 }
 

@@ -132,6 +132,7 @@ def test_fp8(cuda_device, m, n, k, scale_dtype):
 # cases for each smaller tile shape in each direction, for parts of the largest tiles on an idle card, and for many groups
 # of a few rows: (sizes, N, K)
 MIDDLE = [([64, 70, 0, 130] * 8, 1992, 256), ([64, 70, 0, 130] * 8, 256, 1992), ([8, 12, 0, 9] * 16, 640, 320),
+          ([2, 1, 0, 3], 200, 4104), ([1, 0, 2] * 25, 2056, 136),
           ([1800], 4096, 200), ([900, 850], 200, 4100), ([1500, 1536], 1400, 264),
           ([40, 30, 0, 50] * 8, 2048, 256), ([100] * 16, 2000, 320), ([300, 200, 10, 0], 1000, 1000), ([2000], 264, 520),
           ([20] * 60, 1288, 200), ([500, 490], 1792, 136)]
