@@ -12,7 +12,8 @@ the rows that exist; offsets that decrease give unspecified rows, never an acces
 
 Rows that no expert owns (before ``offsets[0]``, from ``offsets[E]`` on: a batch's padding) are left as they are
 in an ``out`` that the caller gives, and are zeros in one that is allocated here. Operands may have any row
-stride; only the last dimension has to be contiguous.
+stride; only the last dimension has to be contiguous. Operands whose rows do not lie on 16 bytes are copied into a
+workspace of the call first (up to 20 rows an expert read them in place).
 """
 
 from __future__ import annotations
