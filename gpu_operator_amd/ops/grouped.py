@@ -119,12 +119,10 @@ def _launch_packed(device, what: str, args: bytes, stream: int) -> None:
     lib = _lib.load_group()
     need = lib.amdgo_group_workspace(args)
     if need < 0:
-        raise ValueError(f"{what}: operands too large to be laid out anew")
+        raise ValueError(f"{what}: 256 rows of an operand or of its scales reach over 2 GiB")
     with torch.cuda.device(device):
         space = torch.empty(need, dtype=torch.uint8, device=device)
         err = lib.amdgo_gemm_group_packed(args, space.data_ptr(), stream)
-    if err == _lib.NEEDS_PACKING:
-        raise ValueError(f"{what}: the scales' strides reach over 2 GiB")
     _lib.check(err, what)
 
 

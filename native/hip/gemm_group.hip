@@ -113,9 +113,7 @@ struct PackPlan {
     if (g.mode != kModeWgrad) g.red = (int)full;
     g.padded = 1;
   }
-  bool fits() const {
-    return g.red >= 0 && a.blocks() + b.blocks() <= 0x7fffffffll && a.to_ld * 256 < 0x7fffffffll && b.to_ld * 256 < 0x7fffffffll;
-  }
+  bool fits() const { return g.red >= 0 && a.blocks() + b.blocks() <= 0x7fffffffll && offsets_fit(g); }
   int launch(char* space, hipStream_t s) {
     for (PackMatrix* m : {&a, &b}) m->to = space + (uintptr_t)m->to;
     if (a.blocks()) g.a = a.to;
@@ -253,8 +251,11 @@ GroupArgs group_args(const void* args) {
   return g;
 }
 
+constexpr int kMostExtent = 0x7fffffff - 4096;                // (a tile's own indices may go past the end)
+
 bool valid(const GroupArgs& g) {
   if (g.rows < 0 || g.cols < 0 || g.red < 0 || g.experts < 1) return false;
+  if (g.rows > kMostExtent || g.cols > kMostExtent || g.red > kMostExtent) return false;
   if (g.dtype == kFp8) return g.mode == kModeForward && (g.scale == kScaleF32 || g.scale == kScaleE8);
   return (g.dtype == kBf16 || g.dtype == kFp16) && g.scale == kScaleNone && g.mode >= kModeForward && g.mode <= kModeWgrad;
 }
@@ -276,7 +277,7 @@ int amdgo_gemm_group(const void* args, hipStream_t s) {
   return valid(g) ? dispatch(g, s) : (int)hipErrorInvalidValue;
 }
 
-// Bytes of the workspace that amdgo_gemm_group_packed needs; negative: an argument is invalid.
+// Bytes of the workspace that amdgo_gemm_group_packed needs; negative: an argument is invalid, or no copy would do.
 long long amdgo_group_workspace(const void* args) {
   if (!args || !valid(group_args(args))) return -1;
   const PackPlan plan(group_args(args));

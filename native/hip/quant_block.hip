@@ -295,6 +295,7 @@ extern "C" int amdgo_quantize_fp8_block(const QuantArgs* args, hipStream_t s) {
   if (!args) return (int)hipErrorInvalidValue;
   const QuantArgs& a = *args;
   if (a.batches < 0 || a.rows < 0 || a.cols < 0 || (a.block_rows != 1 && a.block_rows != 128)) return (int)hipErrorInvalidValue;
+  if (a.rows > 0x7fffffff - 4096 || a.cols > 0x7fffffff - 4096) return (int)hipErrorInvalidValue;      // (indices go past the end)
   if (a.batches == 0 || a.rows == 0 || a.cols == 0) return 0;
   switch (a.dtype) {
     case kInBf16: return a.e8 ? launch_quant<kInBf16, true>(a, s) : launch_quant<kInBf16, false>(a, s);

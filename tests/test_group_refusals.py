@@ -124,8 +124,8 @@ def test_workspace_of_unaligned_operands():
         pytest.skip("the library is not built")
     lib = _lib.load_group()
 
-    def need(mode, rows, cols, red, experts, lda, ldb, b_expert, dtype=0, scale=0, a=1 << 20, b=1 << 21):
-        return lib.amdgo_group_workspace(_lib.pack_group(a, b, 1 << 22, 0, 0, 1 << 23, lda, ldb, cols, b_expert, 0, 0, 0, 0, 0, 0,
+    def need(mode, rows, cols, red, experts, lda, ldb, b_expert, dtype=0, scale=0, a=1 << 20, b=1 << 21, rows_apart=0):
+        return lib.amdgo_group_workspace(_lib.pack_group(a, b, 1 << 22, 0, 0, 1 << 23, lda, ldb, cols, b_expert, 0, rows_apart, 0, 0, 0, 0,
                                                          rows, cols, red, experts, mode, dtype, scale, 0, 0))
 
     assert need(0, 10, 20, 64, 3, 64, 64, 20 * 64) == 0
@@ -138,5 +138,7 @@ def test_workspace_of_unaligned_operands():
     assert need(0, 10, 20, 64, 0, 64, 64, 0) < 0 and need(3, 10, 20, 64, 3, 64, 64, 0) < 0
     assert need(0, 10, 20, 64, 3, 64, 64, 0, dtype=2) < 0 and need(0, 10, 20, 64, 3, 64, 64, 0, scale=1) < 0
     assert need(0, -1, 20, 64, 3, 64, 64, 0) < 0
+    assert need(0, 10, 20, 64, 3, 65, 64, 20 * 64, rows_apart=1 << 30, dtype=2, scale=1) < 0   # scales' rows too far apart
+    assert need(0, 10, 2 ** 31 - 1, 64, 1, 64, 64, 0) < 0                           # indices past 32 bits
     assert need(0, 10, 20, 2 ** 31 - 1, 3, 2 ** 31 - 1, 2 ** 31 - 1, 0) < 0         # rows too long for a copy
     assert need(0, 2 ** 31 - 1, 2 ** 31 - 1, 63, 2 ** 20, 63, 63, 63) < 0           # too many of them
