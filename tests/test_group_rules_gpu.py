@@ -1,3 +1,5 @@
+"""What the grouped and block-scaled products promise beside their formulas."""
+
 
 import pytest
 import torch
