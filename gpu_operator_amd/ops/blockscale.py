@@ -71,6 +71,7 @@ def _result(out, name, shape, dtype, like):
     _matrix(out, name, len(shape), (dtype,), like.device)
     if out.shape != shape or not out.is_contiguous():
         raise ValueError(f"{name} must be contiguous {shape}, got {tuple(out.shape)}")
+    torch.autograd.graph.increment_version(out)       # autograd does not see the kernels' writes
     return out
 
 

@@ -71,6 +71,7 @@ def _out(out, shape, dtype, device):
             raise ValueError(f"out's rows overlap: strides {strides}")
         if len(shape) == 3 and shape[0] > 1 and strides[0] < (shape[1] - 1) * ld + shape[2]:
             raise ValueError(f"out's matrices overlap: strides {strides}")
+    torch.autograd.graph.increment_version(out)       # autograd does not see the kernels' writes
     return out, ld, 0
 
 

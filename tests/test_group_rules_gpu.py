@@ -1,6 +1,5 @@
 """What the grouped and block-scaled products promise beside their formulas."""
 
-
 import pytest
 import torch
 
@@ -65,3 +64,56 @@ def test_a_small_product_beside_ones_that_cancel(cuda_device, m):
 
     assert (product(8.0, 2) == 8.0).all() and (product(4.0, 2) == 0.0).all()
     assert (product(2.0 ** -8, 8) == 2.0 ** -8).all()
+
+
+def _calls(dev, dtype=torch.bfloat16):
+    """name, a call with or without `out`, the operands it differentiates, for every entry point that takes an `out`."""
+    from gpu_operator_amd.ops import blockscale as B
+    from gpu_operator_amd.ops import grouped as G
+
+    off = H.offsets_of([7, 0, 33], 0, dev)
+    a, bt, dc = _rand(dev, 1, dtype, 40, 64), _rand(dev, 2, dtype, 3, 48, 64, scale=0.1), _rand(dev, 3, dtype, 40, 48)
+    qa, sa = B.quantize_fp8_block(a)
+    qb, sb = B.quantize_fp8_block(bt, 128)
+    return {
+        "gemm_grouped": (lambda out, a, bt: G.gemm_grouped(a, bt, off, out), [a, bt]),
+        "gemm_grouped_dgrad": (lambda out, dc, bt: G.gemm_grouped_dgrad(dc, bt, off, out), [dc, bt]),
+        "gemm_grouped_wgrad": (lambda out, dc, a: G.gemm_grouped_wgrad(dc, a, off, out), [dc, a]),
+        "gemm_fp8_block": (lambda out, a, sa, b, sb: B.gemm_fp8_block(a, sa, b, sb, out), [qa, sa, qb[0], sb[0]]),
+        "gemm_grouped_fp8_block": (lambda out, a, sa, b, sb: B.gemm_grouped_fp8_block(a, sa, b, sb, off, out), [qa, sa, qb, sb]),
+        "quantize_fp8_block": (lambda out, x: B.quantize_fp8_block(x, out=out)[0], [a]),
+    }
+
+
+NAMES = ["gemm_grouped", "gemm_grouped_dgrad", "gemm_grouped_wgrad", "gemm_fp8_block", "gemm_grouped_fp8_block", "quantize_fp8_block"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_an_output_of_the_callers_counts_as_written(cuda_device, name):
+    """Autograd has to know that its memory changed: a tensor saved for a backward pass may not be overwritten unnoticed."""
+    call, ops = _calls(cuda_device)[name]
+    out = torch.empty_like(call(None, *ops))
+    before = out._version
+    call(out, *ops)
+    assert out._version > before
+    with torch.inference_mode():
+        call(torch.empty_like(out), *ops)               # (has no version)
+
+
+def test_a_saved_tensor_is_not_overwritten_unnoticed(cuda_device):
+    from gpu_operator_amd.ops import blockscale as B
+
+    call, ops = _calls(cuda_device)["gemm_grouped"]
+    out = call(None, *ops)
+    w = torch.ones_like(out).requires_grad_(True)
+    loss = (out * w).float().sum()                      # saves out
+    call(out, *ops)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    x = _rand(cuda_device, 4, torch.bfloat16, 5, 300)
+    s = torch.ones((5, 3), device=cuda_device)
+    w = torch.ones_like(s).requires_grad_(True)
+    loss = (s * w).sum()
+    B.quantize_fp8_block(x, scale_out=s)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
