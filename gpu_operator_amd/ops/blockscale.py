@@ -15,6 +15,9 @@ product under ``2**(E - 13)`` is cut off, toward zero. That is at most ``7 * 2**
 a sum of 2048 products of normal values is off by 2e-5 of its size, where its rounding to bf16 takes 1.7e-3. A small
 product next to large ones that cancel is lost. Products of bf16 operands (:mod:`.grouped`) are exact in fp32.
 
+None of the three has a gradient: a backward pass that reaches their results raises (training goes through
+:func:`gpu_operator_amd.ops.grouped.grouped_linear`). An ``out`` is refused where an operand needs a gradient.
+
 With float32 scales each block's sum is formed first and then weighted with the product of its two scales (a float32:
 scales whose product leaves float32's range are not supported).
 """
@@ -22,7 +25,7 @@ scales whose product leaves float32's range are not supported).
 from __future__ import annotations
 
 from . import _lib
-from .grouped import MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, _stride, launch
+from .grouped import MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, _stride, launch, recorded, without_gradient
 
 BLOCK = 128
 
@@ -52,6 +55,8 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
         raise TypeError(f"scale_dtype must be torch.float32 or torch.float8_e8m0fnu, got {scale_dtype}")
     rows, cols = shape[-2:]
     scale_shape = (*shape[:-2], rows if block_rows == 1 else _blocks(rows), _blocks(cols))
+    if recorded("quantize_fp8_block", (out, scale_out), (x,)):
+        return without_gradient("quantize_fp8_block", lambda: quantize_fp8_block(x, block_rows, scale_dtype=scale_dtype), x)
     q = _result(out, "out", shape, torch.float8_e4m3fn, x)
     s = _result(scale_out, "scale_out", scale_shape, scale_dtype, x)
     if x.numel():
@@ -104,6 +109,9 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
     _scale(bt_scale, "bt_scale", (*shape_b[:-2], _blocks(n), _blocks(k)), (a_scale.dtype,), device)
     if offsets is not None:
         _offsets(offsets, e, device)
+    what = "gemm_fp8_block" if offsets is None else "gemm_grouped_fp8_block"
+    if recorded(what, (out,), (a, a_scale, bt, bt_scale)):
+        return without_gradient(what, lambda: _product(a, a_scale, bt, bt_scale, offsets, None), a, a_scale, bt, bt_scale)
     out, ldc, rest = _out(out, (m, n), torch.bfloat16, device)
     rest = 0 if offsets is None else rest
     if m and n:

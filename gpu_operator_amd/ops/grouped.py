@@ -11,7 +11,14 @@ the rows that exist; offsets that decrease give unspecified rows, never an acces
 * :func:`grouped_linear`      the product with both gradients under autograd.
 
 Rows that no expert owns (before ``offsets[0]``, from ``offsets[E]`` on: a batch's padding) are left as they are
-in an ``out`` that the caller gives, and are zeros in one that is allocated here. Operands may have any row
+in an ``out`` that the caller gives, and are zeros in one that is allocated here.
+
+Autograd records :func:`grouped_linear`, and :func:`gemm_grouped` where an operand needs a gradient. The two gradients
+have none themselves: a backward pass that reaches their results raises. A call with an ``out`` cannot be recorded and
+is refused where an operand needs a gradient, as are forward-mode gradients. ``torch.func`` transforms and tracing end in
+torch's own errors, since the kernels take addresses.
+
+Operands may have any row
 stride; only the last dimension has to be contiguous. Operands whose rows do not lie on 16 bytes are copied into a
 workspace of the call first (up to 20 rows an expert read them in place).
 """
@@ -86,6 +93,63 @@ def _offsets(offsets, experts: int, device) -> None:
         raise ValueError(f"offsets are on {offsets.device}, the operands on {device}")
 
 
+_FORWARD_AD = None
+
+
+def recorded(what: str, outs, operands) -> bool:
+    """Whether autograd has to record this call. One with an output of the caller's (`outs`: those or None) cannot be, and is
+    refused as torch's own are; so are forward-mode gradients, which would be lost."""
+    global _FORWARD_AD
+    if _FORWARD_AD is None:                  # (a call's own import of it takes 0.2 us)
+        import torch.autograd.forward_ad as _FORWARD_AD
+    if _FORWARD_AD._current_level >= 0:
+        for t in operands:
+            if _FORWARD_AD.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode gradient")
+    for t in operands:
+        if t.requires_grad:
+            break
+    else:
+        for t in outs:
+            if t is not None and getattr(t, "requires_grad", False):
+                break
+        else:
+            return False
+    import torch
+
+    if not torch.is_grad_enabled():
+        return False
+    if any(t is not None for t in outs):
+        raise RuntimeError(f"{what}: functions with out=... don't support automatic differentiation, but one of the "
+                           "arguments requires grad (detach it, or call under torch.no_grad())")
+    return True
+
+
+_NO_GRADIENT = None
+
+
+def without_gradient(what: str, call, *operands):
+    """The results of call() as ones that depend on `operands`: a backward pass that reaches them says that there is no
+    gradient, instead of going on without one."""
+    global _NO_GRADIENT
+    if _NO_GRADIENT is None:
+        import torch
+
+        class NoGradient(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, what, call, *operands):
+                ctx.set_materialize_grads(False)
+                ctx.what = what
+                return call()
+
+            @staticmethod
+            def backward(ctx, *grads):
+                raise RuntimeError(f"{ctx.what} has no gradient: detach its operands, or call it under torch.no_grad()")
+
+        _NO_GRADIENT = NoGradient
+    return _NO_GRADIENT.apply(what, call, *operands)
+
+
 def _shape(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)
@@ -140,7 +204,8 @@ def _halves():
 
 
 def gemm_grouped(a, bt, offsets, out=None):
-    """``out[t] = a[t] @ bt[e(t)].T``. ``a``: [T,K], ``bt``: [E,N,K], bf16 or fp16; ``out``: [T,N] of their type."""
+    """``out[t] = a[t] @ bt[e(t)].T``. ``a``: [T,K], ``bt``: [E,N,K], bf16 or fp16; ``out``: [T,N] of their type.
+    Where ``a`` or ``bt`` needs a gradient this is :func:`grouped_linear`."""
     sa = _matrix(a, "a", 2, _halves())
     device, dtype = a.device, a.dtype
     sb = _matrix(bt, "bt", 3, (dtype,), device)
@@ -149,6 +214,8 @@ def gemm_grouped(a, bt, offsets, out=None):
         raise ValueError(f"a is [{t},{k}], bt is [{e},{n},{kb}]: their last dimensions differ")
     _shape(e >= 1, "bt has no experts")
     _offsets(offsets, e, device)
+    if recorded("gemm_grouped", (out,), (a, bt)):
+        return grouped_linear(a, bt, offsets)
     out, ldc, rest = _out(out, (t, n), dtype, device)
     if t and n:
         launch(device, "amdgo_gemm_group", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
@@ -168,6 +235,8 @@ def gemm_grouped_dgrad(dc, bt, offsets, out=None):
         raise ValueError(f"dc is [{t},{n}], bt is [{e},{nb},{k}]: the middle dimension of bt is not dc's last")
     _shape(e >= 1, "bt has no experts")
     _offsets(offsets, e, device)
+    if recorded("gemm_grouped_dgrad", (out,), (dc, bt)):
+        return without_gradient("gemm_grouped_dgrad", lambda: gemm_grouped_dgrad(dc, bt, offsets), dc, bt)
     out, ldc, rest = _out(out, (t, k), dtype, device)
     if t and k:
         launch(device, "amdgo_gemm_group(dgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
@@ -191,6 +260,8 @@ def gemm_grouped_wgrad(dc, a, offsets, out=None):
     _shape(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.shape[0] >= 2, "offsets must be [E + 1]")
     e = offsets.shape[0] - 1
     _offsets(offsets, e, device)
+    if recorded("gemm_grouped_wgrad", (out,), (dc, a)):
+        return without_gradient("gemm_grouped_wgrad", lambda: gemm_grouped_wgrad(dc, a, offsets), dc, a)
     out, ldc, _ = _out(out, (e, n, k), dtype, device)
     if n and k:
         launch(device, "amdgo_gemm_group(wgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
@@ -235,5 +306,6 @@ def _function():
 
 
 def grouped_linear(a, bt, offsets):
-    """:func:`gemm_grouped` under autograd: gradients for ``a`` (zeros in rows that no expert owns) and ``bt``."""
+    """:func:`gemm_grouped` under autograd: gradients for ``a`` (zeros in rows that no expert owns) and ``bt``. A gradient of
+    the gradients is refused."""
     return _function().apply(a, bt, offsets)

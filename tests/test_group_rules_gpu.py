@@ -117,3 +117,74 @@ def test_a_saved_tensor_is_not_overwritten_unnoticed(cuda_device):
     B.quantize_fp8_block(x, scale_out=s)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_no_gradient_is_lost_in_silence(cuda_device, name):
+    """Operands that need a gradient: gemm_grouped has one, the others' results say at their backward that they have none; an
+    `out` cannot be recorded and is refused, as torch's own are. Without gradients to record everything is as ever."""
+    call, ops = _calls(cuda_device)[name]
+    want = call(None, *ops)
+    assert not want.requires_grad
+    for i in range(len(ops)):
+        need = [t.detach().clone().requires_grad_(True) if j == i else t for j, t in enumerate(ops)]
+        got = call(None, *need)
+        assert got.requires_grad and torch.equal(got.detach().view(torch.uint8), want.view(torch.uint8))
+        if name == "gemm_grouped":
+            assert torch.autograd.grad(got.float().sum(), need[i])[0].shape == need[i].shape
+        else:
+            with pytest.raises(RuntimeError, match="no gradient"):
+                got.float().sum().backward()
+        with pytest.raises(RuntimeError, match="automatic differentiation"):
+            call(torch.empty_like(want), *need)
+        with torch.no_grad():
+            out = torch.empty_like(want)
+            call(out, *need)
+            assert not call(None, *need).requires_grad
+        assert torch.equal(out.view(torch.uint8), want.view(torch.uint8))
+    with pytest.raises(RuntimeError, match="automatic differentiation"):
+        call(torch.empty_like(want).requires_grad_(True), *ops)
+
+
+def test_gemm_grouped_gives_grouped_linears_gradients(cuda_device):
+    from gpu_operator_amd.ops import grouped as G
+
+    off = H.offsets_of([7, 0, 33], 0, cuda_device)
+    a = _rand(cuda_device, 1, torch.bfloat16, 43, 64).requires_grad_(True)
+    bt = _rand(cuda_device, 2, torch.bfloat16, 3, 48, 64, scale=0.1).requires_grad_(True)
+    dc = _rand(cuda_device, 3, torch.bfloat16, 43, 48)
+    one, two = G.gemm_grouped(a, bt, off), G.grouped_linear(a, bt, off)
+    assert torch.equal(one, two)
+    for x, y in zip(torch.autograd.grad(one, (a, bt), dc), torch.autograd.grad(two, (a, bt), dc)):
+        assert torch.equal(x, y)
+    ref, mag = H.dgrad64(dc, bt.detach(), off)
+    H.check(torch.autograd.grad(G.gemm_grouped(a, bt, off), a, dc)[0], ref, mag, 48)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(cuda_device, name):
+    import torch.autograd.forward_ad as fwd
+
+    call, ops = _calls(cuda_device)[name]
+    with fwd.dual_level():
+        call(None, *ops)
+        if ops[0].dtype != torch.float8_e4m3fn:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(None, fwd.make_dual(ops[0], torch.ones_like(ops[0])), *ops[1:])
+        else:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(None, ops[0], fwd.make_dual(ops[1], torch.ones_like(ops[1])), *ops[2:])
+
+
+def test_quantisers_scale_out_is_an_output_too(cuda_device):
+    from gpu_operator_amd.ops import blockscale as B
+
+    x = _rand(cuda_device, 7, torch.bfloat16, 5, 300).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="automatic differentiation"):
+        B.quantize_fp8_block(x, scale_out=torch.empty((5, 3), device=cuda_device))
+    q, s = B.quantize_fp8_block(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        s.sum().backward()
+    q, s = B.quantize_fp8_block(x, scale_dtype=torch.float8_e8m0fnu)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        s.float().sum().backward()
