@@ -64,7 +64,7 @@ def _stride(shape, strides, dim: int) -> int:
 
 def _out(out, shape, dtype, device):
     """(tensor to write, its row stride, whether rows that no expert owns have to be cleared). The rows (and matrices)
-    of an output may be apart, but not overlap."""
+    of an output may be apart, or lie among one another, but not overlap."""
     import torch
 
     if out is None:
@@ -76,8 +76,12 @@ def _out(out, shape, dtype, device):
     if out.numel():
         if ld < shape[-1]:
             raise ValueError(f"out's rows overlap: strides {strides}")
-        if len(shape) == 3 and shape[0] > 1 and strides[0] < (shape[1] - 1) * ld + shape[2]:
-            raise ValueError(f"out's matrices overlap: strides {strides}")
+        if len(shape) == 3 and shape[0] > 1:
+            # the matrices one behind the other, or the rows of one between those of the others
+            apart = strides[0] >= (shape[1] - 1) * ld + shape[2]
+            among = strides[0] >= shape[2] and (shape[1] == 1 or ld >= (shape[0] - 1) * strides[0] + shape[2])
+            if not (apart or among):
+                raise ValueError(f"out's matrices overlap: strides {strides}")
     torch.autograd.graph.increment_version(out)       # autograd does not see the kernels' writes
     return out, ld, 0
 

@@ -188,3 +188,34 @@ def test_quantisers_scale_out_is_an_output_too(cuda_device):
     q, s = B.quantize_fp8_block(x, scale_dtype=torch.float8_e8m0fnu)
     with pytest.raises(RuntimeError, match="no gradient"):
         s.float().sum().backward()
+
+
+@pytest.mark.parametrize("e,n,k", [(3, 48, 64), (3, 300, 520), (70, 260, 1032), (2, 5, 7)])
+def test_weight_gradients_to_interleaved_matrices(cuda_device, e, n, k):
+    """Experts' matrices that lie row by row among one another (an output stored [N, E, K], or with columns between):
+    they do not overlap, so they are written, and nothing between them."""
+    from gpu_operator_amd.ops import grouped as G
+
+    sizes = H.random_sizes(200, e, seed=e, empty=(1,))
+    off = H.offsets_of(sizes, 0, cuda_device)
+    dc, a = _rand(cuda_device, 5, torch.bfloat16, 200, n), _rand(cuda_device, 6, torch.bfloat16, 200, k)
+    want = G.gemm_grouped_wgrad(dc, a, off)
+    for pad in (0, 8, 3):
+        flat = torch.full((n, e, k + pad), 7.0, dtype=torch.bfloat16, device=cuda_device)
+        out = flat[..., :k].transpose(0, 1)
+        assert G.gemm_grouped_wgrad(dc, a, off, out) is out
+        assert torch.equal(out, want) and (flat[..., k:] == 7.0).all()
+
+
+def test_matrices_that_overlap_are_refused(cuda_device):
+    from gpu_operator_amd.ops import grouped as G
+
+    dc, a = torch.ones((9, 4), dtype=torch.bfloat16, device=cuda_device), torch.ones((9, 16), dtype=torch.bfloat16, device=cuda_device)
+    off = H.offsets_of([4, 5], 0, cuda_device)
+    flat = torch.zeros(1000, dtype=torch.bfloat16, device=cuda_device)
+    for strides in ((8, 16, 1), (16, 24, 1), (63, 16, 1), (0, 16, 1), (24, 32, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            G.gemm_grouped_wgrad(dc, a, off, flat.as_strided((2, 4, 16), strides))
+    for strides in ((64, 16, 1), (16, 32, 1), (20, 36, 1)):
+        out = G.gemm_grouped_wgrad(dc, a, off, flat.as_strided((2, 4, 16), strides))
+        assert (out[0] == 4.0).all() and (out[1] == 5.0).all()
