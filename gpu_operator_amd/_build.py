@@ -96,7 +96,7 @@ def _pyext_name(stem: str) -> str:
 GEMM_HEADERS = ["include/gemm_tile_common.h", "hip/gemm_bf16_kernels.h", "hip/gemm_bf16_asm_loop.h",
                 "hip/gemm_fp8_kernels.h", "hip/gemm_fp8_asm_loop.h", "hip/gemm_w4ap.h", "hip/gemm_small.h",
                 "hip/gemm_small_host.h", "hip/gemm_raster_host.h"]
-GROUP_HEADERS = ["include/gemm_tile_common.h", "hip/group_common.h", "hip/group_tile.h", "hip/group_skinny.h"]
+GROUP_HEADERS = ["include/gemm_tile_common.h", "include/memory_reach.h", "hip/group_common.h", "hip/group_tile.h", "hip/group_skinny.h"]
 LAB_HEADERS = GEMM_HEADERS + ["hip/gemm_bf16_asm_loop_lab.h", "hip/gemm_fp8_asm_loop_lab.h"]
 
 TARGETS: List[Target] = [

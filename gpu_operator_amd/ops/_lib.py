@@ -107,6 +107,7 @@ def load() -> ctypes.CDLL:
 # rows, cols, red, experts, mode, dtype, scale, zero_rest, padded
 pack_group = struct.Struct("=6Q10q9i").pack
 NEEDS_PACKING = -1           # amdgo_gemm_group's answer where it cannot read the operands in place
+MAY_SHARE = -2               # the answer where an output's memory reaches into an operand's (the _apart entries do not look)
 # QuantArgs: x, q, s; ld, batch_stride; batches, rows, cols, dtype, block_rows, e8
 pack_quant = struct.Struct("=3Q2q6i").pack
 
@@ -129,14 +130,13 @@ def load_group() -> ctypes.CDLL:
             import torch  # noqa: F401  (its HIP runtime first: see load())
 
             lib = ctypes.CDLL(str(p))
-            lib.amdgo_gemm_group.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
-            lib.amdgo_gemm_group.restype = ctypes.c_int
+            for f in ("amdgo_gemm_group", "amdgo_gemm_group_apart", "amdgo_quantize_fp8_block", "amdgo_quantize_fp8_block_apart"):
+                getattr(lib, f).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+                getattr(lib, f).restype = ctypes.c_int
             lib.amdgo_group_workspace.argtypes = [ctypes.c_char_p]
             lib.amdgo_group_workspace.restype = ctypes.c_longlong
             lib.amdgo_gemm_group_packed.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_void_p]
             lib.amdgo_gemm_group_packed.restype = ctypes.c_int
-            lib.amdgo_quantize_fp8_block.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
-            lib.amdgo_quantize_fp8_block.restype = ctypes.c_int
             _GROUP_LIB = lib
     return _GROUP_LIB
 

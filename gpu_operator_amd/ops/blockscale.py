@@ -40,7 +40,8 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
     ``block_rows``: 1 (activations) or 128 (weights). ``scale_dtype``: ``torch.float32`` (the default) or
     ``torch.float8_e8m0fnu``. The scale is ``amax / 448`` (or the least power of two not under it) over the block's
     finite values, at least 2^-126; ``q`` is the nearest e4m3 value of the exact quotient, ties to even. An infinity
-    or NaN becomes NaN. ``out`` and ``scale_out``, where given, are contiguous tensors of the results' shapes.
+    or NaN becomes NaN. ``out`` and ``scale_out``, where given, are contiguous tensors of the results' shapes, in
+    memory of their own.
     """
     import torch
 
@@ -61,7 +62,7 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
     s = _result(scale_out, "scale_out", scale_shape, scale_dtype, x)
     if x.numel():
         batched = len(shape) == 3
-        launch(x.device, "amdgo_quantize_fp8_block", _lib.load_group().amdgo_quantize_fp8_block, _lib.pack_quant,
+        launch(x.device, "amdgo_quantize_fp8_block", _lib.load_group().amdgo_quantize_fp8_block, (q, s), (x,), _lib.pack_quant,
                x.data_ptr(), q.data_ptr(), s.data_ptr(), _row_stride(shape, strides), strides[0] if batched else 0,
                shape[0] if batched else 1, rows, cols, codes[x.dtype], block_rows,
                0 if scale_dtype == torch.float32 else 1)
@@ -76,7 +77,7 @@ def _result(out, name, shape, dtype, like):
     _matrix(out, name, len(shape), (dtype,), like.device)
     if out.shape != shape or not out.is_contiguous():
         raise ValueError(f"{name} must be contiguous {shape}, got {tuple(out.shape)}")
-    torch.autograd.graph.increment_version(out)       # autograd does not see the kernels' writes
+    torch._C._increment_version((out,))       # autograd does not see the kernels' writes
     return out
 
 
@@ -116,7 +117,8 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
     rest = 0 if offsets is None else rest
     if m and n:
         ssa, ssb, ha, hb = a_scale.stride(), bt_scale.stride(), a_scale.shape, bt_scale.shape
-        launch(device, "amdgo_gemm_group(fp8)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+        launch(device, "amdgo_gemm_group(fp8)", _lib.load_group().amdgo_gemm_group, (out,), (a, a_scale, bt, bt_scale, offsets),
+               _lib.pack_group,
                a.data_ptr(), bt.data_ptr(), out.data_ptr(), a_scale.data_ptr(), bt_scale.data_ptr(),
                0 if offsets is None else offsets.data_ptr(),
                _row_stride((m, k), sa), _row_stride((n, k), sb), ldc, sb[0] if e > 1 else 0, 0,

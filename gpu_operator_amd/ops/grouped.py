@@ -11,7 +11,8 @@ the rows that exist; offsets that decrease give unspecified rows, never an acces
 * :func:`grouped_linear`      the product with both gradients under autograd.
 
 Rows that no expert owns (before ``offsets[0]``, from ``offsets[E]`` on: a batch's padding) are left as they are
-in an ``out`` that the caller gives, and are zeros in one that is allocated here.
+in an ``out`` that the caller gives, and are zeros in one that is allocated here. An ``out`` shares no memory with the
+operands (rows side by side in one buffer are none).
 
 Autograd records :func:`grouped_linear`, and :func:`gemm_grouped` where an operand needs a gradient. The two gradients
 have none themselves: a backward pass that reaches their results raises. A call with an ``out`` cannot be recorded and
@@ -62,6 +63,52 @@ def _stride(shape, strides, dim: int) -> int:
     return strides[dim] if shape[dim] > 1 else 0
 
 
+def _reach(t) -> int:
+    """Bytes from t's first to behind its last."""
+    last = 1
+    for n, s in zip(t.shape, t.stride()):
+        last += (n - 1) * s
+    return last * t.element_size()
+
+
+def _rows(t):
+    """The addresses of t's rows (of its elements, where those lie apart), sorted, and the bytes of each."""
+    import torch
+
+    size, whole = t.element_size(), t.stride(-1) == 1 or t.shape[-1] == 1
+    at = torch.tensor([t.data_ptr()], device="cpu")
+    for n, s in list(zip(t.shape, t.stride()))[: -1 if whole else None]:
+        at = (at[:, None] + torch.arange(n, device="cpu") * (s * size)).flatten()
+    return at.unique(), (t.shape[-1] if whole else 1) * size
+
+
+def _shares_memory(out, t) -> bool:
+    """Whether a byte of `out` is one of t's."""
+    import torch
+
+    begin, first = out.data_ptr(), t.data_ptr()
+    if first >= begin + _reach(out) or begin >= first + _reach(t) or not out.numel() or not t.numel():
+        return False
+    size, other = out.element_size(), t.element_size()
+    if out.dim() == t.dim() == 2 and out.stride(0) > 0 and out.stride(0) * size == t.stride(0) * other and t.stride(1) == 1:
+        pitch = out.stride(0) * size                     # rows as far apart: shared, or side by side, in every row alike
+        d = (first - begin) % pitch
+        if out.shape[1] * size <= d and d + t.shape[1] * other <= pitch:
+            return False
+    (at, width), (b, wide) = _rows(out), _rows(t)
+    i = torch.searchsorted(at, b)                        # at[i - 1] < b <= at[i]
+    after, before = at[i.clamp_max(len(at) - 1)], at[(i - 1).clamp_min(0)]
+    return bool((((i < len(at)) & (after < b + wide)) | ((i > 0) & (before + width > b))).any())
+
+
+def _refuse_shared(outs, operands) -> None:
+    """Where the library says that the outputs may share memory with the operands, or with each other."""
+    for i, out in enumerate(outs):
+        for t in (*outs[:i], *operands):
+            if t is not None and _shares_memory(out, t):
+                raise ValueError("an output shares memory with an operand or with another output")
+
+
 def _out(out, shape, dtype, device):
     """(tensor to write, its row stride, whether rows that no expert owns have to be cleared). The rows (and matrices)
     of an output may be apart, or lie among one another, but not overlap."""
@@ -82,7 +129,7 @@ def _out(out, shape, dtype, device):
             among = strides[0] >= shape[2] and (shape[1] == 1 or ld >= (shape[0] - 1) * strides[0] + shape[2])
             if not (apart or among):
                 raise ValueError(f"out's matrices overlap: strides {strides}")
-    torch.autograd.graph.increment_version(out)       # autograd does not see the kernels' writes
+    torch._C._increment_version((out,))       # autograd does not see the kernels' writes
     return out, ld, 0
 
 
@@ -159,7 +206,7 @@ def _shape(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def launch(device, what: str, entry, pack, *fields) -> None:
+def launch(device, what: str, entry, outs, operands, pack, *fields) -> None:
     """One launch on the device's current stream; `entry`: a function of the library, `pack`: its arguments' packer."""
     import torch
 
@@ -176,6 +223,10 @@ def launch(device, what: str, entry, pack, *fields) -> None:
         with torch.cuda.device(index):
             err = entry(args, stream)
     if err:
+        if err == _lib.MAY_SHARE:
+            _refuse_shared(outs, operands)
+            with torch.cuda.device(index):
+                err = getattr(_lib.load_group(), entry.__name__ + "_apart")(args, stream)
         if err == _lib.NEEDS_PACKING:
             return _launch_packed(device, what, args, stream)
         _lib.check(err, what)
@@ -222,7 +273,7 @@ def gemm_grouped(a, bt, offsets, out=None):
         return grouped_linear(a, bt, offsets)
     out, ldc, rest = _out(out, (t, n), dtype, device)
     if t and n:
-        launch(device, "amdgo_gemm_group", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+        launch(device, "amdgo_gemm_group", _lib.load_group().amdgo_gemm_group, (out,), (a, bt, offsets), _lib.pack_group,
                a.data_ptr(), bt.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
                _row_stride((t, k), sa), _row_stride((n, k), sb), ldc, _stride((e,), sb, 0), 0, 0, 0, 0, 0, 0,
                t, n, k, e, MODE_FORWARD, _dtype_code(dtype), 0, rest, 0)
@@ -243,7 +294,7 @@ def gemm_grouped_dgrad(dc, bt, offsets, out=None):
         return without_gradient("gemm_grouped_dgrad", lambda: gemm_grouped_dgrad(dc, bt, offsets), dc, bt)
     out, ldc, rest = _out(out, (t, k), dtype, device)
     if t and k:
-        launch(device, "amdgo_gemm_group(dgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+        launch(device, "amdgo_gemm_group(dgrad)", _lib.load_group().amdgo_gemm_group, (out,), (dc, bt, offsets), _lib.pack_group,
                dc.data_ptr(), bt.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
                _row_stride((t, n), sd), _row_stride((n, k), sb), ldc, _stride((e,), sb, 0), 0, 0, 0, 0, 0, 0,
                t, k, n, e, MODE_DGRAD, _dtype_code(dtype), 0, rest, 0)
@@ -268,7 +319,7 @@ def gemm_grouped_wgrad(dc, a, offsets, out=None):
         return without_gradient("gemm_grouped_wgrad", lambda: gemm_grouped_wgrad(dc, a, offsets), dc, a)
     out, ldc, _ = _out(out, (e, n, k), dtype, device)
     if n and k:
-        launch(device, "amdgo_gemm_group(wgrad)", _lib.load_group().amdgo_gemm_group, _lib.pack_group,
+        launch(device, "amdgo_gemm_group(wgrad)", _lib.load_group().amdgo_gemm_group, (out,), (dc, a, offsets), _lib.pack_group,
                dc.data_ptr(), a.data_ptr(), out.data_ptr(), 0, 0, offsets.data_ptr(),
                _row_stride((t, n), sd), _row_stride((t, k), sa), ldc, 0, out.stride(0) if e > 1 else 0, 0, 0, 0, 0, 0,
                n, k, t, e, MODE_WGRAD, _dtype_code(dtype), 0, 0, 0)

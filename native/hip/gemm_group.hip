@@ -1,6 +1,7 @@
 // Grouped (ragged by expert) and block-scaled fp8 matrix products: the dispatch and the C entry.
 // The mathematics and the modes: group_common.h. Kernels: group_tile.h, group_skinny.h.
 #include "group_skinny.h"
+#include "memory_reach.h"
 
 #include <stddef.h>
 
@@ -260,6 +261,28 @@ bool valid(const GroupArgs& g) {
   return (g.dtype == kBf16 || g.dtype == kFp16) && g.scale == kScaleNone && g.mode >= kModeForward && g.mode <= kModeWgrad;
 }
 
+// Whether c may share memory with an operand.
+bool may_share(const GroupArgs& g) {
+  const int es = g.dtype == kFp8 ? 1 : 2, ss = g.scale == kScaleF32 ? 4 : 1;
+  const bool wgrad = g.mode == kModeWgrad, b_tr = g.mode != kModeForward;
+  const long long kb = ((long long)g.red + kScaleBlock - 1) / kScaleBlock, nb = ((long long)g.cols + kScaleBlock - 1) / kScaleBlock;
+  const auto reach = [](const void* p, int size, __int128 n0, __int128 s0, __int128 n1, __int128 s1, __int128 n2, __int128 s2) {
+    return MemoryReach(p, n0 <= 0 || n1 <= 0 || n2 <= 0, (n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2, size);
+  };
+  const MemoryReach c = reach(g.c, 2, wgrad ? g.experts : 1, g.c_expert, g.rows, g.ldc, g.cols, 1);
+  const long long a_rows = wgrad ? g.red : g.rows, a_cols = wgrad ? g.rows : g.red;
+  if (c.meets(reach(g.a, es, 1, 0, a_rows, g.lda, a_cols, 1))) {
+    // side by side in rows of one pitch, none of them shared
+    const __int128 pitch = (__int128)g.lda * es, d = pitch > 0 ? ((__int128)(uintptr_t)g.a - (uintptr_t)g.c) % pitch : 0;
+    const __int128 at = d < 0 ? d + pitch : d;
+    if (wgrad || pitch != (__int128)g.ldc * 2 || at < 2ll * g.cols || at + a_cols * es > pitch) return true;
+  }
+  if (c.meets(reach(g.b, es, wgrad ? 1 : g.experts, g.b_expert, b_tr ? g.red : g.cols, g.ldb, b_tr ? g.cols : g.red, 1))) return true;
+  if (g.offsets != nullptr && c.meets(reach(g.offsets, 4, 1, 0, 1, 0, (__int128)g.experts + 1, 1))) return true;
+  return g.scale != kScaleNone && (c.meets(reach(g.a_scale, ss, 1, 0, g.rows, g.as_row, kb, g.as_k)) ||
+                                   c.meets(reach(g.b_scale, ss, g.experts, g.bs_expert, nb, g.bs_row, kb, g.bs_k)));
+}
+
 int dispatch(const GroupArgs& g, hipStream_t s) {
   if (g.rows == 0 || g.cols == 0) return 0;
   if (g.dtype == kFp8) return g.scale == kScaleF32 ? dispatch_tile<kFp8, kScaleF32, false, false>(g, s)
@@ -272,6 +295,14 @@ int dispatch(const GroupArgs& g, hipStream_t s) {
 extern "C" {
 
 int amdgo_gemm_group(const void* args, hipStream_t s) {
+  if (!args) return (int)hipErrorInvalidValue;
+  const GroupArgs g = group_args(args);
+  if (!valid(g)) return (int)hipErrorInvalidValue;
+  return may_share(g) ? kMayShare : dispatch(g, s);
+}
+
+// The same where the caller knows that c shares no memory with an operand.
+int amdgo_gemm_group_apart(const void* args, hipStream_t s) {
   if (!args) return (int)hipErrorInvalidValue;
   const GroupArgs g = group_args(args);
   return valid(g) ? dispatch(g, s) : (int)hipErrorInvalidValue;

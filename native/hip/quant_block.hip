@@ -19,6 +19,7 @@
 // Bound by the memory: 2 (4) bytes read and 1 written for each element. 16384 x 8192 bf16, a scale a row's block: 70 us (5.7
 // TB/s; a large copy 5.1); 12200 x 8256 fp32, 128 x 128 blocks: 95 us (5.3 TB/s).
 #include "gemm_tile_common.h"
+#include "memory_reach.h"
 
 enum : int { kInBf16 = 0, kInFp16 = 1, kInFp32 = 2 };
 
@@ -289,14 +290,21 @@ int launch_quant(const QuantArgs& a, hipStream_t s) {
   return (int)hipGetLastError();
 }
 
-}  // namespace
+// Whether the outputs, which are contiguous, may share memory with x or with each other.
+bool may_share(const QuantArgs& a) {
+  const __int128 elements = (__int128)a.batches * a.rows * a.cols;
+  const __int128 scales = (__int128)a.batches * (((long long)a.rows + a.block_rows - 1) / a.block_rows) * (((long long)a.cols + 127) / 128);
+  const MemoryReach x(a.x, elements == 0, (__int128)(a.batches - 1) * a.batch_stride + (__int128)(a.rows - 1) * a.ld + a.cols - 1,
+                      a.dtype == kInFp32 ? 4 : 2);
+  const MemoryReach q(a.q, elements == 0, elements - 1, 1), s(a.s, elements == 0, scales - 1, a.e8 ? 1 : 4);
+  return q.meets(x) || s.meets(x) || q.meets(s);
+}
 
-extern "C" int amdgo_quantize_fp8_block(const QuantArgs* args, hipStream_t s) {
-  if (!args) return (int)hipErrorInvalidValue;
-  const QuantArgs& a = *args;
+int quantize(const QuantArgs& a, bool look, hipStream_t s) {
   if (a.batches < 0 || a.rows < 0 || a.cols < 0 || (a.block_rows != 1 && a.block_rows != 128)) return (int)hipErrorInvalidValue;
   if (a.rows > 0x7fffffff - 4096 || a.cols > 0x7fffffff - 4096) return (int)hipErrorInvalidValue;      // (indices go past the end)
   if (a.batches == 0 || a.rows == 0 || a.cols == 0) return 0;
+  if (look && may_share(a)) return kMayShare;
   switch (a.dtype) {
     case kInBf16: return a.e8 ? launch_quant<kInBf16, true>(a, s) : launch_quant<kInBf16, false>(a, s);
     case kInFp16: return a.e8 ? launch_quant<kInFp16, true>(a, s) : launch_quant<kInFp16, false>(a, s);
@@ -304,3 +312,16 @@ extern "C" int amdgo_quantize_fp8_block(const QuantArgs* args, hipStream_t s) {
   }
   return (int)hipErrorInvalidValue;
 }
+
+}  // namespace
+
+extern "C" {
+
+int amdgo_quantize_fp8_block(const QuantArgs* args, hipStream_t s) { return args ? quantize(*args, true, s) : (int)hipErrorInvalidValue; }
+
+// The same where the caller knows that the outputs share no memory with x or with each other.
+int amdgo_quantize_fp8_block_apart(const QuantArgs* args, hipStream_t s) {
+  return args ? quantize(*args, false, s) : (int)hipErrorInvalidValue;
+}
+
+}  // extern "C"

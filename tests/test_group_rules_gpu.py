@@ -219,3 +219,28 @@ def test_matrices_that_overlap_are_refused(cuda_device):
     for strides in ((64, 16, 1), (16, 32, 1), (20, 36, 1)):
         out = G.gemm_grouped_wgrad(dc, a, off, flat.as_strided((2, 4, 16), strides))
         assert (out[0] == 4.0).all() and (out[1] == 5.0).all()
+
+
+def test_outputs_that_share_memory_with_an_operand_are_refused(cuda_device):
+    """A workgroup would read what another has written. (Rows side by side in one buffer share none.)"""
+    from gpu_operator_amd.ops import blockscale as B
+    from gpu_operator_amd.ops import grouped as G
+
+    off = H.offsets_of([16, 24], 0, cuda_device)
+    a, bt = _rand(cuda_device, 1, torch.bfloat16, 40, 64), _rand(cuda_device, 2, torch.bfloat16, 2, 64, 64)
+    q, s = B.quantize_fp8_block(a)
+    qb, sb = B.quantize_fp8_block(bt, 128)
+    whole = torch.zeros(40 * 64 * 4, dtype=torch.uint8, device=cuda_device)
+    x = whole[: 40 * 64 * 2].view(torch.bfloat16).view(40, 64)
+    for call in (lambda: G.gemm_grouped(a, bt, off, a), lambda: G.gemm_grouped(a, bt, off, bt.view(-1, 64)[30:70]),
+                 lambda: G.gemm_grouped_dgrad(a, bt, off, a), lambda: G.gemm_grouped_wgrad(a, bt[0, :40], off, bt),
+                 lambda: B.gemm_fp8_block(q, s, qb[0], whole[:4].view(torch.float32).view(1, 1), x),
+                 lambda: B.gemm_grouped_fp8_block(q, whole[: 40 * 4].view(torch.float32).view(40, 1), qb, sb, off, x),
+                 lambda: B.quantize_fp8_block(x, out=whole[64 : 64 + 40 * 64].view(torch.float8_e4m3fn).view(40, 64)),
+                 lambda: B.quantize_fp8_block(a, out=whole[: 40 * 64].view(torch.float8_e4m3fn).view(40, 64),
+                                              scale_out=whole[: 160].view(torch.float32).view(40, 1))):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    both = torch.zeros((40, 128), dtype=torch.bfloat16, device=cuda_device)
+    both[:, :64] = a
+    assert torch.equal(G.gemm_grouped(both[:, :64], bt, off, both[:, 64:]), G.gemm_grouped(a, bt, off))
