@@ -25,7 +25,8 @@ scales whose product leaves float32's range are not supported).
 from __future__ import annotations
 
 from . import _lib
-from .grouped import MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, _stride, launch, recorded, without_gradient
+from .grouped import (MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, _stride, launch, load_torch, recorded,
+                      without_gradient)
 
 BLOCK = 128
 
@@ -43,8 +44,7 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
     or NaN becomes NaN. ``out`` and ``scale_out``, where given, are contiguous tensors of the results' shapes, in
     memory of their own.
     """
-    import torch
-
+    torch = load_torch()
     scale_dtype = scale_dtype or torch.float32
     codes = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
     _shape(isinstance(x, torch.Tensor) and x.dim() in (2, 3), "x must be a tensor of 2 or 3 dimensions")
@@ -94,8 +94,7 @@ def _scale(t, name, shape, dtypes, device) -> None:
 
 
 def _product(a, a_scale, bt, bt_scale, offsets, out):
-    import torch
-
+    torch = load_torch()
     f8 = (torch.float8_e4m3fn,)
     dims = 2 if offsets is None else 3
     sa = _matrix(a, "a", 2, f8)

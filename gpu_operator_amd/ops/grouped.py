@@ -32,6 +32,23 @@ from . import _lib
 
 MODE_FORWARD, MODE_DGRAD, MODE_WGRAD = 0, 1, 2
 
+# torch, from the first call on: the package imports without it, and looking it up in every helper took 0.4 us of a call
+torch = None
+_FORWARD_AD = None
+_HALVES = ()
+
+
+def load_torch():
+    """torch, also for this module's helpers. Every entry point calls it before them."""
+    global torch, _FORWARD_AD, _HALVES
+    if torch is None:
+        import torch as module
+        import torch.autograd.forward_ad as _FORWARD_AD
+
+        _HALVES = (module.bfloat16, module.float16)
+        torch = module
+    return torch
+
 
 def _matrix(t, name: str, dims: int, dtypes, device=None):
     """A GPU tensor of `dims` dimensions whose last one is contiguous; its strides."""
@@ -73,8 +90,6 @@ def _reach(t) -> int:
 
 def _rows(t):
     """The addresses of t's rows (of its elements, where those lie apart), sorted, and the bytes of each."""
-    import torch
-
     size, whole = t.element_size(), t.stride(-1) == 1 or t.shape[-1] == 1
     at = torch.tensor([t.data_ptr()], device="cpu")
     for n, s in list(zip(t.shape, t.stride()))[: -1 if whole else None]:
@@ -84,8 +99,7 @@ def _rows(t):
 
 def _shares_memory(out, t) -> bool:
     """Whether a byte of `out` is one of t's."""
-    import torch
-
+    load_torch()
     begin, first = out.data_ptr(), t.data_ptr()
     if first >= begin + _reach(out) or begin >= first + _reach(t) or not out.numel() or not t.numel():
         return False
@@ -112,8 +126,6 @@ def _refuse_shared(outs, operands) -> None:
 def _out(out, shape, dtype, device):
     """(tensor to write, its row stride, whether rows that no expert owns have to be cleared). The rows (and matrices)
     of an output may be apart, or lie among one another, but not overlap."""
-    import torch
-
     if out is None:
         return torch.empty(shape, dtype=dtype, device=device), shape[-1], 1
     strides = _matrix(out, "out", len(shape), (dtype,), device)
@@ -134,8 +146,6 @@ def _out(out, shape, dtype, device):
 
 
 def _offsets(offsets, experts: int, device) -> None:
-    import torch
-
     if not isinstance(offsets, torch.Tensor) or offsets.dtype != torch.int32:
         raise TypeError("offsets must be an int32 tensor")
     if offsets.dim() != 1 or offsets.shape[0] != experts + 1 or not offsets.is_contiguous():
@@ -144,19 +154,15 @@ def _offsets(offsets, experts: int, device) -> None:
         raise ValueError(f"offsets are on {offsets.device}, the operands on {device}")
 
 
-_FORWARD_AD = None
-
-
 def recorded(what: str, outs, operands) -> bool:
     """Whether autograd has to record this call. One with an output of the caller's (`outs`: those or None) cannot be, and is
     refused as torch's own are; so are forward-mode gradients, which would be lost."""
-    global _FORWARD_AD
-    if _FORWARD_AD is None:                  # (a call's own import of it takes 0.2 us)
-        import torch.autograd.forward_ad as _FORWARD_AD
     if _FORWARD_AD._current_level >= 0:
         for t in operands:
             if _FORWARD_AD.unpack_dual(t).tangent is not None:
                 raise NotImplementedError(f"{what} has no forward-mode gradient")
+    if not torch.is_grad_enabled():
+        return False
     for t in operands:
         if t.requires_grad:
             break
@@ -166,10 +172,6 @@ def recorded(what: str, outs, operands) -> bool:
                 break
         else:
             return False
-    import torch
-
-    if not torch.is_grad_enabled():
-        return False
     if any(t is not None for t in outs):
         raise RuntimeError(f"{what}: functions with out=... don't support automatic differentiation, but one of the "
                            "arguments requires grad (detach it, or call under torch.no_grad())")
@@ -184,8 +186,6 @@ def without_gradient(what: str, call, *operands):
     gradient, instead of going on without one."""
     global _NO_GRADIENT
     if _NO_GRADIENT is None:
-        import torch
-
         class NoGradient(torch.autograd.Function):
             @staticmethod
             def forward(ctx, what, call, *operands):
@@ -208,8 +208,6 @@ def _shape(ok: bool, what: str) -> None:
 
 def launch(device, what: str, entry, outs, operands, pack, *fields) -> None:
     """One launch on the device's current stream; `entry`: a function of the library, `pack`: its arguments' packer."""
-    import torch
-
     try:
         args = pack(*fields)
     except struct.error:
@@ -234,8 +232,6 @@ def launch(device, what: str, entry, outs, operands, pack, *fields) -> None:
 
 def _launch_packed(device, what: str, args: bytes, stream: int) -> None:
     """The product on copies, in a workspace of the call, of what the kernels cannot read in place."""
-    import torch
-
     lib = _lib.load_group()
     need = lib.amdgo_group_workspace(args)
     if need < 0:
@@ -247,21 +243,14 @@ def _launch_packed(device, what: str, args: bytes, stream: int) -> None:
 
 
 def _dtype_code(dtype) -> int:
-    import torch
-
     return 0 if dtype == torch.bfloat16 else 1
-
-
-def _halves():
-    import torch
-
-    return (torch.bfloat16, torch.float16)
 
 
 def gemm_grouped(a, bt, offsets, out=None):
     """``out[t] = a[t] @ bt[e(t)].T``. ``a``: [T,K], ``bt``: [E,N,K], bf16 or fp16; ``out``: [T,N] of their type.
     Where ``a`` or ``bt`` needs a gradient this is :func:`grouped_linear`."""
-    sa = _matrix(a, "a", 2, _halves())
+    load_torch()
+    sa = _matrix(a, "a", 2, _HALVES)
     device, dtype = a.device, a.dtype
     sb = _matrix(bt, "bt", 3, (dtype,), device)
     (t, k), (e, n, kb) = a.shape, bt.shape
@@ -282,7 +271,8 @@ def gemm_grouped(a, bt, offsets, out=None):
 
 def gemm_grouped_dgrad(dc, bt, offsets, out=None):
     """The product's gradient for its rows: ``out[t] = dc[t] @ bt[e(t)]``. ``dc``: [T,N], ``bt``: [E,N,K]; ``out``: [T,K]."""
-    sd = _matrix(dc, "dc", 2, _halves())
+    load_torch()
+    sd = _matrix(dc, "dc", 2, _HALVES)
     device, dtype = dc.device, dc.dtype
     sb = _matrix(bt, "bt", 3, (dtype,), device)
     (t, n), (e, nb, k) = dc.shape, bt.shape
@@ -304,9 +294,8 @@ def gemm_grouped_dgrad(dc, bt, offsets, out=None):
 def gemm_grouped_wgrad(dc, a, offsets, out=None):
     """The product's gradient for its weights: ``out[e] = dc_e.T @ a_e`` over the rows of expert ``e`` (zeros where it
     has none). ``dc``: [T,N], ``a``: [T,K]; ``out``: [E,N,K] of their type, rounded once from the fp32 sum."""
-    import torch
-
-    sd = _matrix(dc, "dc", 2, _halves())
+    load_torch()
+    sd = _matrix(dc, "dc", 2, _HALVES)
     device, dtype = dc.device, dc.dtype
     sa = _matrix(a, "a", 2, (dtype,), device)
     (t, n), (ta, k) = dc.shape, a.shape
@@ -332,9 +321,8 @@ _FUNCTION = None
 def _function():
     """The autograd function, made at its first use (the package imports without torch)."""
     global _FUNCTION
+    load_torch()
     if _FUNCTION is None:
-        import torch
-
         def gradients(ctx, dc):
             a, bt, offsets = ctx.saved_tensors
             if dc.stride(-1) != 1:
