@@ -144,11 +144,11 @@ int skinny_columns(const GroupArgs& g, hipStream_t s) {
   const long long tiles_m = group_tile_bound(g.rows, g.experts, g.offsets != nullptr, 16 * MT);
   const long long busy = g.experts < g.rows ? g.experts : g.rows;
   const bool narrow = DT != kFp8 && g.rows <= 4 * busy;
-  if (!narrow && tiles_m * ((g.cols + 63) / 64) > 512) return launch_skinny<SkinnyCfg<DT, SC, MT, 4, 4, 1>>(g, tiles_m, s);
+  if (!narrow && tiles_m * ((g.cols + 63) / 64) > 512) return launch_skinny<SkinnyCfg<DT, SC, MT, 4, 4>>(g, tiles_m, s);
   if constexpr (MT == 1)
     if ((narrow && g.red >= 4096) || tiles_m * ((g.cols + 31) / 32) < 256)
-      return launch_skinny<SkinnyCfg<DT, SC, 1, 1, 8, 1>>(g, tiles_m, s);
-  return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1>>(g, tiles_m, s);
+      return launch_skinny<SkinnyCfg<DT, SC, 1, 1, 8>>(g, tiles_m, s);
+  return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8>>(g, tiles_m, s);
 }
 
 // The same for operands without whole aligned chunks: rows that start on 4 bytes are loaded as they lie, others in words (8192
@@ -158,8 +158,8 @@ int skinny_unaligned(const GroupArgs& g, hipStream_t s) {
   if (!offsets_fit(g)) return kNeedsPacking;
   const long long tiles_m = group_tile_bound(g.rows, g.experts, g.offsets != nullptr, 16 * MT), es = DT == kFp8 ? 1 : 2;
   if ((((uintptr_t)g.a | (uintptr_t)g.b | (uintptr_t)(g.lda * es) | (uintptr_t)(g.ldb * es) | (uintptr_t)(g.b_expert * es)) & 3) == 0)
-    return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1, 4>>(g, tiles_m, s);
-  return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1, 1>>(g, tiles_m, s);
+    return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 4>>(g, tiles_m, s);
+  return launch_skinny<SkinnyCfg<DT, SC, MT, 2, 8, 1>>(g, tiles_m, s);
 }
 
 // Few rows: the skinny kernel with tiles of 16 rows, or of 32 for a single group of 17 to 64 (8192 x 8192 fp8, 32 rows:
