@@ -244,3 +244,19 @@ def test_outputs_that_share_memory_with_an_operand_are_refused(cuda_device):
     both = torch.zeros((40, 128), dtype=torch.bfloat16, device=cuda_device)
     both[:, :64] = a
     assert torch.equal(G.gemm_grouped(both[:, :64], bt, off, both[:, 64:]), G.gemm_grouped(a, bt, off))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("e,n,k", [(70, 512, 1024), (130, 504, 1016), (200, 250, 1021)])
+def test_weight_gradients_of_more_experts_than_lanes(cuda_device, e, n, k, dtype):
+    """The largest tiles with more than 64 experts, whose order is then the experts' own: experts without rows among them, rows
+    that no expert owns around them."""
+    from gpu_operator_amd.ops import grouped as G
+
+    sizes = H.random_sizes(3000, e, seed=e, empty=range(3, e, 9))
+    a, dc = _rand(cuda_device, 8, dtype, 3020, k), _rand(cuda_device, 9, dtype, 3020, n)
+    off = H.offsets_of(sizes, 5, cuda_device)
+    for x in (a, dc):
+        x[:5], x[3005:] = float("nan"), float("inf")
+    ref, mag = H.wgrad64(dc, a, off)
+    H.check(G.gemm_grouped_wgrad(dc, a, off), ref, mag, max(sizes))
