@@ -29,6 +29,13 @@ from .grouped import (MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape
                       without_gradient)
 
 BLOCK = 128
+_INPUTS = {}
+
+
+def _inputs(torch):
+    """The types that quantize_fp8_block takes, and the kernel's names of them."""
+    _INPUTS.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
+    return _INPUTS
 
 
 def _blocks(n: int) -> int:
@@ -46,7 +53,7 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
     """
     torch = load_torch()
     scale_dtype = scale_dtype or torch.float32
-    codes = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    codes = _INPUTS or _inputs(torch)
     _shape(isinstance(x, torch.Tensor) and x.dim() in (2, 3), "x must be a tensor of 2 or 3 dimensions")
     shape = tuple(x.shape)
     strides = _matrix(x, "x", len(shape), codes)
@@ -58,8 +65,8 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
     scale_shape = (*shape[:-2], rows if block_rows == 1 else _blocks(rows), _blocks(cols))
     if recorded("quantize_fp8_block", (out, scale_out), (x,)):
         return without_gradient("quantize_fp8_block", lambda: quantize_fp8_block(x, block_rows, scale_dtype=scale_dtype), x)
-    q = _result(out, "out", shape, torch.float8_e4m3fn, x)
-    s = _result(scale_out, "scale_out", scale_shape, scale_dtype, x)
+    q = _result(torch, out, "out", shape, torch.float8_e4m3fn, x)
+    s = _result(torch, scale_out, "scale_out", scale_shape, scale_dtype, x)
     if x.numel():
         batched = len(shape) == 3
         launch(x.device, "amdgo_quantize_fp8_block", _lib.load_group().amdgo_quantize_fp8_block, (q, s), (x,), _lib.pack_quant,
@@ -69,9 +76,7 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
     return q, s
 
 
-def _result(out, name, shape, dtype, like):
-    import torch
-
+def _result(torch, out, name, shape, dtype, like):
     if out is None:
         return torch.empty(shape, dtype=dtype, device=like.device)
     _matrix(out, name, len(shape), (dtype,), like.device)
@@ -81,9 +86,7 @@ def _result(out, name, shape, dtype, like):
     return out
 
 
-def _scale(t, name, shape, dtypes, device) -> None:
-    import torch
-
+def _scale(torch, t, name, shape, dtypes, device) -> None:
     if not isinstance(t, torch.Tensor) or t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, "
                         f"got {getattr(t, 'dtype', type(t).__name__)}")
@@ -105,8 +108,8 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
     if shape_b[-1] != k:
         raise ValueError(f"a is [{m},{k}], bt is {shape_b}: their last dimensions differ")
     _shape(e >= 1, "bt has no experts")
-    _scale(a_scale, "a_scale", (m, _blocks(k)), (torch.float32, torch.float8_e8m0fnu), device)
-    _scale(bt_scale, "bt_scale", (*shape_b[:-2], _blocks(n), _blocks(k)), (a_scale.dtype,), device)
+    _scale(torch, a_scale, "a_scale", (m, _blocks(k)), (torch.float32, torch.float8_e8m0fnu), device)
+    _scale(torch, bt_scale, "bt_scale", (*shape_b[:-2], _blocks(n), _blocks(k)), (a_scale.dtype,), device)
     if offsets is not None:
         _offsets(offsets, e, device)
     what = "gemm_fp8_block" if offsets is None else "gemm_grouped_fp8_block"
