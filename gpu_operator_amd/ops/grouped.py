@@ -19,9 +19,10 @@ have none themselves: a backward pass that reaches their results raises. A call 
 is refused where an operand needs a gradient, as are forward-mode gradients. ``torch.func`` transforms and tracing end in
 torch's own errors, since the kernels take addresses.
 
-Operands may have any row
-stride; only the last dimension has to be contiguous. Operands whose rows do not lie on 16 bytes are copied into a
-workspace of the call first (up to 20 rows an expert read them in place).
+Operands may have any row stride; only the last dimension has to be contiguous. Operands whose rows do not lie on 16
+bytes (or whose reduction does not fill 16-byte pieces) are copied into a workspace of the call first, all experts'
+weights with them, to rows of whole 128-byte lines: it is about as large as those operands. Only the forward product of
+up to 20 rows an expert reads them in place.
 """
 
 from __future__ import annotations

@@ -166,7 +166,9 @@ int skinny_unaligned(const GroupArgs& g, hipStream_t s) {
 // 16-row tiles 30 us, 32-row ones 22.5; 64 rows of 4096 x 4096: 15.6, 12.2). Groups of more than 12 rows on average
 // are for the tiled kernel (16 of 16 rows, 4096 x 2048: 65.5 us, Low 60.4; 64 of 8 rows: 93.8, Small 110.5); of more than
 // 20 where the operands are not `ready`, since that one needs a copy of the weights then (16 of 15 rows, 2048 x 1537 bf16:
-// 42.9, 59.1; of 25: 58.4, 59.5; fp8 29.8, 33.6 and 40.0, 34.4). 0: not here.
+// 42.9, 59.1; of 25: 58.4, 59.5; fp8 29.8, 33.6 and 40.0, 34.4). The offsets are on the device, so the mean is all that there is
+// to go by, padding and idle experts included: 700 rows over 64 experts of 4096 x 2048 bf16 take 208 us evenly and 103 where one
+// expert has all of them, which as a product of one expert's take 21 (fp8: 109, 63, 14). 0: not here.
 int skinny_rows(const GroupArgs& g, bool ready) {
   if (g.mode != kModeForward) return 0;
   if (g.offsets == nullptr) return g.rows <= 16 ? 1 : g.rows <= 64 ? 2 : 0;
@@ -184,7 +186,8 @@ int skinny_rows(const GroupArgs& g, bool ready) {
 //            x 4096 fp8: 64.5, 50.6)
 //   Small    128 x 128, two a CU, so that one's prologue and epilogue run under the other's loop: one round to about
 //            two of groups that fill most of it (16 groups of 128 rows, 2048 x 2048: 41.3 us, Low 47.5, Deep 44.9;
-//            700 x 8192 x 2048 fp8: 17.8, 23.3, 25.5; 32 groups of 94 rows, 880 tiles: 83.7, 70.6, 73.7)
+//            700 x 8192 x 2048 fp8: 17.8, 23.3, 25.5; 32 groups of 94 rows, 880 tiles: 83.7, 70.6, 73.7). Not compared between
+//            40 and 90 rows a group: 28 of 73, 1032 x 2056 fp16, take 57 us here, and their dgrad, of the same weights, 35 by Low
 //   Deep     128 x 128, 8 waves, a ring of four: most of one round, where a workgroup's own latency is the time (fp8
 //            512 x 8192 x 8192: 52.9 us, Low 59.7, Small 60.2; 16 groups of 125 rows, 1024 x 2048: 23.4, 26.2, 32.6)
 //   Low      64 x 128, a ring of three: few rows a group, or fewer tiles than that (fp8 128 x 4096 x 4096: 13.5 us,

@@ -9,8 +9,9 @@
 // 4096 x 2048 fp8 with a row each 93.7, 101.5, 144.9 (and 94.8 as a loop over panels without batches: the compiler then orders
 // the waits otherwise). The waves' partial sums are joined through LDS in wave order: the same bits every time.
 //
-// 16 rows of 8192 x 8192 fp8: 17.5 us (3.8 TB/s of weights; a large copy reads and writes 5.1); 64 rows over 64 experts of
-// 4096 x 2048 fp8, 37 of them busy: 53 us (5.9 TB/s); 8 rows over 6 busy experts of 4096 x 4096 bf16: 33.7 us (6.0 TB/s).
+// 16 rows of 8192 x 8192 fp8: 17.3 us one after the other over the same weights (3.9 TB/s of weights; a large copy reads and
+// writes 5.1), 20.3 over other weights each time, and 18.2 to 20.8 in a trace; 64 rows over 64 experts of 4096 x 2048 fp8, 37 of
+// them busy: 51 to 56 us (5.9 TB/s); 8 rows over 6 busy experts of 4096 x 4096 bf16: 33 us (6.0 TB/s).
 #pragma once
 
 #include "group_tile.h"

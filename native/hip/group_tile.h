@@ -934,9 +934,10 @@ __device__ __forceinline__ bool pp_next(const GroupArgs& g, TilePlan<C>& plan, i
 // tile's loop (a workgroup a tile: 11 us a tile between the loops, 9.4 for fp8; like this 6 and 8). What the tiles'
 // starts and ends need is kept in LDS and read there, not in registers across the loops.
 //
-// Bound by the matrix unit, which the card clocks down under it: 8192^3 fp8 444 to 500 us (2200 to 2480 TFLOP/s; each
-// further 4096 of K at 2620, e8m0 2970), bf16 of 8192 x 8192 x 4096 361 us (1520; 1630). With groups, by their last tiles: 8 of
-// 2048 rows on average, 8192 x 4096 bf16, 815 to 860 us (1350 to 1280), 26 fp8 ones of 590, 4096 x 4096, 315 to 330 (1640).
+// Bound by the matrix unit, which the card clocks down under it: 8192^3 fp8 444 to 504 us by card (2180 to 2480 TFLOP/s; 539
+// as the median of 30 from a cold start; each further 4096 of K at 2620, e8m0 2970), bf16 of 8192 x 8192 x 4096 361 us (1520; 1630).
+// With groups, by their last tiles: 8 of 2048 rows on average, 8192 x 4096 bf16, 815 to 877 us (1350 to 1250; 913 from a cold
+// start), 26 fp8 ones of 590, 4096 x 4096, 315 to 330 (1640).
 template <class C>
 __global__ void __launch_bounds__(C::THREADS) __attribute__((amdgpu_waves_per_eu(2, 2))) group_tile_pp(const GroupArgs args) {
   using P = PingPong<C>;

@@ -16,8 +16,8 @@
 // exact (many are: half of all blocks hold an x of 3/4 or 3/8 amax). Of float32 inputs the rare values within 8 units of
 // a border are compared with it exactly, in float64.
 //
-// Bound by the memory: 2 (4) bytes read and 1 written for each element. 16384 x 8192 bf16, a scale a row's block: 70 us (5.7
-// TB/s; a large copy 5.1); 12200 x 8256 fp32, 128 x 128 blocks: 95 us (5.3 TB/s).
+// Bound by the memory: 2 (4) bytes read and 1 written for each element. 16384 x 8192 bf16, a scale a row's block: 69 us (5.8
+// TB/s; a large copy 5.1), 70 to 75 as one call among others; 12200 x 8256 fp32, 128 x 128 blocks: 95 us (5.3 TB/s).
 #include "gemm_tile_common.h"
 #include "memory_reach.h"
 
@@ -91,9 +91,9 @@ constexpr unsigned int kLeastAmax = ((unsigned)(127 - 118) << 23) | 0x600000u;  
 
 struct Scale {
   float f;            // float32: the scale; e8m0: 2^e
-  int e;              // float32: amax's exponent; e8m0: e
+  int e;              // float32: amax's exponent, -118 to 127; e8m0: e, -126 to 120
   float d;            // float32: amax * 2^-e in [1, 2)
-  float m;            // float32: 448 / amax nearly; e8m0: 2^-e (a power of two more or less rounds nothing: -118 <= e <= 127)
+  float m;            // float32: 448 / amax nearly; e8m0: 2^-e (normal numbers either way, so a power of two in them rounds nothing)
 };
 
 template <bool E8>
