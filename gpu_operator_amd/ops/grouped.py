@@ -16,8 +16,8 @@ operands (rows side by side in one buffer are none).
 
 Autograd records :func:`grouped_linear`, and :func:`gemm_grouped` where an operand needs a gradient. The two gradients
 have none themselves: a backward pass that reaches their results raises. A call with an ``out`` cannot be recorded and
-is refused where an operand needs a gradient, as are forward-mode gradients. ``torch.func`` transforms and tracing end in
-torch's own errors, since the kernels take addresses.
+is refused where an operand needs a gradient, as are forward-mode gradients. ``torch.func`` transforms end in torch's own
+errors, since the kernels take addresses; ``torch.compile`` runs the calls between its graphs.
 
 Operands may have any row stride; only the last dimension has to be contiguous. Operands whose rows do not lie on 16
 bytes (or whose reduction does not fill 16-byte pieces) are copied into a workspace of the call first, all experts'
