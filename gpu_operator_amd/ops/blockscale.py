@@ -25,8 +25,8 @@ scales whose product leaves float32's range are not supported).
 from __future__ import annotations
 
 from . import _lib
-from .grouped import (MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, _stride, launch, load_torch, recorded,
-                      without_gradient)
+from .grouped import (MODE_FORWARD, _matrix, _offsets, _out, _row_stride, _shape, _stride, launch, load_torch, needs_gradient,
+                      recorded, without_gradient)
 
 BLOCK = 128
 _INPUTS = {}
@@ -63,7 +63,7 @@ def quantize_fp8_block(x, block_rows: int = 1, *, scale_dtype=None, out=None, sc
         raise TypeError(f"scale_dtype must be torch.float32 or torch.float8_e8m0fnu, got {scale_dtype}")
     rows, cols = shape[-2:]
     scale_shape = (*shape[:-2], rows if block_rows == 1 else _blocks(rows), _blocks(cols))
-    if recorded("quantize_fp8_block", (out, scale_out), (x,)):
+    if (x.requires_grad or needs_gradient(out) or needs_gradient(scale_out)) and recorded("quantize_fp8_block", out, scale_out):
         return without_gradient("quantize_fp8_block", lambda: quantize_fp8_block(x, block_rows, scale_dtype=scale_dtype), x)
     q = _result(torch, out, "out", shape, torch.float8_e4m3fn, x)
     s = _result(torch, scale_out, "scale_out", scale_shape, scale_dtype, x)
@@ -107,13 +107,15 @@ def _product(a, a_scale, bt, bt_scale, offsets, out):
     n, e = shape_b[-2], shape_b[0] if dims == 3 else 1
     if shape_b[-1] != k:
         raise ValueError(f"a is [{m},{k}], bt is {shape_b}: their last dimensions differ")
-    _shape(e >= 1, "bt has no experts")
+    if e < 1:
+        raise ValueError("bt has no experts")
     _scale(torch, a_scale, "a_scale", (m, _blocks(k)), (torch.float32, torch.float8_e8m0fnu), device)
     _scale(torch, bt_scale, "bt_scale", (*shape_b[:-2], _blocks(n), _blocks(k)), (a_scale.dtype,), device)
     if offsets is not None:
         _offsets(offsets, e, device)
-    what = "gemm_fp8_block" if offsets is None else "gemm_grouped_fp8_block"
-    if recorded(what, (out,), (a, a_scale, bt, bt_scale)):
+    what = "gemm_fp8_block" if dims == 2 else "gemm_grouped_fp8_block"
+    if (a.requires_grad or a_scale.requires_grad or bt.requires_grad or bt_scale.requires_grad or needs_gradient(out)) \
+            and recorded(what, out):
         return without_gradient(what, lambda: _product(a, a_scale, bt, bt_scale, offsets, None), a, a_scale, bt, bt_scale)
     out, ldc, rest = _out(out, (m, n), torch.bfloat16, device)
     rest = 0 if offsets is None else rest

@@ -155,24 +155,16 @@ def _offsets(offsets, experts: int, device) -> None:
         raise ValueError(f"offsets are on {offsets.device}, the operands on {device}")
 
 
-def recorded(what: str, outs, operands) -> bool:
-    """Whether autograd has to record this call. One with an output of the caller's (`outs`: those or None) cannot be, and is
-    refused as torch's own are; so are forward-mode gradients, which would be lost."""
-    if _FORWARD_AD._current_level >= 0:
-        for t in operands:
-            if _FORWARD_AD.unpack_dual(t).tangent is not None:
-                raise NotImplementedError(f"{what} has no forward-mode gradient")
+def needs_gradient(out) -> bool:
+    """Whether an output, or None, does (it may be anything yet)."""
+    return out is not None and getattr(out, "requires_grad", False)
+
+
+def recorded(what: str, *outs) -> bool:
+    """Whether autograd has to record this call, an operand or output of which needs a gradient. One with an output of the
+    caller's (`outs`: those or None) cannot be, and is refused as torch's own are. (launch() refuses forward-mode gradients.)"""
     if not torch.is_grad_enabled():
         return False
-    for t in operands:
-        if t.requires_grad:
-            break
-    else:
-        for t in outs:
-            if t is not None and getattr(t, "requires_grad", False):
-                break
-        else:
-            return False
     if any(t is not None for t in outs):
         raise RuntimeError(f"{what}: functions with out=... don't support automatic differentiation, but one of the "
                            "arguments requires grad (detach it, or call under torch.no_grad())")
@@ -213,6 +205,10 @@ def launch(device, what: str, entry, outs, operands, pack, *fields) -> None:
         args = pack(*fields)
     except struct.error:
         raise ValueError(f"{what}: a dimension over 2^31 - 1 or a stride over 2^63 - 1") from None
+    if _FORWARD_AD._current_level >= 0:
+        for t in operands:
+            if t is not None and _FORWARD_AD.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode gradient")
     # (torch.cuda.current_device() and current_stream() make a call 1.2 us longer)
     index = device.index
     stream = torch._C._cuda_getCurrentRawStream(index)
@@ -257,9 +253,10 @@ def gemm_grouped(a, bt, offsets, out=None):
     (t, k), (e, n, kb) = a.shape, bt.shape
     if kb != k:
         raise ValueError(f"a is [{t},{k}], bt is [{e},{n},{kb}]: their last dimensions differ")
-    _shape(e >= 1, "bt has no experts")
+    if e < 1:
+        raise ValueError("bt has no experts")
     _offsets(offsets, e, device)
-    if recorded("gemm_grouped", (out,), (a, bt)):
+    if (a.requires_grad or bt.requires_grad or needs_gradient(out)) and recorded("gemm_grouped", out):
         return grouped_linear(a, bt, offsets)
     out, ldc, rest = _out(out, (t, n), dtype, device)
     if t and n:
@@ -279,9 +276,10 @@ def gemm_grouped_dgrad(dc, bt, offsets, out=None):
     (t, n), (e, nb, k) = dc.shape, bt.shape
     if nb != n:
         raise ValueError(f"dc is [{t},{n}], bt is [{e},{nb},{k}]: the middle dimension of bt is not dc's last")
-    _shape(e >= 1, "bt has no experts")
+    if e < 1:
+        raise ValueError("bt has no experts")
     _offsets(offsets, e, device)
-    if recorded("gemm_grouped_dgrad", (out,), (dc, bt)):
+    if (dc.requires_grad or bt.requires_grad or needs_gradient(out)) and recorded("gemm_grouped_dgrad", out):
         return without_gradient("gemm_grouped_dgrad", lambda: gemm_grouped_dgrad(dc, bt, offsets), dc, bt)
     out, ldc, rest = _out(out, (t, k), dtype, device)
     if t and k:
@@ -305,7 +303,7 @@ def gemm_grouped_wgrad(dc, a, offsets, out=None):
     _shape(isinstance(offsets, torch.Tensor) and offsets.dim() == 1 and offsets.shape[0] >= 2, "offsets must be [E + 1]")
     e = offsets.shape[0] - 1
     _offsets(offsets, e, device)
-    if recorded("gemm_grouped_wgrad", (out,), (dc, a)):
+    if (dc.requires_grad or a.requires_grad or needs_gradient(out)) and recorded("gemm_grouped_wgrad", out):
         return without_gradient("gemm_grouped_wgrad", lambda: gemm_grouped_wgrad(dc, a, offsets), dc, a)
     out, ldc, _ = _out(out, (e, n, k), dtype, device)
     if n and k:
