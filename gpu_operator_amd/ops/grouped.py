@@ -349,5 +349,6 @@ def _function():
 
 def grouped_linear(a, bt, offsets):
     """:func:`gemm_grouped` under autograd: gradients for ``a`` (zeros in rows that no expert owns) and ``bt``. A gradient of
-    the gradients is refused."""
+    the gradients is refused. A step may be captured into a graph, forward and backward together, once the results of
+    earlier calls on the same leaves are gone (torch ends the process where such an eager graph still lives)."""
     return _function().apply(a, bt, offsets)
