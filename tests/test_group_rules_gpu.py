@@ -260,3 +260,16 @@ def test_weight_gradients_of_more_experts_than_lanes(cuda_device, e, n, k, dtype
         x[:5], x[3005:] = float("nan"), float("inf")
     ref, mag = H.wgrad64(dc, a, off)
     H.check(G.gemm_grouped_wgrad(dc, a, off), ref, mag, max(sizes))
+
+
+def test_grouped_linear_has_no_forward_mode(cuda_device):
+    import torch.autograd.forward_ad as fwd
+
+    from gpu_operator_amd.ops import grouped as G
+
+    off = H.offsets_of([7, 0, 33], 0, cuda_device)
+    a, bt = _rand(cuda_device, 1, torch.bfloat16, 40, 64), _rand(cuda_device, 2, torch.bfloat16, 3, 48, 64)
+    with fwd.dual_level():
+        for need in (False, True):
+            with pytest.raises(RuntimeError):
+                G.grouped_linear(fwd.make_dual(a, torch.ones_like(a)), bt.clone().requires_grad_(need), off)
